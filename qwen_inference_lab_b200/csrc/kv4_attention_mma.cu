@@ -1,0 +1,632 @@
+// Attention of single tokens and of a few tokens at a time over pages of 4 bits (layout: kv4.h) on mma.sync, bfloat16 queries, for one
+// head size (-DQIL_HEAD_DIM=32, 64, ..., 256).
+//
+//   out = sum_t p_t (m_t + s_t c_t),  p = softmax over the keys t in (pos - window, pos] of scale q . (m_t + s_t c_t)
+//
+// A block takes a segment's tokens x the query heads of one kv head, up to 8 NT of these rows, and a span of the context; each
+// of its four warps walks every fourth tile of 32 keys on its own: 16-byte copies into a ring of stages in shared memory, then
+//
+//   scores   S^T = K q^T, 16 keys x 8 rows x 16 dimensions a bfloat16 MMA.  A code in the lowest bits of a half word is, read as
+//            bfloat16, code 2^-133, and four bits higher code 2^-129: numbers below and in the first binade have one spacing, and an
+//            MMA takes them exactly.  So an AND makes an operand of two codes, and a shift two more; a query row carries the power of two
+//            that keeps the products normal (and 1/16 where the codes lie higher).  S += s (q . c) in float32, and one MMA more adds
+//            sum_g m_g sum(q_g), the sums as three bfloat16 parts each.  Nothing is rounded but the float32 sums.
+//   softmax  in the accumulators' layout; the maximum moves when it grew by more than 2^8 (p <= 256 until then, exact algebra)
+//   output   O^T = V^T p^T, 16 dimensions x 8 rows x 16 keys an MMA.  p is rounded to bfloat16 and transposed (movmatrix), a group's steps
+//            multiply it once more (p s rounded again), the codes go in as above and p carries the power of two (`lift`, by the
+//            largest step so far).  With two MMAs more
+//            out = sum (c - 8) (p s) + sum p (m + 8 s):
+//            counted from the middle of a group's range the second rounding acts on |c - 8| steps, about the size of the value itself;
+//            counted from its end it cost 1.5 times the error.  The sum of p comes from the same MMA as the last sum.
+//
+// What bounds it: with few blocks the chain description -> block table -> first tile, with many the instructions a tile takes (an
+// SM issues at most 2 of AND, shift and byte permutation a cycle, 0.47 MMAs).  Other operands cost more: 128 + c or 1 + c / 16 with
+// the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits: 393
+// instructions for 16 keys and values of 128 dimensions.
+//
+// The lanes' keys are permuted (row r of a tile of 8: key r / 2 + 4 (r & 1)) so that the two keys that a register of the second product
+// pairs are c and c + 4.  Every read of shared memory is free of bank conflicts.
+//
+// Keys that a row does not see are selected away among the scores.  Their values take part with weight zero, so groups of values that
+// are NaN are set to zero, and the rows that do see them are marked: their outputs of that group are NaN.
+//
+// Warps merge in shared memory, spans by the last block to arrive, in the order of the spans.
+#include "kv4.h"
+
+QIL_ERROR_STORAGE
+
+#ifndef QIL_HEAD_DIM
+#define QIL_HEAD_DIM 128
+#endif
+#define D QIL_HEAD_DIM
+static_assert(D % KV4_GROUP == 0 && D >= 32 && D <= KV4_MAX_DIM, "head sizes 32, 64, ..., 256");
+static constexpr int G = D / KV4_GROUP, RUN = 160 * G;
+static constexpr int WARPS = 4, TILE = 32, STAGES = 2;
+static constexpr int STAGE_BYTES = 8 * RUN;            // 4 runs of keys, 4 of values
+static constexpr int MOST_SPANS = 128;
+static constexpr int MOST_LIFT = 90;
+#ifndef KV4_B1
+#define KV4_B1 4
+#endif
+
+struct Kv4Few {
+    const bf16* q;                  // [tokens, q_heads * D]
+    const uint8_t* pages;
+    bf16* out;
+    const int* info;                // [n][8]: first token, its position, tokens, table row, tokens of the segments before, longest context of the step
+    float* part_o;                  // [few tokens][q_heads][n_spans][D]
+    float* part_ml;                 // [few tokens][q_heads][n_spans][2]
+    int* tickets;                   // [few tokens][q_heads], zero between launches
+    const int* block_table;
+    int table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window;
+    float scale_log2;
+};
+
+// Pure functions of their operands: the compiler may move them.
+__device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The first product of a sum: nothing to add to.
+__device__ __forceinline__ void mma_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// The larger of two pairs, half by half; NaN if either is.
+__device__ __forceinline__ unsigned max_pairs(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned transposed(unsigned v) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned pack_bf16(float low, float high) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned times_bf16(unsigned a, unsigned b) {
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+// m + 8 s of two pairs, rounded once.
+__device__ __forceinline__ unsigned middles(unsigned a, unsigned b) {
+    const unsigned steps = __byte_perm(a, b, 0x5410), bases = __byte_perm(a, b, 0x7632);
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&steps), __float2bfloat162_rn(8.f), *reinterpret_cast<const __nv_bfloat162*>(&bases));
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// The pairs of a row's groups.
+__device__ __forceinline__ void load_pairs(const uint8_t* at, unsigned (&w)[G]) {
+    if constexpr (G % 4 == 0) {
+#pragma unroll
+        for (int g = 0; g < G; g += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at + 4 * g);
+            w[g] = v.x; w[g + 1] = v.y; w[g + 2] = v.z; w[g + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < G; ++g) w[g] = *reinterpret_cast<const unsigned*>(at + 4 * g);
+    }
+}
+
+// How many blocks of this kernel share an SM (registers): what the launch bounds ask for.
+constexpr int blocks_a_sm(int nt) { return nt == 1 ? (D <= 128 ? KV4_B1 : 2) : nt == 2 ? (D <= 64 ? 4 : D <= 128 ? 3 : 1) : (D <= 32 ? 4 : D <= 64 ? 3 : 2); }
+
+template <int NT>
+__global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(const Kv4Few a) {
+    extern __shared__ __align__(16) unsigned char shared[];
+    __shared__ uint4 q_frag[G * NT][32];                   // the second operand of the scores' MMAs, as the lanes hold it
+    __shared__ unsigned q_sums[8 * NT][2 * G];             // of a row's groups: the sums' first two parts, the third
+    __shared__ float q_unit[8 * NT];                       // what a row's scores are counted in
+    __shared__ float row_ml[WARPS][8 * NT][2];
+    __shared__ int last_block;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int share = a.q_heads / a.kv_heads;
+    const int4 info = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z];
+    const int4 more = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z + 1];
+    const int first_token = info.x, pos0 = info.y, all_rows = info.z * share, longest = more.y;
+    const int kv = blockIdx.y % a.kv_heads, row0 = blockIdx.y / a.kv_heads * 8 * NT;
+    if (row0 >= all_rows) return;
+    const int rows = min(8 * NT, all_rows - row0);
+    const int pos_low = pos0 + row0 / share, pos_high = pos0 + (row0 + rows - 1) / share;        // of the block's rows
+    const int low = a.window > 0 ? max(0, pos_low + 1 - a.window) : 0;
+    const int reach = a.window > 0 ? min(longest, a.window + info.z + TILE - 1) : longest;
+    const Kv4Span span = kv4_span(blockIdx.x, a.n_spans, reach, low, pos_high + 1, TILE);
+    if ((int)blockIdx.x >= span.count) return;
+    const int* table = a.block_table + (size_t)info.w * a.table_width;
+
+    // ---- copies: this warp's tiles are first_tile, first_tile + WARPS, ...
+    const int first_tile = span.first / TILE + warp, end_tile = (span.last + TILE - 1) / TILE;
+    const int tiles = end_tile > first_tile ? (end_tile - first_tile + WARPS - 1) / WARPS : 0;
+    const int page_runs = a.page_size >> 3;
+    // the number of the run of keys of lane's (tile lane / 4 of eight, run lane % 4) among all runs of the layer, or -1
+    auto runs_of = [&](int tile0) -> int {
+        const int key = (first_tile + WARPS * (tile0 + (lane >> 2))) * TILE + (lane & 3) * 8;
+        if (key >= span.last) return -1;
+        const int page = kv4_page(table, a.table_width, key, a.page_size, a.num_pages);
+        return page < 0 ? -1 : (page * 2 * a.kv_heads + kv) * page_runs + (key % a.page_size >> 3);
+    };
+    const unsigned char* ring_at = shared + warp * STAGES * STAGE_BYTES;
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(ring_at) + (lane >> 3) * RUN + (lane & 7) * 16;
+    int runs_now = tiles ? runs_of(0) : -1, runs_next = tiles > 8 ? runs_of(8) : -1, issued = 0;
+    const size_t value_plane = (size_t)a.kv_heads * page_runs * RUN;
+    const unsigned char* my_pages = a.pages + (lane & 7) * 16;
+    qil_wait_for_producer();                                 // the description and the table are older than the kernel before this one
+    qil_release_consumer();
+    auto issue = [&](int stage) {
+        if (issued < tiles) {
+            const int run = __shfl_sync(0xffffffffu, runs_now, (issued & 7) * 4 + (lane >> 3));
+            const unsigned char* from = my_pages + (size_t)max(run, 0) * RUN;
+            const unsigned to = ring + stage * STAGE_BYTES;
+            const int bytes = run < 0 ? 0 : 16;             // no page: zeros
+#pragma unroll
+            for (int i = 0; i < (10 * G + 7) / 8; ++i) {
+                if ((10 * G) % 8 == 0 || (lane & 7) + 8 * i < 10 * G) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + i * 128), "l"(from + i * 128), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + 4 * RUN + i * 128), "l"(from + value_plane + i * 128), "r"(bytes) : "memory");
+                }
+            }
+            ++issued;
+            if ((issued & 7) == 0) {
+                runs_now = runs_next;
+                runs_next = issued + 8 < tiles ? runs_of(issued + 8) : -1;
+            }
+        }
+        copies_commit();
+    };
+    unsigned absent = __ballot_sync(0xffffffffu, runs_now < 0);           // of the eight tiles with the one at hand: 4 bits a tile
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+
+    // ---- queries: a warp a row, a lane D / 32 dimensions; times 2^up the row's largest lies in [2^99, 2^100)
+    for (int of = warp; of < 8 * NT; of += WARPS) {
+        const int row = row0 + of;
+        float q[G], most_q = 0.f;
+        const bf16* src = a.q + ((size_t)(first_token + min(row, all_rows - 1) / share) * a.q_heads + kv * share + min(row, all_rows - 1) % share) * D;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            q[g] = row < all_rows ? __bfloat162float(src[g * KV4_GROUP + lane]) : 0.f;
+            most_q = fmaxf(most_q, fabsf(q[g]));
+        }
+        most_q = warp_max(most_q);
+        const int up = most_q > 0.f && most_q < INFINITY ? 99 - ilogbf(most_q) : 0;
+        // lane's dimension is 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one
+        const float mine = lane & 1 ? 0.0625f : 1.f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float x = scalbnf(q[g], up);
+            const float sum = scalbnf(warp_sum(x), -133);
+            bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 3)]) + (lane & 3) * 2 + (lane >> 2 & 1);
+            *to = __float2bfloat16_rn(x * mine);
+            if (lane == 0) {
+                const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
+                q_sums[of][2 * g] = pack_bf16(first, second);
+                q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+            }
+        }
+        if (lane == 0) q_unit[of] = scalbnf(a.scale_log2, 133 - up);
+    }
+    __syncthreads();
+    constexpr int SUMS = (G + 3) / 4;               // MMAs for the bases: four groups each, lane c the parts of group 4 i + c
+    uint4 q_reg[NT == 1 ? G : 1];
+    unsigned sum_reg[NT][SUMS][2];
+    float unit[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (NT == 1) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) q_reg[g] = q_frag[g][lane];
+        }
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) {
+            const int g = 4 * i + c;
+            sum_reg[nt][i][0] = g < G ? q_sums[nt * 8 + r][2 * min(g, G - 1)] : 0u;
+            sum_reg[nt][i][1] = g < G ? q_sums[nt * 8 + r][2 * min(g, G - 1) + 1] : 0u;
+        }
+        unit[nt][0] = q_unit[nt * 8 + 2 * c];
+        unit[nt][1] = q_unit[nt * 8 + 2 * c + 1];
+    }
+
+    float acc[NT][G][2][4], side[NT][4], less[NT][4];
+    // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p (m + 8 s)), row 8 sum(p); less: row g -8 sum(p s), as acc's row
+    float most[NT][2];                          // of rows 2 c, 2 c + 1
+    int lift = MOST_LIFT;                       // p s stays below 2^108, so that it overflows nowhere, and far above 2^7
+    unsigned lift_limit = (100 - MOST_LIFT + 128) << 7;                       // a step of that many bits or more (NaN too) asks for another lift
+    unsigned marked[NT][2];                     // groups whose values are NaN for them
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[nt][g][0][i] = acc[nt][g][1][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) side[nt][i] = less[nt][i] = 0.f;
+        most[nt][0] = most[nt][1] = -INFINITY;
+        marked[nt][0] = marked[nt][1] = 0u;
+    }
+    const int order = (r >> 1) + (r & 1) * 4;                     // the key of 8 that row r stands for
+    const unsigned half = r & 1 ? 0x7632u : 0x5410u;              // my half of a word of values, of two keys
+    auto row_pos = [&](int nt, int i) { return pos0 + min(row0 + nt * 8 + 2 * c + i, all_rows - 1) / share; };
+
+    float minus[NT][2];                                           // what is added to a scaled score before the exponential
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) minus[nt][0] = minus[nt][1] = (float)MOST_LIFT;
+    unsigned sink = (127 - MOST_LIFT) << 7 | (127 - MOST_LIFT) << 23;         // 2^-lift, twice
+    const unsigned one = r == 0 ? 0x3f803f80u : 0u;
+    // tiles of keys that every row sees begin in [plain_low, plain_low + plain_more]
+    const int plain_low = max(span.first, a.window > 0 ? pos_high - a.window + 1 : 0);
+    const int plain_more = min(pos_low - TILE + 1, span.last - TILE) - plain_low;
+    int stage = 0;
+    for (int n = 0; n < tiles; ++n) {
+        if ((n & 7) == 0 && n > 0) absent = __ballot_sync(0xffffffffu, runs_now < 0);
+        issue(stage == 0 ? STAGES - 1 : stage - 1);
+        copies_wait<STAGES - 1>();
+        __syncwarp();
+        const int k0 = (first_tile + WARPS * n) * TILE;
+        const unsigned char* keys = ring_at + stage * STAGE_BYTES;
+        unsigned char* values = const_cast<unsigned char*>(keys) + 4 * RUN;
+        const unsigned gone = absent >> 4 * (n & 7) & 15u;
+        // ---- scores [32 keys][8 NT rows] in the rows' units: sc[u][nt][i]: key 16 u + 8 (i / 2) + order, row 8 nt + 2 c + (i & 1)
+        float sc[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned char* run0 = keys + 2 * u * RUN;
+            const unsigned char* run1 = run0 + RUN;
+            unsigned pair0[G], pair1[G];
+            load_pairs(run0 + 128 * G + order * 4 * G, pair0);
+            load_pairs(run1 + 128 * G + order * 4 * G, pair1);
+#pragma unroll
+            for (int i = 0; i < SUMS; ++i) {
+                unsigned base0 = 0u, base1 = 0u;
+                if (G % 4 == 0 || 4 * i + c < G) {
+                    const unsigned own0 = *reinterpret_cast<const unsigned*>(run0 + 128 * G + order * 4 * G + 16 * i + 4 * c);
+                    const unsigned own1 = *reinterpret_cast<const unsigned*>(run1 + 128 * G + order * 4 * G + 16 * i + 4 * c);
+                    base0 = __byte_perm(own0, own0, 0x3232);
+                    base1 = __byte_perm(own1, own1, 0x3232);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (i == 0) mma_first(sc[u][nt], base0, base1, base0, base1, sum_reg[nt][i][0], sum_reg[nt][i][1]);
+                    else mma(sc[u][nt], base0, base1, base0, base1, sum_reg[nt][i][0], sum_reg[nt][i][1]);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const unsigned w0 = *reinterpret_cast<const unsigned*>(run0 + g * 128 + order * 16 + c * 4);
+                const unsigned w1 = *reinterpret_cast<const unsigned*>(run1 + g * 128 + order * 16 + c * 4);
+                const unsigned w2 = w0 >> 8, w3 = w1 >> 8;
+                const float s0 = kv4_step(pair0[g]), s1 = kv4_step(pair1[g]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4 q = NT == 1 ? q_reg[NT == 1 ? g : 0] : q_frag[g * NT + nt][lane];
+                    float dot[4];
+                    mma_first(dot, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q.x, q.y);
+                    mma(dot, w2 & 0x000f000fu, w3 & 0x000f000fu, w2 & 0x00f000f0u, w3 & 0x00f000f0u, q.z, q.w);
+                    sc[u][nt][0] = fmaf(s0, dot[0], sc[u][nt][0]);
+                    sc[u][nt][1] = fmaf(s0, dot[1], sc[u][nt][1]);
+                    sc[u][nt][2] = fmaf(s1, dot[2], sc[u][nt][2]);
+                    sc[u][nt][3] = fmaf(s1, dot[3], sc[u][nt][3]);
+                }
+            }
+        }
+        // ---- values that are NaN, and a tile with keys that not every row sees
+        unsigned* my_pairs = reinterpret_cast<unsigned*>(values + (lane >> 3) * RUN + 128 * G + (lane & 7) * 4 * G);      // of key k0 + lane
+        unsigned pairs[G];
+        load_pairs(reinterpret_cast<const uint8_t*>(my_pairs), pairs);
+        unsigned largest = pairs[0];
+#pragma unroll
+        for (int g = 1; g < G; ++g) largest = max_pairs(largest, pairs[g]);
+        const bool partly = (unsigned)(k0 - plain_low) > (unsigned)plain_more || plain_more < 0 || gone;
+        if (partly || __any_sync(0xffffffffu, (largest & 0xffffu) >= lift_limit)) {
+            const int key = k0 + lane;
+            const bool inside = key >= span.first && key < span.last && !(gone >> (lane >> 3) & 1);
+            unsigned nan = 0;
+            largest = 0u;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const bool is_nan = !__hbeq2(*reinterpret_cast<const __nv_bfloat162*>(&pairs[g]), *reinterpret_cast<const __nv_bfloat162*>(&pairs[g]));
+                if (is_nan) nan |= 1u << g;
+                if (!inside || is_nan) my_pairs[g] = 0u;
+                else largest = max_pairs(largest, pairs[g]);
+            }
+            for (unsigned left = __ballot_sync(0xffffffffu, inside && nan != 0); left; left &= left - 1) {
+                const int j = __ffs(left) - 1;
+                const unsigned groups = __shfl_sync(0xffffffffu, nan, j);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int pos = row_pos(nt, i);
+                        if (k0 + j <= pos && (a.window == 0 || k0 + j > pos - a.window)) marked[nt][i] |= groups;
+                    }
+            }
+            // the lift: by the exponent of the tile's largest step
+            const int exponent = (int)(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 7) - 127;
+            if (exponent + lift > 100) {
+                const int lower = 92 - exponent;
+                const float by = scalbnf(1.f, lower - lift);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[nt][g][0][i] *= by;
+                            acc[nt][g][1][i] *= by;
+                        }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) less[nt][i] *= by;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) minus[nt][i] += (float)(lower - lift);
+                }
+                lift = lower;
+                lift_limit = (unsigned)min(max(228 - lift, 0), 255) << 7;
+                sink = (unsigned)(127 - lift) << 7 | (unsigned)(127 - lift) << 23;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = k0 + 16 * u + 8 * (i >> 1) + order, pos = row_pos(nt, i & 1);
+                        const bool seen = key >= span.first && key < span.last && key <= pos && (a.window == 0 || key > pos - a.window)
+                            && !(gone >> (2 * u + (i >> 1)) & 1);
+                        if (!seen) sc[u][nt][i] = -INFINITY;
+                    }
+        }
+        unsigned p0[2][NT], p1[2][NT];
+        // ---- softmax, and p 2^lift as the second product's operand: p0[u][nt], p1: keys c, c + 4 of runs 2 u and 2 u + 1, row 8 nt + r
+        float peak[NT][2];
+        bool grew = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                peak[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i])) * unit[nt][i];
+                grew |= peak[nt][i] > most[nt][i] + 8.f;          // the first finite one too
+            }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float keep[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float p = peak[nt][i];
+                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 4));
+                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 8));
+                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 16));
+                    const bool grow = p > most[nt][i] + 8.f;
+                    keep[i] = grow ? fast_exp2(most[nt][i] - p) : 1.f;
+                    if (grow) {
+                        most[nt][i] = p;
+                        minus[nt][i] = (float)lift - p;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[nt][g][0][i] *= keep[i & 1];
+                        acc[nt][g][1][i] *= keep[i & 1];
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    side[nt][i] *= keep[i & 1];
+                    less[nt][i] *= keep[i & 1];
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = fast_exp2(fmaf(sc[u][nt][i], unit[nt][i & 1], minus[nt][i & 1]));
+                }
+                p0[u][nt] = transposed(pack_bf16(e[0], e[1]));
+                p1[u][nt] = transposed(pack_bf16(e[2], e[3]));
+            }
+        }        // ---- output
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned char* run0 = values + 2 * u * RUN;
+            const unsigned char* run1 = run0 + RUN;
+            unsigned pa[G], pb[G], steps0[G], steps1[G];
+            load_pairs(run0 + 128 * G + c * 4 * G, pa);
+            load_pairs(run0 + 128 * G + (c + 4) * 4 * G, pb);
+#pragma unroll
+            for (int g = 0; g < G; ++g) steps0[g] = __byte_perm(pa[g], pb[g], 0x5410);
+            load_pairs(run1 + 128 * G + c * 4 * G, pa);
+            load_pairs(run1 + 128 * G + (c + 4) * 4 * G, pb);
+#pragma unroll
+            for (int g = 0; g < G; ++g) steps1[g] = __byte_perm(pa[g], pb[g], 0x5410);
+            unsigned base0 = 0u, base1 = 0u;                       // row g of the side sums: m + 8 s of group r
+            if (r < G) {
+                const unsigned* at0 = reinterpret_cast<const unsigned*>(run0 + 128 * G + 4 * r);
+                const unsigned* at1 = reinterpret_cast<const unsigned*>(run1 + 128 * G + 4 * r);
+                base0 = middles(at0[c * G], at0[(c + 4) * G]);
+                base1 = middles(at1[c * G], at1[(c + 4) * G]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma(side[nt], base0, one, base1, one, times_bf16(p0[u][nt], sink), times_bf16(p1[u][nt], sink));
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const unsigned char* at0 = run0 + g * 128 + (r >> 1) * 4;
+                const unsigned char* at1 = run1 + g * 128 + (r >> 1) * 4;
+                const unsigned x = __byte_perm(*reinterpret_cast<const unsigned*>(at0 + c * 16), *reinterpret_cast<const unsigned*>(at0 + (c + 4) * 16), half);
+                const unsigned y = __byte_perm(*reinterpret_cast<const unsigned*>(at1 + c * 16), *reinterpret_cast<const unsigned*>(at1 + (c + 4) * 16), half);
+                const unsigned xs = x >> 8, ys = y >> 8;
+                const unsigned eight = r == g ? 0x80088008u : 0u;          // a code of -8 in row g
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const unsigned b0 = times_bf16(p0[u][nt], steps0[g]), b1 = times_bf16(p1[u][nt], steps1[g]);
+                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0, b1);
+                    mma(less[nt], eight, 0u, eight, 0u, b0, b1);
+                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, b0, b1);
+                }
+            }
+        }
+        __syncwarp();
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+    copies_wait<0>();
+
+    // ---- the block's rows: [WARPS][8 rows][D] floats at a time
+    const bool alone = span.count == 1;
+    float* rows_o = reinterpret_cast<float*>(shared);
+    const float down = scalbnf(1.f, 33 - lift);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        if (r == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                row_ml[warp][nt * 8 + 2 * c + i][0] = most[nt][i];
+                row_ml[warp][nt * 8 + 2 * c + i][1] = side[nt][2 + i];
+            }
+        }
+        __syncthreads();               // the ring, or the rows before these, are done with
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float middle = __shfl_sync(0xffffffffu, side[nt][i], 4 * g + c), eights = __shfl_sync(0xffffffffu, less[nt][i], 4 * g + c);
+                const float add = (marked[nt][i] >> g & 1) ? __int_as_float(0x7fc00000) : fmaf(eights * 0x1p100f, down, middle);
+                float4 o;                                  // 2^133 2^-lift is beyond float32 for a lift below 6: in two steps
+                o.x = fmaf(acc[nt][g][0][i] * 0x1p100f, down, add);
+                o.y = fmaf(acc[nt][g][0][2 + i] * 0x1p96f, down, add);
+                o.z = fmaf(acc[nt][g][1][i] * 0x1p100f, down, add);
+                o.w = fmaf(acc[nt][g][1][2 + i] * 0x1p96f, down, add);
+                *reinterpret_cast<float4*>(rows_o + (warp * 8 + 2 * c + i) * D + g * KV4_GROUP + 4 * r) = o;
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * (D / 4); i += 32 * WARPS) {
+            const int of = i / (D / 4), d = i % (D / 4) * 4, row = row0 + nt * 8 + of;
+            if (row >= all_rows) break;
+            float peak = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) peak = fmaxf(peak, row_ml[w][nt * 8 + of][0]);
+            const float against = peak == -INFINITY ? 0.f : peak;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float keep = fast_exp2(row_ml[w][nt * 8 + of][0] - against);
+                const float4 o = *reinterpret_cast<const float4*>(rows_o + (w * 8 + of) * D + d);
+                sum.x = fmaf(o.x, keep, sum.x); sum.y = fmaf(o.y, keep, sum.y);
+                sum.z = fmaf(o.z, keep, sum.z); sum.w = fmaf(o.w, keep, sum.w);
+                l = fmaf(row_ml[w][nt * 8 + of][1], keep, l);
+            }
+            const int head = kv * share + row % share;
+            if (alone) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                *reinterpret_cast<uint2*>(a.out + ((size_t)(first_token + row / share) * a.q_heads + head) * D + d)
+                    = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+            } else {
+                const size_t slot = ((size_t)(more.x + row / share) * a.q_heads + head) * a.n_spans + blockIdx.x;
+                *reinterpret_cast<float4*>(a.part_o + slot * D + d) = sum;
+                if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(peak, l);
+            }
+        }
+    }
+    if (alone) return;
+    // ---- the last block of these rows joins the spans
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* ticket = a.tickets + (size_t)more.x * a.q_heads + kv * all_rows + row0 / (8 * NT);
+        last_block = atomicAdd(ticket, 1) == span.count - 1;
+        if (last_block) *ticket = 0;
+    }
+    __syncthreads();
+    if (!last_block) return;
+    __threadfence();
+    float* weight = reinterpret_cast<float*>(shared);          // [8 NT][n_spans], then the sums of the rows
+    for (int of = warp; of < rows; of += WARPS) {
+        const int row = row0 + of;
+        const size_t slot = ((size_t)(more.x + row / share) * a.q_heads + kv * share + row % share) * a.n_spans;
+        float peak = -INFINITY, l = 0.f;
+        for (int s = lane; s < span.count; s += 32) peak = fmaxf(peak, __ldcg(a.part_ml + (slot + s) * 2));
+        peak = warp_max(peak);
+        const float against = peak == -INFINITY ? 0.f : peak;
+        for (int s = lane; s < span.count; s += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + (slot + s) * 2));
+            const float keep = fast_exp2(ml.x - against);
+            weight[of * a.n_spans + s] = keep;
+            l = fmaf(ml.y, keep, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) row_ml[0][of][0] = l == 0.f ? 0.f : 1.f / l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * WARPS) {
+        const int of = i / (D / 4), d = i % (D / 4) * 4, row = row0 + of, head = kv * share + row % share;
+        const float* from = a.part_o + ((size_t)(more.x + row / share) * a.q_heads + head) * a.n_spans * D + d;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int s = 0; s < span.count; ++s) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(from + (size_t)s * D));
+            const float keep = weight[of * a.n_spans + s];
+            sum.x = fmaf(o.x, keep, sum.x); sum.y = fmaf(o.y, keep, sum.y);
+            sum.z = fmaf(o.z, keep, sum.z); sum.w = fmaf(o.w, keep, sum.w);
+        }
+        const float inv = row_ml[0][of][0];
+        *reinterpret_cast<uint2*>(a.out + ((size_t)(first_token + row / share) * a.q_heads + head) * D + d)
+            = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+    }
+}
+
+template <int NT>
+static int launch(const Kv4Few& a, int n, int most_rows, cudaStream_t stream) {
+    const int ring = WARPS * STAGES * STAGE_BYTES, rows = WARPS * 8 * D * 4, weights = 8 * NT * a.n_spans * 4;
+    const int smem = ring > rows ? (ring > weights ? ring : weights) : (rows > weights ? rows : weights);
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory: %s", cudaGetErrorString(e));
+        configured = true;
+    }
+    const dim3 grid(a.n_spans, a.kv_heads * ((most_rows + 8 * NT - 1) / (8 * NT)), n);
+    if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments, %d rows a kv head", n, most_rows);
+    const cudaError_t e = qil_launch_chained(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, stream, a);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        snprintf(qil_error_text, sizeof(qil_error_text), "%s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return 0;
+}
+
+extern "C" int qil_kv4_few_head_dim() { return D; }
+extern "C" int qil_kv4_few_most_spans() { return MOST_SPANS; }
+extern "C" int qil_kv4_few_blocks_a_sm(int nt) { return blocks_a_sm(nt); }
+
+// info: see Kv4Few; most_tokens: of a segment; nt: 8-row tiles a block takes (1, 2 or 4; 1 or 2 of heads beyond 128).
+extern "C" int qil_kv4_few(const void* q, const void* pages, void* out, const void* info, int n, int most_tokens, int nt, void* part_o, void* part_ml,
+                           void* tickets, int n_spans, const void* block_table, int table_width, int q_heads, int kv_heads, int page_size, int num_pages,
+                           int window, float scale, cudaStream_t stream) {
+    if (n <= 0) return 0;
+    if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
+    if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n_spans < 1 || n_spans > MOST_SPANS || most_tokens < 1 || window < 0)
+        QIL_REFUSE("%d query heads, %d kv heads, %d spans", q_heads, kv_heads, n_spans);
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages | (uintptr_t)info | (uintptr_t)part_o) & 15) QIL_REFUSE("kv4: operands must be 16-byte aligned");
+    const Kv4Few a = {(const bf16*)q, (const uint8_t*)pages, (bf16*)out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
+                      (const int*)block_table, table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, scale * 1.4426950408889634f};
+    const int rows = most_tokens * (q_heads / kv_heads);
+    if (nt == 1) return launch<1>(a, n, rows, stream);
+    if (nt == 2) return launch<2>(a, n, rows, stream);
+#if QIL_HEAD_DIM <= 128
+    if (nt == 4) return launch<4>(a, n, rows, stream);
+#endif
+    QIL_REFUSE("kv4: %d tiles of rows a block", nt);
+}

@@ -13,6 +13,7 @@ package the functions launch on torch's current stream, on the current device, a
 """
 from __future__ import annotations
 
+import functools
 from ctypes import c_float, c_int, c_longlong
 from types import SimpleNamespace
 
@@ -20,14 +21,14 @@ import numpy as np
 import torch
 
 from ..parts.base import PlanView, Segments
-from . import attention_f32, attention_mma, build, ops
+from . import attention_f32, attention_mma, attention_tc, build, ops, tuning
 from .ops import F32, KernelError, _check, _need, _p, _stream, dtype_code
 
 GROUP = 32
 MOST_DIM = 256
 PLAN_KEY = "kv4_attention"        # the step planner whose arrays ``attend`` reads (``describe_segments`` makes them)
-#: Tokens up to which a segment's tokens are taken one by one, each walking the context by itself; longer portions' rows are
-#: read back once and attended to as ordinary pages.
+#: Tokens of a segment up to which the kernels that walk the codes take it; longer portions' rows are read back once and attended to
+#: as ordinary pages.
 FEW_TOKENS = 8
 #: Positions per page of rows that are read back for a portion, and the most of them at a time (of several portions; a single
 #: one may be longer): 8 heads of 128 in bfloat16 take 4 KB a position.
@@ -35,6 +36,23 @@ READ_PAGE, MOST_READ = 64, 1 << 16
 
 SOURCES, DEPENDS = ["kv4_store.cu", "kv4_attention.cu"], ["kv4.h"]
 _lib = None
+_few_libs: dict = {}
+
+
+def few_library_name(head_dim):
+    """(name, defines) of the tensor-core library for heads of ``head_dim``."""
+    return f"qil_kv4_d{head_dim}", {"QIL_HEAD_DIM": head_dim}
+
+
+def few_library(head_dim):
+    lib = _few_libs.get(head_dim)
+    if lib is None:
+        name, defines = few_library_name(head_dim)
+        lib = build.load(name, ["kv4_attention_mma.cu"], defines, depends=DEPENDS)
+        if lib.qil_kv4_few_head_dim() != head_dim:
+            raise KernelError("the 4-bit attention library was built for another head size")
+        _few_libs[head_dim] = lib
+    return lib
 
 
 def library():
@@ -163,15 +181,23 @@ def describe_segments(first, starts, lens, rows) -> dict:
     """A step's segments as ``attend`` wants them (numpy int64 arrays in, one entry per segment: first token in the flat batch,
     its absolute position, tokens, block-table row).
 
-    ``tokens``          the tokens of segments of at most FEW_TOKENS: four ints each, (token, its position, block-table row, the longest
-                        context among these segments)
-    ``portion_tokens``  the same of all other segments
-    ``b0.read`` ...     the other segments in batches whose contexts are read back together: ``kv4.read``'s info, the block table of the
+    ``singles``, ``few``, ``portions``  the segments of one token, of up to FEW_TOKENS and the others: eight ints each, (first token, its
+                        position, tokens, block-table row, tokens of the segments before in this array, the longest context among these, 0, 0)
+    ``single_tokens``, ``few_tokens``, ``portion_tokens``  the same token by token, four ints each, (token, its position, block-table row, the
+                        longest context among these)
+    ``b0.read`` ...     the portions in batches whose contexts are read back together: ``kv4.read``'s info, the block table of the
                         pages they are read to, and their query tiles over that table (``attention_mma.describe_segments``)
     """
     lens, starts = np.asarray(lens, dtype=np.int64), np.asarray(starts, dtype=np.int64)
     first, rows = np.asarray(first, dtype=np.int64), np.asarray(rows, dtype=np.int64)
     ends = starts + lens
+
+    def segments(indices):
+        if not len(indices):
+            return np.zeros(0, dtype=np.int64)
+        before = np.cumsum(lens[indices]) - lens[indices]
+        none = np.zeros_like(before)
+        return np.stack([first[indices], starts[indices], lens[indices], rows[indices], before, none + ends[indices].max(), none, none], axis=1).reshape(-1)
 
     def one_by_one(indices):
         if not len(indices):
@@ -180,8 +206,12 @@ def describe_segments(first, starts, lens, rows) -> dict:
         offset = np.arange(len(of)) - np.repeat(np.cumsum(lens[indices]) - lens[indices], lens[indices])
         return np.stack([first[of] + offset, starts[of] + offset, rows[of], np.full_like(of, ends[indices].max())], axis=1).reshape(-1)
 
+    arrays = {}
+    for name, tokens, some in (("singles", "single_tokens", lens == 1), ("few", "few_tokens", (lens > 1) & (lens <= FEW_TOKENS)),
+                               ("portions", "portion_tokens", lens > FEW_TOKENS)):
+        indices = np.nonzero(some)[0]
+        arrays[name], arrays[tokens] = segments(indices), one_by_one(indices)
     portions = np.nonzero(lens > FEW_TOKENS)[0]
-    arrays = dict(tokens=one_by_one(np.nonzero((lens > 0) & (lens <= FEW_TOKENS))[0]), portion_tokens=one_by_one(portions))
     order = portions[np.argsort(-ends[portions], kind="stable")]
     batch = 0
     while len(order):
@@ -200,18 +230,19 @@ def describe_segments(first, starts, lens, rows) -> dict:
 
 def refresh_single_tokens(arrays, starts) -> None:
     """``describe_segments`` of a step of single tokens whose rows are those of the step before: only the positions change."""
-    info = arrays["tokens"]
-    n = len(starts)
-    info[1:4 * n:4] = starts
-    info[3:4 * n:4] = int(starts.max()) + 1
+    n, longest = len(starts), int(starts.max()) + 1
+    for info, width, last in ((arrays["singles"], 8, 5), (arrays["single_tokens"], 4, 3)):
+        info[1:width * n:width] = starts
+        info[last:width * n:width] = longest
 
 
 class StepPlan:
     """A step's segments on the device, as ``attend`` reads them.  ``max_context``: the longest context; of a recorded step the
     longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest."""
 
-    def __init__(self, array, count, max_context, min_context=0):
+    def __init__(self, array, count, max_context, min_context=0, most_tokens=0):
         self.array, self.count = array, count
+        self.most_tokens = int(most_tokens)          # of a segment
         self.max_context, self.min_context = int(max_context), int(min_context)
         self.batches = 0
         while f"b{self.batches}.read" in count:
@@ -226,13 +257,14 @@ class StepPlan:
             raise KernelError("kv4.StepPlan: a row, a start and at least one token a segment")
         arrays = describe_segments(np.cumsum(lens) - lens, starts, lens, rows)
         array = {name: torch.from_numpy(values.astype(np.int32)).to(device) for name, values in arrays.items()}
-        return cls(array, {name: len(values) for name, values in arrays.items()}, int((starts + lens).max(initial=0)))
+        return cls(array, {name: len(values) for name, values in arrays.items()}, int((starts + lens).max(initial=0)),
+                   most_tokens=lens.max(initial=0))
 
     @classmethod
     def of_step(cls, ctx):
         """Of the step in flight, from the arrays that the planner made for it."""
         view = ctx.plans[PLAN_KEY]
-        return cls(view.array, view.count, ctx.max_context, ctx.min_context)
+        return cls(view.array, view.count, ctx.max_context, ctx.min_context, most_tokens=max(ctx.h_seg_len))
 
 
 # ------------------------------------------------------------------ attention
@@ -246,24 +278,55 @@ def _slots(blocks_per_sm) -> int:
     return _sms * blocks_per_sm
 
 
-def _spans(blocks_per_span, slots, plan, window) -> int:
-    """Parts to cut the contexts into: as many as fill the GPU once (``attention_mma.plan_spans`` has the model)."""
-    tile = attention_mma.KV_TILE
-    reach = lambda context: min(context, window + tile) if window else context
-    hi = max(1, -(-reach(plan.max_context) // tile))
-    lo = max(1, min(hi, -(-reach(plan.min_context or plan.max_context) // tile)))
-    return attention_mma._plan_tiles(blocks_per_span, slots, lo, hi)
+#: Keys that a block of the span kernels takes at a time: a tile of 32 for each of its four warps.
+STEP = 128
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan(blocks_per_span, slots, lo, hi, most) -> int:
+    """The number of spans with the lowest cost per step of keys at both ends of [lo, hi] steps of longest context.  A wave of blocks takes
+    the steps of a span and a start-up; every span costs the join something."""
+    def cost(steps, n):
+        each = -(-steps // n)
+        n = -(-steps // each)
+        return (-(-blocks_per_span * n // slots) * (each + tuning.KV4_SPAN_STARTUP) + tuning.KV4_SPAN_JOIN * n) / steps
+    return min(range(1, min(hi, most) + 1), key=lambda n: cost(hi, n) + (cost(lo, min(n, lo)) if lo != hi else 0.0))
+
+
+def _spans(blocks_per_span, slots, plan, window, most) -> int:
+    """Parts to cut the contexts into."""
+    reach = lambda context: min(context, window + STEP) if window else context
+    hi = max(1, -(-reach(plan.max_context) // STEP))
+    lo = max(1, min(hi, -(-reach(plan.min_context or plan.max_context) // STEP)))
+    return _plan(blocks_per_span, slots, lo, hi, max(1, most))
+
+
+def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
+    return attention_mma.decode_scratch(SimpleNamespace(extras=extras, device=device), tokens, n_q_heads, n_spans, head_dim,
+                                        most=attention_f32.MOST_SCRATCH)
+
+
+def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
+    lib = few_library(head_dim)
+    rows = most_tokens * (n_q_heads // n_kv_heads)
+    nt = 1 if rows <= 8 else 2 if rows <= 16 or head_dim > 128 else 4
+    blocks = n * n_kv_heads * -(-rows // (8 * nt))
+    # the partial sums of all spans: fewer spans where they would outgrow their limit
+    most = min(lib.qil_kv4_few_most_spans(), attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
+    n_spans = _spans(blocks, _slots(lib.qil_kv4_few_blocks_a_sm(c_int(nt))), plan, window, most)
+    part_o, part_ml, tickets = _scratch(extras, q.device, tokens, n_q_heads, n_spans, head_dim)
+    _check(lib, lib.qil_kv4_few(_p(q), _p(pages), _p(out), _p(info), c_int(n), c_int(most_tokens), c_int(nt), _p(part_o), _p(part_ml), _p(tickets),
+                                c_int(n_spans), _p(block_table), c_int(block_table.shape[1]), c_int(n_q_heads), c_int(n_kv_heads), c_int(page_size),
+                                c_int(pages.shape[0]), c_int(window), c_float(scale), _stream()), "kv4.attend (few tokens)")
 
 
 def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib = library()
     share = n_q_heads // n_kv_heads
     chunks = -(-share // lib.qil_kv4_singles_heads(c_int(share)))
-    n_spans = _spans(n * n_kv_heads * chunks, _slots(3), plan, window)
-    # the partial sums of all spans: fewer spans where they would outgrow their limit
-    n_spans = max(1, min(n_spans, attention_f32.MOST_SCRATCH // (4 * n * n_q_heads * head_dim)))
-    part_o, part_ml, tickets = attention_mma.decode_scratch(SimpleNamespace(extras=extras, device=q.device), n, n_q_heads, n_spans, head_dim,
-                                                            most=attention_f32.MOST_SCRATCH)
+    most = attention_f32.MOST_SCRATCH // (4 * n * n_q_heads * head_dim)
+    n_spans = _spans(n * n_kv_heads * chunks, _slots(3), plan, window, most)
+    part_o, part_ml, tickets = _scratch(extras, q.device, n, n_q_heads, n_spans, head_dim)
     _check(lib, lib.qil_kv4_singles(_p(q), _p(pages), _p(out), _p(info), c_int(n), _p(part_o), _p(part_ml), _p(tickets), c_int(n_spans),
                                     _p(block_table), c_int(block_table.shape[1]), c_int(n_q_heads), c_int(n_kv_heads), c_int(head_dim),
                                     c_int(page_size), c_int(pages.shape[0]), c_int(window), c_float(scale), c_int(dtype_code(q.dtype)), _stream()),
@@ -311,16 +374,28 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
         raise KernelError(f"kv4.attend: queries {tuple(q.shape)}, output {tuple(out.shape)}")
     if window < 0:
         raise KernelError("kv4.attend: a window cannot be negative")
-    _here("kv4.attend", q, pages, out, block_table, plan.array["tokens"])
+    _here("kv4.attend", q, pages, out, block_table, plan.array["singles"])
     shape = (q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, float(scale), int(window), extras)
-    if plan.count["tokens"]:
-        _singles(plan.array["tokens"], plan.count["tokens"] // 4, plan, *shape)
-    if plan.count["portion_tokens"]:
-        by_tile = attention_mma.supports(head_dim, n_q_heads, n_kv_heads) if q.dtype == torch.bfloat16 \
-            else attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads)
-        if by_tile:
+    count, array = plan.count, plan.array
+    if q.dtype == torch.float32:
+        for name in ("single_tokens", "few_tokens"):
+            if count[name]:
+                _singles(array[name], count[name] // 4, plan, *shape)
+        if count["portion_tokens"]:
+            if attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads):
+                for batch in range(plan.batches):
+                    _portions(plan, batch, *shape)
+            else:       # heads of a size that the tile kernel does not take: token by token
+                _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan, *shape)
+        return out
+    if count["singles"]:
+        _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, *shape)
+    if count["few"]:
+        _few(array["few"], count["few"] // 8, count["few_tokens"] // 4, FEW_TOKENS, plan, *shape)
+    if count["portions"]:
+        if attention_tc.supports(head_dim, READ_PAGE, window):
             for batch in range(plan.batches):
                 _portions(plan, batch, *shape)
-        else:       # float32 heads of a size that the tile kernel does not take: token by token
-            _singles(plan.array["portion_tokens"], plan.count["portion_tokens"] // 4, plan, *shape)
+        else:           # heads beyond 128
+            _few(array["portions"], count["portions"] // 8, count["portion_tokens"] // 4, plan.most_tokens, plan, *shape)
     return out

@@ -217,8 +217,8 @@ def attend_run(case, window=0, scale=None, extras=None, plan=None, out=None):
 def attend_check(case, out, window=0, scale=None):
     """Against 64 bits.  A relative error e of every weight p moves a result by e sum p |v| at most, and of the sum that divides it by as much.
     A weight's error is twice that of its score at most: float32 sums of dim terms are off by dim 2^-24 scale sum |q k|, keys in 11 bits
-    (long portions) by 2^-11 of it.  For bfloat16 queries the kernels round p once (2^-8) and its product with a step once, or the values
-    that it weighs; then the result."""
+    (long portions) by 2^-11 of it.  For bfloat16 queries the kernels round p once (2^-8) and its product with a step once more, which moves
+    the result by 2^-8 sum p (v - m), or the values that it weighs; then the result."""
     scale = case["dim"] ** -0.5 if scale is None else scale
     first = 0
     got = out.cpu().double().view(len(out), case["hq"], case["dim"])
@@ -229,7 +229,9 @@ def attend_check(case, out, window=0, scale=None):
         off = (got[first:first + n] - exact).abs()
         most = scale * torch.einsum("nhd,thd->nht", q.abs(), keys.abs()).amax(-1, keepdim=True)      # of the terms of a score
         if case["dtype"] == BF16:
-            bar = 2.0 ** -8 * exact.abs() + (4 * 2.0 ** -8 + 2 * 2.0 ** -11 * most) * size
+            groups = case["held"][i][1].unflatten(-1, (-1, 32))
+            _, above = plain.attention(q, case["held"][i][0], (groups - groups.amin(-1, keepdim=True)).flatten(-2), torch.arange(start, start + n), scale, window)
+            bar = 2.0 ** -8 * exact.abs() + (4 * 2.0 ** -8 + 2 * 2.0 ** -11 * most) * size + 2.0 ** -8 * above
         else:
             bar = 2.0 ** -24 * (start + n + 64 + 2 * case["dim"] * most) * size
         assert torch.isfinite(got[first:first + n]).all() and (off <= bar).all(), (i, float((off / bar).max()))
