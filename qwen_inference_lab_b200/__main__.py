@@ -25,6 +25,7 @@ def build_parser():
     parser.add_argument("--page-size", default=16, type=int)
     parser.add_argument("--chunk-size", default=64, type=int, help="most prompt tokens of a request per step")
     parser.add_argument("--token-budget", default=128, type=int, help="most tokens per step over all requests")
+    parser.add_argument("--kv-bits", default=None, type=int, choices=[4], help="keep cached keys and values in 4 bits")
     parser.add_argument("--max-active", default=4, type=int)
     parser.add_argument("--temperature", default=0.0, type=float, help="0 = greedy")
     parser.add_argument("--seed", default=0, type=int, help="sampling seed")
@@ -55,7 +56,7 @@ def main(argv=None):
         tokens = json.loads(args.token_ids)
     model = load_model(args.model, device=args.device, dtype=args.dtype)
     engine = Engine(model, num_pages=args.pages, page_size=args.page_size, prefill_chunk=args.chunk_size,
-                    token_budget=args.token_budget, max_active=args.max_active, seed=args.seed)
+                    token_budget=args.token_budget, max_active=args.max_active, seed=args.seed, kv_bits=args.kv_bits)
     try:
         result = engine.generate([tokens], max_new_tokens=args.max_new_tokens, ignore_eos=args.ignore_eos,
                                  temperature=args.temperature, seed=args.seed)[0]

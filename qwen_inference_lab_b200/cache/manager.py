@@ -21,7 +21,8 @@ limit reserves nothing and grows until the free list is empty (trace replay).
 Layout of a group's storage: ``[member, page, 2 (K,V), kv_head, slot, head_dim]``; where values have
 another size than keys, ``[member, page, kv_head * slot * (head_dim + v_head_dim)]``: a page's key rows
 ``[kv_head, slot, head_dim]`` followed by its value rows ``[kv_head, slot, v_head_dim]``; where a position's value is
-the head of its key (``shared_rows``), ``[member, page, 1, kv_head, slot, head_dim]``.
+the head of its key (``shared_rows``), ``[member, page, 1, kv_head, slot, head_dim]``; where rows are kept in 4 bits, bytes
+``[member, page, 2 (K,V), kv_head, slot / 8, 160 * head_dim / 32]``.
 """
 from __future__ import annotations
 
@@ -30,7 +31,8 @@ from dataclasses import dataclass
 
 import torch
 
-from ..parts.base import KVCacheSpec, StateSpec
+from ..kernels import kv4
+from ..parts.base import KVCacheSpec, StateSpec, cache_planners
 from ..utils.staging import PinnedRing
 
 
@@ -49,6 +51,7 @@ class KVCacheView:
     block_table: torch.Tensor    # int32 [max_requests, table_width]; -1 where no page is held
     page_size: int
     window: int
+    bits: int = 0                # 4: pages of 4-bit rows, uint8
 
 
 @dataclass
@@ -61,7 +64,12 @@ class _KVGroup:
     def __init__(self, spec, members, num_pages, page_size, max_requests, table_width, dtype, device):
         self.spec, self.members = spec, list(members)
         self.capacity, self.page_size = int(num_pages), int(page_size)
-        if spec.shared_rows:   # one row per position: the key, whose leading columns are the value
+        if spec.bits:
+            if spec.bits != 4 or spec.shared_rows or spec.value_dim != spec.head_dim or not kv4.supports(spec.head_dim, page_size):
+                raise CacheError(f"4-bit pages hold keys and values of one size, 32, 64, ..., {kv4.MOST_DIM}, and a multiple of 8 positions, "
+                                 f"not {spec} on pages of {page_size}")
+            shape, dtype = (len(self.members), num_pages, *kv4.page_shape(spec.kv_heads, spec.head_dim, page_size)), torch.uint8
+        elif spec.shared_rows:   # one row per position: the key, whose leading columns are the value
             shape = (len(self.members), num_pages, 1, spec.kv_heads, page_size, spec.head_dim)
         elif spec.value_dim == spec.head_dim:
             shape = (len(self.members), num_pages, 2, spec.kv_heads, page_size, spec.head_dim)
@@ -148,6 +156,11 @@ class CacheManager:
         self.rows: dict = {}       # request -> row
         self.limits: dict = {}     # request -> reserved tokens or None
         self.progress: dict = {}   # request -> tokens written (all layers; a step is atomic)
+
+    def step_planners(self) -> dict:
+        """The planners of kernels that a cache of its own format needs: key -> StepPlanner."""
+        planners = [cache_planners[bits] for bits in sorted({g.spec.bits for g in self.kv_groups if g.spec.bits})]
+        return {planner.key: planner for planner in planners}
 
     # ------------------------------------------------------------------ sizes
     def pages_for(self, tokens):
@@ -311,7 +324,7 @@ class CacheManager:
                 return None
             if owner[0] == "kv":
                 g = self.kv_groups[owner[1]]
-                return KVCacheView(g.storage[owner[2]], g.dev_table, g.page_size, g.spec.window)
+                return KVCacheView(g.storage[owner[2]], g.dev_table, g.page_size, g.spec.window, g.spec.bits)
             return StateView(self.state_groups[owner[1]][2][owner[2]])
 
         result = []
@@ -327,9 +340,10 @@ class CacheManager:
         return result
 
     def poison(self, value=float("nan")) -> None:
-        """Fill every page with ``value`` (tests: reads of unwritten memory then show)."""
+        """Fill every page with ``value`` (tests: reads of unwritten memory then show); 4-bit pages with bytes of 255, whose steps
+        and bases are NaN."""
         for g in self.kv_groups:
-            g.storage.fill_(value)
+            g.storage.fill_(255 if g.spec.bits else value)
 
     # ------------------------------------------------------------------ checks
     def check_invariants(self) -> None:

@@ -38,14 +38,18 @@ class _Flight:
 
 class Engine:
     def __init__(self, model, *, num_pages=256, page_size=16, token_budget=128, prefill_chunk=64,
-                 max_active=4, clock=perf_counter, seed=0, use_graphs=True, overlap=False):
+                 max_active=4, clock=perf_counter, seed=0, use_graphs=True, overlap=False, kv_bits=None):
+        """``kv_bits``: 4 keeps the cache's keys and values in 4 bits (5 with the steps and bases of their groups of 32: 3.2 times the
+        positions of bfloat16 in the same memory), for models whose attention can read them; ``num_pages`` counts pages of
+        ``page_size`` positions either way.  None: in the run's dtype."""
         self.model = model
         self.overlap = bool(overlap)
         self.clock = clock
         self.seed = int(seed)
         self.next_id = 0
         self._in_flight = None        # the step that is on the GPU and whose tokens the host has not read
-        self.cache = CacheManager(model.cache_specs(), num_pages=num_pages, page_size=page_size,
+        specs = model.cache_specs() if kv_bits is None else model.cache_specs(kv_bits=kv_bits)
+        self.cache = CacheManager(specs, num_pages=num_pages, page_size=page_size,
                                   max_requests=max_active, max_context=model.max_positions,
                                   dtype=model.dtype, device=model.device, max_step_tokens=token_budget,
                                   request_state={"sampler": SLOT})

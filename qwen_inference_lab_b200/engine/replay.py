@@ -29,6 +29,7 @@ def build_parser():
     parser.add_argument("--max-tokens", required=True, type=int,
                         help="most tokens live requests hold at any time (each rounded up to 64)")
     parser.add_argument("--page-size", type=int, default=16, help="tokens per cache page (divides 64)")
+    parser.add_argument("--kv-bits", type=int, default=None, choices=[4], help="keep cached keys and values in 4 bits")
     parser.add_argument("--max-live", type=int, default=4, help="most requests alive at once (state slots)")
     return parser
 
@@ -50,7 +51,8 @@ def main(argv=None, stdin=None, stdout=None) -> int:
     dtype = resolve_dtype(args.dtype)
     model = load_model(args.model, device="cuda", dtype=dtype)
     pool_tokens = (args.max_tokens + 63) // 64 * 64
-    cache = CacheManager(model.cache_specs(), num_pages=pool_tokens // args.page_size, page_size=args.page_size,
+    specs = model.cache_specs() if args.kv_bits is None else model.cache_specs(kv_bits=args.kv_bits)
+    cache = CacheManager(specs, num_pages=pool_tokens // args.page_size, page_size=args.page_size,
                          max_requests=args.max_live, max_context=model.max_positions, dtype=dtype,
                          device=model.device)
     runner = StepRunner(model, cache, max_step_tokens=min(pool_tokens, 8192))

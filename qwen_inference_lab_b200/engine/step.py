@@ -61,7 +61,7 @@ class StepRunner:
         self.views = cache.views(model.order)
         self.use_graphs = bool(use_graphs) and self.device.type == "cuda" and model.is_graph_safe()
         self.graph_max_batch = graph_max_batch
-        planners = model.step_planners() if hasattr(model, "step_planners") else {}
+        planners = {**(model.step_planners() if hasattr(model, "step_planners") else {}), **cache.step_planners()}
         self.planners = [planners[key] for key in sorted(planners)]
         self._capacity = 0
         self._meta_dev = None

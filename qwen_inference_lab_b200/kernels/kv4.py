@@ -20,7 +20,6 @@ from types import SimpleNamespace
 import numpy as np
 import torch
 
-from ..parts.base import PlanView, Segments
 from . import attention_f32, attention_mma, attention_tc, build, ops, tuning
 from .ops import F32, KernelError, _check, _need, _p, _stream, dtype_code
 
@@ -349,7 +348,7 @@ def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, he
     table = array["table"][:count["table"]].view(segments, width)
     if q.dtype == torch.bfloat16:
         array["decode_info"], count["decode_info"] = None, 0
-        ctx = SimpleNamespace(plans={attention_mma.PLAN_KEY: PlanView(array, count)}, max_context=plan.max_context, min_context=0,
+        ctx = SimpleNamespace(plans={attention_mma.PLAN_KEY: SimpleNamespace(array=array, count=count)}, max_context=plan.max_context, min_context=0,
                               extras=extras, device=q.device)
         view = SimpleNamespace(pages=rows, block_table=table, page_size=READ_PAGE, window=window)
         attention_mma.attend(ctx, q, view, out, n_q_heads, n_kv_heads, head_dim, window, scale)

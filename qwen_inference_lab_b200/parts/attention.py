@@ -47,8 +47,8 @@ import math
 
 import torch
 
-from ..kernels import attention_f32, attention_mma, gemm_tc, ops
-from .base import KVCacheSpec, Mixer, Param, StateSpec, StepPlanner
+from ..kernels import attention_f32, attention_mma, gemm_tc, kv4, ops
+from .base import KVCacheSpec, Mixer, Param, StateSpec, StepPlanner, cache_planners
 from .linear import Linear, StackedLinear
 from .rotary import RotaryFrequencies
 
@@ -68,6 +68,21 @@ class PagedAttentionPlanner(StepPlanner):
 
 
 _PLANNER = PagedAttentionPlanner()
+
+
+class NarrowCachePlanner(StepPlanner):
+    """The host hook of the kernels over 4-bit pages (``kv4.describe_segments``), for every step over such a cache."""
+    key = kv4.PLAN_KEY
+
+    def plan(self, segments):
+        return kv4.describe_segments(segments.first, segments.starts, segments.lens, segments.rows)
+
+    def refresh_single_tokens(self, arrays, segments):
+        kv4.refresh_single_tokens(arrays, segments.starts)
+        return True
+
+
+cache_planners[4] = NarrowCachePlanner()
 
 
 def distance_rows(rows: int, farthest: int, count: int) -> list:
@@ -258,6 +273,16 @@ class GroupedQueryAttention(Mixer):
             return (pages, StateSpec((self.conv_taps - 1, self.qkv.out_features), torch.float32))
         return pages
 
+    def kv_bits_refusal(self, bits):
+        if self.head_dim % kv4.GROUP or self.head_dim > kv4.MOST_DIM or self.v_head_dim != self.head_dim:
+            return f"4-bit rows are of keys and values of one size, a multiple of {kv4.GROUP} up to {kv4.MOST_DIM}, " \
+                   f"not {self.head_dim} and {self.v_head_dim}"
+        if self.conv_taps or self.q_temperature is not None or self.distance_slopes is not None or self.modified_scores:
+            return "its scores or projections are changed in ways that the kernels over 4-bit pages do not have"
+        if self.whole_qk_norm_eps is not None or self.mixes_values:
+            return "norms over whole projections and mixed values are not written to 4-bit pages"
+        return None
+
     takes_norm = True
 
     @property
@@ -274,6 +299,8 @@ class GroupedQueryAttention(Mixer):
         applies the norm.  ``joint``: the rows of a product that holds the first projection already."""
         n = x.shape[0]
         n_kv = 0 if self.reads_shared_cache else self.n_kv_heads
+        if getattr(cache, "bits", 0):
+            return self._forward_narrow(ctx, x, cache, n_kv, residual, norm, out_scale, out_float32, joint)
         if self.frequency_tail:
             qkv, at = self.qkv.columns_of(ctx, x, joint, norm)
             q = ctx.empty((n, self.n_q_heads * self.head_dim))
@@ -360,6 +387,41 @@ class GroupedQueryAttention(Mixer):
                                ctx.token_row, cache.block_table, self.n_q_heads, n_kv, self.head_dim, cache.page_size)
         attended = ctx.empty((n, self.n_q_heads * self.head_dim))
         self._attend(ctx, q, cache, attended)
+        return self.out.forward(ctx, attended, residual=residual)
+
+    def _forward_narrow(self, ctx, x, cache, n_kv, residual, norm, out_scale, out_float32, joint):
+        """``forward`` over 4-bit pages: projection, its tail into the pages, attention over them."""
+        n = x.shape[0]
+        if self.frequency_tail:
+            qkv, at = self.qkv.columns_of(ctx, x, joint, norm)
+        else:
+            if out_float32 or out_scale is not None:
+                raise ValueError("a float32 result and an output scale are taken by the layers that rotate by frequencies only")
+            qkv, at = self.qkv.forward(ctx, x, norm=norm), 0
+        q_width, k_width = self.n_q_heads * self.head_dim, n_kv * self.head_dim
+        rotation = self.position
+        table = getattr(rotation, "table", None)
+        q = ctx.empty((n, q_width))
+        kv4.store(qkv, (at, at + q_width, at + (q_width if self.values_from_keys else q_width + k_width)), q, cache.pages, ctx.positions,
+                  ctx.token_row, cache.block_table, self.n_q_heads, n_kv, self.head_dim, cache.page_size,
+                  q_norm_w=self.q_norm.data if self.q_norm is not None else None,
+                  k_norm_w=self.k_norm.data if self.k_norm is not None else None,
+                  eps=self.qk_norm_eps or self.unit_qk_norm_eps or 0.0, unit_heads=self.unit_qk_norm_eps is not None, table=table,
+                  freq=rotation.freq if rotation is not None and table is None else None,
+                  rot_dims=rotation.rotary_dim if rotation is not None else 0, layout=getattr(rotation, "layout", ops.ROTARY_HALVES),
+                  gain=getattr(rotation, "gain", 1.0))
+        plan = ctx.shared.get(kv4.PLAN_KEY)
+        if plan is None:
+            plan = ctx.shared[kv4.PLAN_KEY] = kv4.StepPlan.of_step(ctx)
+        attended = ctx.empty((n, q_width))
+        kv4.attend(plan, q, cache.pages, attended, cache.block_table, self.n_q_heads, self.n_kv_heads, self.head_dim, cache.page_size,
+                   self.scale, window=self.window, extras=ctx.extras)
+        if self.head_gate:
+            ops.head_gate(attended, self.v_head_dim, qkv, at + self.qkv.out_features - self.n_q_heads)
+        if self.element_gate:
+            ops.head_gate(attended, 1, qkv, at + self.qkv.out_features - q_width)
+        if self.frequency_tail:
+            return self.out.forward(ctx, attended, residual=residual, out_scale=out_scale, out_float32=out_float32)
         return self.out.forward(ctx, attended, residual=residual)
 
     def _attend(self, ctx, q, cache, out):

@@ -69,6 +69,8 @@ class KVCacheSpec:
     (chunks counted from position 0), so pages of chunks that are over are given back as well.
     ``shared_rows``: a position's value is the leading ``v_head_dim`` columns of its key (all of it when 0), so a
     page holds one row per position and kv head and no value rows.
+    ``bits``: 0 holds rows in the run's dtype; 4 in groups of 32 elements, 4 bits each beside a step and a base of 16
+    bits a group (``kernels.kv4``), for mixers that say so (``Mixer.kv_bits_refusal``).
     """
     kv_heads: int
     head_dim: int
@@ -76,6 +78,7 @@ class KVCacheSpec:
     v_head_dim: int = 0
     chunk: int = 0
     shared_rows: bool = False
+    bits: int = 0
 
     @property
     def value_dim(self) -> int:
@@ -151,9 +154,18 @@ class PositionEncoding(Part):
     table: torch.Tensor | None = None
 
 
+#: Bits of a cache whose rows are not of the run's dtype -> the ``StepPlanner`` of the kernels over it: a step over such a cache
+#: needs that plan beside its parts' own.
+cache_planners: dict = {}
+
+
 class Mixer(Part):
     def cache_spec(self):
         return None
+
+    def kv_bits_refusal(self, bits) -> str | None:
+        """Why this mixer cannot keep its keys and values in ``bits`` bits; None if it can, or has none."""
+        return "it keeps keys and values in the run's dtype only"
 
     def forward(self, ctx, x, cache):
         raise NotImplementedError

@@ -12,12 +12,12 @@ run only for the positions whose logits were asked for, logits are float32.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
 from ..kernels import ops
-from .base import Param, Part
+from .base import KVCacheSpec, Mixer, Param, Part
 from .block import settle_stream
 from .linear import Linear
 
@@ -28,6 +28,18 @@ class LayerCall:
     order) of the earlier call whose cache this call reads, or None to own one."""
     layer: int
     reads_cache_of: int | None = None
+
+
+def _mixers(part) -> list:
+    """The part's mixers, those inside other mixers in their place."""
+    inner = [mixer for child in part.children() for mixer in _mixers(child)]
+    return inner or ([part] if isinstance(part, Mixer) else [])
+
+
+def _reads_pages(mixer) -> bool:
+    spec = mixer.cache_spec()
+    owns = any(isinstance(one, KVCacheSpec) for one in (spec if isinstance(spec, tuple) else (spec,)))
+    return owns or getattr(mixer, "reads_shared_cache", False)
 
 
 class TokenEmbedding(Part):
@@ -96,10 +108,22 @@ class DecoderModel(Part):
     def children(self):
         return [self.embedding, *self.layers, self.final_norm, self.head]
 
-    def cache_specs(self):
-        """One entry per call of the order: the cache it owns, or None."""
-        return [None if call.reads_cache_of is not None else self.layers[call.layer].cache_spec()
-                for call in self.order]
+    def cache_specs(self, kv_bits=None):
+        """One entry per call of the order: the cache it owns, or None.  ``kv_bits``: bits of a cached key or value, for models
+        whose every attention can read such a cache (None: the run's dtype)."""
+        specs = [None if call.reads_cache_of is not None else self.layers[call.layer].cache_spec()
+                 for call in self.order]
+        if kv_bits is None:
+            return specs
+        if kv_bits != 4:
+            raise ValueError(f"keys and values are kept in the run's dtype or in 4 bits, not in {kv_bits}")
+        for index, layer in enumerate(self.layers):
+            for mixer in _mixers(layer):
+                reason = mixer.kv_bits_refusal(kv_bits) if _reads_pages(mixer) else None
+                if reason:
+                    raise ValueError(f"layer {index} cannot keep keys and values in {kv_bits} bits: {reason}")
+        narrow = lambda one: replace(one, bits=kv_bits) if isinstance(one, KVCacheSpec) else one
+        return [tuple(narrow(one) for one in spec) if isinstance(spec, tuple) else narrow(spec) for spec in specs]
 
     def finalize(self, device, dtype):
         self.device, self.dtype = torch.device(device), dtype
