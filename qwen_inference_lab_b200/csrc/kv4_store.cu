@@ -6,7 +6,13 @@
 // beyond 2^17 loses 0.01 rad).  Without weights the norm may come after the turn ("unit heads").  Queries are rounded once to
 // their type and written; keys and values are cut into groups and coded.  Keys are computed in 64 bits: which code an element
 // gets is a step function of its value, and so is the same here as in any other arithmetic that keeps 64 bits, where in 32 bits one of
-// 10^6 elements would land on the other side of a border.  Queries have no borders and stay in 32 bits.
+// 10^5 elements would land on the other side of a border.  Queries have no borders and stay in 32 bits.
+//
+// 64-bit arithmetic is what such a kernel would take its time for, and hardly any element needs it: a row is computed in 32 bits first,
+// with a bound on what that may be off (12 roundings of the two products that a turn adds), and again in 64 bits only if a step, a
+// base or a code could come out otherwise within that bound (a few rows in a hundred).  The rest is instructions: a lane takes 8
+// neighbouring elements, so that a head of 128 is half a warp and a group's codes are one word of each of four lanes, and a token's
+// cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
 //
 // kv4_read: rows of requests as ordinary pages [page][2][kv head][slot][d] of float32 or bfloat16.
 #include "kv4.h"
@@ -34,22 +40,38 @@ struct Kv4Store {
     const int* token_row;
     const int* block_table;
     int table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages;
+    int vectors;                    // four elements are read and written at a time: columns, strides and pointers allow it
 };
 
-__device__ __forceinline__ double shfl_xor_double(double v, int mask) { return __shfl_xor_sync(0xffffffffu, v, mask); }
-
-// Elements 4 lane .. 4 lane + 3 of a row in every lane; the 8 lanes of a group agree on (s, m).  Returns the codes of the four and
-// the pair.
-__device__ __forceinline__ void quantise4(const double y[4], unsigned& codes, unsigned& pair) {
-    double lo = fmin(fmin(y[0], y[1]), fmin(y[2], y[3])), hi = fmax(fmax(y[0], y[1]), fmax(y[2], y[3]));
-    bool good = isfinite(y[0]) && isfinite(y[1]) && isfinite(y[2]) && isfinite(y[3]);
+__device__ __forceinline__ float shfl_xor(float v, int mask) { return __shfl_xor_sync(0xffffffffu, v, mask); }
+__device__ __forceinline__ double shfl_xor(double v, int mask) { return __shfl_xor_sync(0xffffffffu, v, mask); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+// Smallest and largest of a group, in its four lanes.
+template <typename R> __device__ __forceinline__ void range_of(const R (&y)[8], R& lo, R& hi) {
+    lo = smaller(smaller(smaller(y[0], y[1]), smaller(y[2], y[3])), smaller(smaller(y[4], y[5]), smaller(y[6], y[7])));
+    hi = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        lo = fmin(lo, shfl_xor_double(lo, o));
-        hi = fmax(hi, shfl_xor_double(hi, o));
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = smaller(lo, shfl_xor(lo, o));
+        hi = larger(hi, shfl_xor(hi, o));
     }
-    const unsigned votes = __ballot_sync(0xffffffffu, good);
-    good = ((votes >> (threadIdx.x & 24)) & 0xffu) == 0xffu;
+}
+__device__ __forceinline__ unsigned pair_of(bf16 step, bf16 base) {
+    return (unsigned)__bfloat16_as_ushort(base) << 16 | __bfloat16_as_ushort(step);
+}
+static constexpr unsigned NAN_PAIR = 0x7fc07fc0u;
+
+// Eight elements a lane, exact: the definition.
+__device__ __forceinline__ void code_exact(const double (&y)[8], unsigned& codes, unsigned& pair) {
+    double lo, hi;
+    range_of(y, lo, hi);
+    bool good = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) good = good && isfinite(y[i]);
+    good = ((__ballot_sync(0xffffffffu, good) >> (threadIdx.x & 28)) & 0xfu) == 0xfu;          // in all lanes of the group
     const bf16 base = __float2bfloat16_rn(__double2float_rn(lo));
     const bf16 step = __float2bfloat16_rn(__double2float_rn((hi - lo) / 15.0));
     const double m = (double)__bfloat162float(base), s = (double)__bfloat162float(step);
@@ -57,136 +79,311 @@ __device__ __forceinline__ void quantise4(const double y[4], unsigned& codes, un
     codes = 0;
     if (good && s > 0.0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) codes |= (unsigned)fmin(fmax(rint((y[i] - m) / s), 0.0), 15.0) << (4 * i);
+        for (int i = 0; i < 8; ++i) codes |= (unsigned)fmin(fmax(rint((y[i] - m) / s), 0.0), 15.0) << (4 * i);
     }
-    pair = good ? ((unsigned)__bfloat16_as_ushort(base) << 16 | __bfloat16_as_ushort(step)) : 0x7fc07fc0u;
+    pair = good ? pair_of(step, base) : NAN_PAIR;
+}
+// The same from elements of which those of this lane's group are off by `off` at most; false where that could make a difference.
+// Elements that are exact (off = 0) as their distances from the base are, as bfloat16 values are, lie between two codes often
+// (s times a half is a number like they are): the sign of (y - m) - (n + 1/2) s, one rounding, decides them, and 0 is a tie.
+__device__ __forceinline__ bool code_within(const float (&y)[8], float off, unsigned& codes, unsigned& pair) {
+    float lo, hi;
+    range_of(y, lo, hi);
+    const float range = hi - lo, wide = fmaf(range, 2.4e-7f, 2.f * off) * 1.001f;      // what the range may be off, its own rounding included
+    const bf16 base = __float2bfloat16_rn(lo - off), step = __float2bfloat16_rn((range - wide) * ((1.f / 15.f) * (1.f - 2.4e-7f)));
+    const bf16 base_up = __float2bfloat16_rn(lo + off), step_up = __float2bfloat16_rn((range + wide) * ((1.f / 15.f) * (1.f + 2.4e-7f)));
+    const float m = __bfloat162float(base), s = __bfloat162float(step);
+    bool sure = pair_of(step, base) == pair_of(step_up, base_up) && s > 1e-30f && hi < 1e30f && lo > -1e30f;
+    const float inverse = 1.f / s, most = 0.5f - fmaf(off, inverse, 8e-6f);            // 16 codes' three roundings are 3e-6
+    codes = 0;
+    float furthest = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = (y[i] - m) * inverse;
+        const float up = fminf(fmaxf(t, 0.f), 15.f) + 12582912.f;                      // 1.5 2^23: its last bits are the whole number, ties to even
+        furthest = fmaxf(furthest, fabsf(t - (up - 12582912.f)));
+        sum += t;                                                                      // NaN stays in a sum, not in a maximum
+        codes |= (__float_as_uint(up) & 15u) << (4 * i);
+    }
+    pair = pair_of(step, base);
+    sure = sure && sum == sum;
+    if (sure && off == 0.f && !(furthest < most)) {
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = y[i] - m, below = floorf(fminf(fmaxf(d * inverse, 0.f), 15.f));
+            const float side = fmaf(-(below + 0.5f), s, d);
+            const unsigned n = (unsigned)(int)below;
+            sure = sure && d + m == y[i] && y[i] - d == m;
+            codes |= min(n + (side > 0.f || (side == 0.f && (n & 1u)) ? 1u : 0u), 15u) << (4 * i);
+        }
+        return sure;
+    }
+    return sure && furthest < most;
 }
 
-// Sum over the warp, the same in every lane.
-__device__ __forceinline__ double sum_of(double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += shfl_xor_double(v, o);
-    return v;
-}
-__device__ __forceinline__ float sum_of(float v) { return warp_sum(v); }
-
-// One head of a token, normed and turned, in arithmetic R; y[q][i] is element 4 (lane + 32 q) + i.
-template <typename R, typename T, typename W>
-__device__ __forceinline__ void head_row(const Kv4Store& a, const float* __restrict__ x, const R* __restrict__ cs, const W* __restrict__ w,
-                                         int lane, R y[2][4]) {
-    const int dim = a.dim, half = a.rot_dims >> 1;
-    R r = (R)1;
-    if (a.norm == 1) {
-        R sq = 0;
-        for (int j = lane; j < dim; j += 32) sq += (R)x[j] * (R)x[j];
-        r = (R)1 / sqrt(sum_of(sq) / (R)dim + (R)a.eps);
+// Eight elements of a row as they lie there, and as floats.
+struct EightBf16 {
+    uint4 v;
+    __device__ __forceinline__ void load(const bf16* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void one_by_one(const bf16* p) {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+        v = make_uint4(u[0] | (unsigned)u[1] << 16, u[2] | (unsigned)u[3] << 16, u[4] | (unsigned)u[5] << 16, u[6] | (unsigned)u[7] << 16);
     }
-    R sq = 0;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    __device__ __forceinline__ void zero() { v = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ EightBf16 of_lane(int lane) const {
+        EightBf16 o;
+        o.v = make_uint4(__shfl_sync(0xffffffffu, v.x, lane), __shfl_sync(0xffffffffu, v.y, lane), __shfl_sync(0xffffffffu, v.z, lane), __shfl_sync(0xffffffffu, v.w, lane));
+        return o;
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int d = 4 * (lane + 32 * q) + i;
-            y[q][i] = 0;
-            if (d >= dim) continue;
-            R own = (R)x[d];
-            if (a.norm == 1) own = own * r * (R)to_f32<W>(w[d]);
-            if (d < a.rot_dims) {
-                const bool second = a.interleaved ? (d & 1) : d >= half;
-                const int other = a.interleaved ? (d ^ 1) : (second ? d - half : d + half);
-                const int pair = a.interleaved ? d >> 1 : (second ? other : d);
-                R partner = (R)x[other];
-                if (a.norm == 1) partner = partner * r * (R)to_f32<W>(w[other]);
-                const R c = cs[pair], s = cs[half + pair];
-                own = second ? own * c + partner * s : own * c - partner * s;
-            }
-            y[q][i] = own;
-            sq += own * own;
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
-    if (a.norm == 2) {
-        r = (R)1 / sqrt(sum_of(sq) / (R)dim + (R)a.eps);
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[q][i] *= r;
+};
+struct EightF32 {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = reinterpret_cast<const float4*>(p)[0];
+        b = reinterpret_cast<const float4*>(p)[1];
     }
+    __device__ __forceinline__ void one_by_one(const float* p) {
+        a = make_float4(p[0], p[1], p[2], p[3]);
+        b = make_float4(p[4], p[5], p[6], p[7]);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ EightF32 of_lane(int lane) const {
+        EightF32 o;
+        o.a = make_float4(__shfl_sync(0xffffffffu, a.x, lane), __shfl_sync(0xffffffffu, a.y, lane), __shfl_sync(0xffffffffu, a.z, lane), __shfl_sync(0xffffffffu, a.w, lane));
+        o.b = make_float4(__shfl_sync(0xffffffffu, b.x, lane), __shfl_sync(0xffffffffu, b.y, lane), __shfl_sync(0xffffffffu, b.z, lane), __shfl_sync(0xffffffffu, b.w, lane));
+        return o;
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+};
+template <typename T> struct Eight;
+template <> struct Eight<bf16> { typedef EightBf16 type; };
+template <> struct Eight<float> { typedef EightF32 type; };
+
+__device__ __forceinline__ unsigned two_bf16(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
 }
 
-// A block: a token and STORE_WARPS heads, a warp each.
-template <typename T, typename W>
-__global__ void __launch_bounds__(32 * STORE_WARPS) kv4_store_kernel(const Kv4Store a) {
-    __shared__ double angle_d[KV4_MAX_DIM];
-    __shared__ float angle_f[KV4_MAX_DIM];
-    __shared__ float rows[STORE_WARPS][KV4_MAX_DIM];
+// Sum over the lanes of a head.
+template <int LANES, typename R> __device__ __forceinline__ R head_sum(R v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += shfl_xor(v, o);
+    return v;
+}
+
+// Where an element's angle comes from: element d < rot_dims belongs to pair pair_of(d); its partner is other_of(d), and it is the second
+// of the two where second(d).
+struct Turn {
+    int rot_dims, half, interleaved;
+    __device__ __forceinline__ int other_of(int d) const { return d >= rot_dims ? d : interleaved ? d ^ 1 : d < half ? d + half : d - half; }
+    __device__ __forceinline__ int pair_at(int d) const { return interleaved ? d >> 1 : d < half ? d : d - half; }
+    __device__ __forceinline__ bool second(int d) const { return interleaved ? (d & 1) != 0 : d >= half; }
+};
+// Cosine and sine of a pair at a position, gain included.
+__device__ __forceinline__ void angle_of(const Kv4Store& a, int pos, int pair, double& c, double& s) {
+    if (a.table != nullptr) {
+        const float* row = a.table + (size_t)min(max(pos, 0), a.table_rows - 1) * a.rot_dims;
+        c = row[pair];
+        s = row[(a.rot_dims >> 1) + pair];
+    } else {
+        sincos((double)pos * (double)a.freq[pair], &s, &c);
+        c *= (double)a.gain;
+        s *= (double)a.gain;
+    }
+}
+struct EightPairs { float x[8], partner[8]; };
+// A warp's keys in 64 bits, and their codes.  Out of line: few rows come here, and its registers are twice the others'.
+template <typename W, int LANES>
+__device__ __noinline__ uint2 keys_exact(const Kv4Store* p, EightPairs e, int pos, int d0) {
+    const Kv4Store& a = *p;
+    const Turn turn = {a.rot_dims, a.rot_dims >> 1, a.interleaved};
+    const W* weight = reinterpret_cast<const W*>(a.k_weight);
+    double exact[8], r = 1.0, sq = 0.0;
+    if (a.norm == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq += (double)e.x[i] * (double)e.x[i];
+        r = 1.0 / sqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+        sq = 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        double u = (double)e.x[i], v = (double)e.partner[i];
+        if (a.norm == 1 && d < a.dim) {
+            u = u * r * (double)to_f32<W>(weight[d]);
+            v = v * r * (double)to_f32<W>(weight[turn.other_of(d)]);
+        }
+        if (d < a.rot_dims) {
+            double c, s;
+            angle_of(a, pos, turn.pair_at(d), c, s);
+            u = turn.second(d) ? u * c + v * s : u * c - v * s;
+        }
+        exact[i] = u;
+        sq += u * u;
+    }
+    if (a.norm == 2) {
+        r = 1.0 / sqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) exact[i] *= r;
+    }
+    uint2 found;
+    code_exact(exact, found.x, found.y);
+    return found;
+}
+__device__ __noinline__ uint2 values_exact(EightPairs e) {
+    double exact[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) exact[i] = (double)e.x[i];
+    uint2 found;
+    code_exact(exact, found.x, found.y);
+    return found;
+}
+
+// A block: a token and every (gridDim.y)th set of STORE_WARPS steps; a warp takes 32 / LANES heads of one kind a step, LANES lanes of 8
+// elements each (the first dim / 8 of them; a power of two).
+template <typename T, typename W, int LANES>
+__global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __grid_constant__ Kv4Store a) {
+    constexpr int HEADS = 32 / LANES;
+    // what an element and its partner are multiplied by: cosines times own weights, signed sines times partners', of queries and of keys
+    __shared__ __align__(16) float factor[2][2][8 * LANES];
     qil_wait_for_producer();
     qil_release_consumer();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, token = blockIdx.x;
-    const int pos = a.positions[token], half = a.rot_dims >> 1;
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        double c, s;
-        if (a.table != nullptr) {
-            const float* row = a.table + (size_t)min(max(pos, 0), a.table_rows - 1) * a.rot_dims;
-            c = row[i];
-            s = row[half + i];
-        } else {
-            sincos((double)pos * (double)a.freq[i], &s, &c);
-            c *= (double)a.gain;
-            s *= (double)a.gain;
-        }
-        angle_d[i] = c;
-        angle_d[half + i] = s;
-        angle_f[i] = (float)c;
-        angle_f[half + i] = (float)s;
+    const int pos = a.positions[token], half = a.rot_dims >> 1, groups = a.dim / KV4_GROUP;
+    const Turn turn = {a.rot_dims, half, a.interleaved};
+    int page = -1;
+    if (a.kv_heads) page = kv4_page(a.block_table + (size_t)a.token_row[token] * a.table_width, a.table_width, pos, a.page_size, a.num_pages);
+    for (int d = threadIdx.x; d < 8 * LANES; d += 32 * STORE_WARPS) {
+        double cosine = 1.0, sine = 0.0;
+        if (d < a.rot_dims) angle_of(a, pos, turn.pair_at(d), cosine, sine);
+        const float c = (float)cosine, s = turn.second(d) ? (float)sine : -(float)sine;
+        const bool weighs = a.norm == 1 && d < a.dim;
+        const W* q_weight = reinterpret_cast<const W*>(a.q_weight);
+        const W* k_weight = reinterpret_cast<const W*>(a.k_weight);
+        factor[0][0][d] = weighs ? c * to_f32<W>(q_weight[d]) : c;
+        factor[0][1][d] = weighs ? s * to_f32<W>(q_weight[turn.other_of(d)]) : s;
+        factor[1][0][d] = weighs ? c * to_f32<W>(k_weight[d]) : c;
+        factor[1][1][d] = weighs ? s * to_f32<W>(k_weight[turn.other_of(d)]) : s;
     }
     __syncthreads();
-    const int head = blockIdx.y * STORE_WARPS + warp;
-    if (head >= a.q_heads + 2 * a.kv_heads) return;
-    const bool is_q = head < a.q_heads, is_k = !is_q && head < a.q_heads + a.kv_heads;
-    const int kv = head - a.q_heads - (is_k ? 0 : a.kv_heads);
-    const int column = is_q ? a.q_col + head * a.dim : (is_k ? a.k_col : a.v_col) + kv * a.dim;
-    const T* src = reinterpret_cast<const T*>(a.proj) + (size_t)token * a.ld + column;
-    float* x = rows[warp];
-    for (int j = lane; j < a.dim; j += 32) x[j] = to_f32<T>(src[j]);
-    __syncwarp();
-    if (is_q) {
-        float y[2][4];
-        head_row<float, T, W>(a, x, angle_f, reinterpret_cast<const W*>(a.q_weight), lane, y);
-        T* dst = reinterpret_cast<T*>(a.q_out) + ((size_t)token * a.q_heads + head) * a.dim;
+    const int sub = lane / LANES, l = lane % LANES, d0 = 8 * l;
+    const int steps_q = (a.q_heads + HEADS - 1) / HEADS, steps_kv = (a.kv_heads + HEADS - 1) / HEADS;
+    // where a halves layout's other elements lie: whole lanes away, or anywhere
+    const bool by_lanes = half % 8 == 0;
+    const int other_lane = lane + (d0 >= a.rot_dims ? 0 : d0 < half ? half / 8 : -(half / 8));
+    float cw[8], sw[8];
+    int kind = -1;
+    // neighbouring steps for a warp: they are mostly of one kind
+    const int steps = steps_q + 2 * steps_kv, each = (steps + gridDim.y * STORE_WARPS - 1) / (gridDim.y * STORE_WARPS);
+    const int begin = (blockIdx.y * STORE_WARPS + warp) * each;
+    for (int step = begin; step < min(begin + each, steps); ++step) {
+        const int now = step < steps_q ? 0 : step < steps_q + steps_kv ? 1 : 2;              // queries, keys, values
+        if (now > 0 && page < 0) break;
+        const int head = (step - (now == 0 ? 0 : now == 1 ? steps_q : steps_q + steps_kv)) * HEADS + sub;
+        const bool mine = head < (now == 0 ? a.q_heads : a.kv_heads) && d0 < a.dim;
+        const T* src = reinterpret_cast<const T*>(a.proj) + (size_t)token * a.ld + (now == 0 ? a.q_col : now == 1 ? a.k_col : a.v_col) + (size_t)head * a.dim;
+        typename Eight<T>::type own, partner;
+        own.zero();
+        if (mine) {
+            if (a.vectors) own.load(src + d0);
+            else own.one_by_one(src + d0);
+        }
+        if (now != kind && now < 2) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 4 * (lane + 32 * q) + i;
-                if (d < a.dim) dst[d] = from_f32<T>(y[q][i]);
+            for (int i = 0; i < 8; i += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(&factor[now][0][d0 + i]), s = *reinterpret_cast<const float4*>(&factor[now][1][d0 + i]);
+                cw[i] = c.x; cw[i + 1] = c.y; cw[i + 2] = c.z; cw[i + 3] = c.w;
+                sw[i] = s.x; sw[i + 1] = s.y; sw[i + 2] = s.z; sw[i + 3] = s.w;
             }
-        return;
-    }
-    double y[2][4];
-    if (is_k) {
-        head_row<double, T, W>(a, x, angle_d, reinterpret_cast<const W*>(a.k_weight), lane, y);
-    } else {
+            kind = now;
+        }
+        float x[8], y[8], off = 0.f;
+        own.floats(x);
+        float xp[8];
+        if (now < 2) {
+            if (a.interleaved) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+                for (int i = 0; i < 8; ++i) xp[i] = x[i ^ 1];
+            } else if (by_lanes) {
+                partner = own.of_lane(other_lane & 31);
+                partner.floats(xp);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 4 * (lane + 32 * q) + i;
-                y[q][i] = d < a.dim ? (double)x[d] : 0.0;
+                for (int i = 0; i < 8; ++i) xp[i] = mine ? to_f32<T>(src[turn.other_of(d0 + i)]) : 0.f;
             }
-    }
-    const int page = kv4_page(a.block_table + (size_t)a.token_row[token] * a.table_width, a.table_width, pos, a.page_size, a.num_pages);
-    if (page < 0) return;
-    const int slot = pos % a.page_size, groups = a.dim / KV4_GROUP;
-    uint8_t* run = a.pages + kv4_run_at(page, is_k ? 0 : 1, kv, slot, a.kv_heads, a.page_size, groups);
+            float r = 1.f;
+            if (a.norm == 1) {
+                float sq = 0.f;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        if (128 * q >= a.dim) break;
+                for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
+                r = 1.f / sqrtf(head_sum<LANES>(sq) / (float)a.dim + a.eps);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float turned = xp[i] * sw[i];
+                y[i] = fmaf(x[i], cw[i], turned);
+                if (now == 1) off = fmaxf(off, fmaf(fabsf(x[i]), fabsf(cw[i]), fabsf(turned)));
+            }
+            if (a.norm == 2) {
+                float sq = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sq = fmaf(y[i], y[i], sq);
+                r = 1.f / sqrtf(head_sum<LANES>(sq) / (float)a.dim + a.eps);
+            }
+            if (a.norm) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] *= r;
+                off *= r;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i];
+        }
+        if (now == 0) {
+            if (mine) store8(reinterpret_cast<T*>(a.q_out) + ((size_t)token * a.q_heads + head) * a.dim + d0, y);
+            continue;
+        }
+        // 12 roundings of the two products; where the norm is of the turned head their errors go into its sum of squares, and so from
+        // any element into any other: up to 60 roundings of the largest (one large element among 255 equal ones)
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1)
+            if (o < 4 || a.norm == 2) off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, o));
         unsigned codes, pair;
-        quantise4(y[q], codes, pair);
-        const int d = 4 * (lane + 32 * q), group = d / KV4_GROUP;
-        if (d < a.dim) {
-            *reinterpret_cast<uint16_t*>(run + kv4_code_at(group, slot) + (lane & 7) * 2) = (uint16_t)codes;
-            if ((lane & 7) == 0) *reinterpret_cast<unsigned*>(run + kv4_pair_at(group, slot, groups)) = pair;
+        const bool sure = code_within(y, off * (a.norm == 2 ? 0x1p-18f : 0x1p-20f), codes, pair);
+        if (__any_sync(0xffffffffu, mine && !sure)) {
+            EightPairs e;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e.x[i] = x[i];
+                e.partner[i] = now == 1 ? xp[i] : 0.f;
+            }
+            const uint2 found = now == 1 ? keys_exact<W, LANES>(&a, e, pos, d0) : values_exact(e);
+            codes = found.x;
+            pair = found.y;
+        }
+        if (mine) {
+            const int slot = pos % a.page_size;
+            uint8_t* run = a.pages + kv4_run_at(page, now - 1, head, slot, a.kv_heads, a.page_size, groups);
+            *reinterpret_cast<unsigned*>(run + kv4_code_at(l >> 2, slot) + (l & 3) * 4) = codes;
+            if ((l & 3) == 0) *reinterpret_cast<unsigned*>(run + kv4_pair_at(l >> 2, slot, groups)) = pair;
         }
     }
 }
@@ -205,57 +402,70 @@ extern "C" int qil_kv4_store(const void* proj, long long ld, int q_col, int k_co
     if (q_heads < 0 || kv_heads < 0 || q_heads + kv_heads == 0) QIL_REFUSE("no heads");
     Kv4Store a = {proj, ld, q_col, k_col, v_col, q_out, (uint8_t*)pages, q_weight, k_weight, eps, norm, (const float*)table, table_rows,
                   (const float*)freq, gain, rot_dims, interleaved, (const int*)positions, (const int*)token_row, (const int*)block_table,
-                  table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages};
-    const dim3 grid(tokens, (q_heads + 2 * kv_heads + STORE_WARPS - 1) / STORE_WARPS);
-    QIL_DISPATCH_2(act, weight, qil_launch_chained(kv4_store_kernel<T, W>, grid, dim3(32 * STORE_WARPS), 0, stream, a));
+                  table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages, 0};
+    const int eight = act == QIL_BF16 ? 8 : 4;               // elements of 16 bytes
+    a.vectors = ld % eight == 0 && q_col % eight == 0 && k_col % eight == 0 && v_col % eight == 0 && (uintptr_t)proj % 16 == 0;
+    if ((uintptr_t)q_out % 16) QIL_REFUSE("queries out must start on a 16-byte boundary");
+    const int lanes = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32, heads = 32 / lanes;
+    const int steps = (q_heads + heads - 1) / heads + 2 * ((kv_heads + heads - 1) / heads), sets = (steps + STORE_WARPS - 1) / STORE_WARPS;
+    // a step a warp while that does not fill the GPU (148 SMs of 3 blocks), else all of a token's in one block: its angles are made once
+    const dim3 grid(tokens, tokens * sets <= 444 ? sets : 1);
+#define KV4_STORE(L)                                                                                                       \
+    if (lanes == L) QIL_DISPATCH_2(act, weight, qil_launch_chained(kv4_store_kernel<T, W, L>, grid, dim3(32 * STORE_WARPS), 0, stream, a))
+    KV4_STORE(4);
+    KV4_STORE(8);
+    KV4_STORE(16);
+    KV4_STORE(32);
     QIL_CHECK_LAUNCH();
 }
 
 // ------------------------------------------------------------------ rows back
-__device__ __forceinline__ unsigned two_bf16(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const unsigned*>(&v);
+// A warp: a run of 8 positions of a head's keys or values, groups one after the other: lane (position lane / 4, word lane % 4 of the
+// group), 8 elements.  A group of the run is 128 neighbouring bytes.  info: (table row, first position, positions, first page of out)
+// a segment; rows of positions without a page are zeros.
+static constexpr int READ_WARPS = 8;
+// element I of a word of codes as float, exact
+template <int I> __device__ __forceinline__ float code_float(unsigned word) {
+    return __uint_as_float((word >> (4 * I) & 15u) | 0x4b000000u) - 8388608.f;
 }
-
-// A thread: 8 neighbouring elements (one word of codes) of a position's key or value row.  info: (table row, first position,
-// positions, first page of out) a segment; rows of positions without a page are zeros.
-static constexpr int READ_THREADS = 256;
+__device__ __forceinline__ void eight_values(unsigned word, unsigned pair, float (&v)[8]) {
+    const float s = kv4_step(pair), m = kv4_base(pair);
+    v[0] = fmaf(s, code_float<0>(word), m); v[1] = fmaf(s, code_float<1>(word), m);
+    v[2] = fmaf(s, code_float<2>(word), m); v[3] = fmaf(s, code_float<3>(word), m);
+    v[4] = fmaf(s, code_float<4>(word), m); v[5] = fmaf(s, code_float<5>(word), m);
+    v[6] = fmaf(s, code_float<6>(word), m); v[7] = fmaf(s, code_float<7>(word), m);
+}
 template <typename T>
-__global__ void __launch_bounds__(READ_THREADS)
+__global__ void __launch_bounds__(32 * READ_WARPS)
 kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ block_table, int table_width, const int* __restrict__ info,
                 T* __restrict__ out, int out_pages, int out_page_size, int kv_heads, int dim, int page_size, int num_pages) {
     qil_wait_for_producer();
     qil_release_consumer();
-    const int* mine = info + 4 * blockIdx.z;
-    const int row = mine[0], first = mine[1], count = mine[2], out_first = mine[3];
-    const int words = dim >> 3, groups = dim / KV4_GROUP;
+    const int4 mine = reinterpret_cast<const int4*>(info)[blockIdx.z];
+    const int row = mine.x, first = mine.y, count = mine.z, out_first = mine.w;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = dim / KV4_GROUP;
     const int plane = blockIdx.y / kv_heads, head = blockIdx.y % kv_heads;
-    const long long at = (long long)blockIdx.x * READ_THREADS + threadIdx.x;
-    const int index = (int)(at / words), word = (int)(at % words);
-    if (index >= count) return;
+    // runs are of the pages' positions; a segment may begin inside one
+    const int pos = (first / 8 + blockIdx.x * READ_WARPS + warp) * 8 + (lane >> 2), index = pos - first;
+    if (index < 0 || index >= count) return;
     const int out_page = out_first + index / out_page_size;
     if (out_page < 0 || out_page >= out_pages) return;
-    const int pos = first + index;
     const int page = kv4_page(block_table + (size_t)row * table_width, table_width, pos, page_size, num_pages);
-    float v[8];
-    if (page >= 0) {
-        const int slot = pos % page_size, group = word >> 2;
-        const uint8_t* run = pages + kv4_run_at(page, plane, head, slot, kv_heads, page_size, groups);
-        const unsigned codes = *reinterpret_cast<const unsigned*>(run + kv4_code_at(group, slot) + (word & 3) * 4);
-        const unsigned pair = *reinterpret_cast<const unsigned*>(run + kv4_pair_at(group, slot, groups));
-        const float s = kv4_step(pair), m = kv4_base(pair);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(s, (float)((codes >> (4 * i)) & 15u), m);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    T* dst = out + ((((size_t)out_page * 2 + plane) * kv_heads + head) * out_page_size + index % out_page_size) * dim + (lane & 3) * 8;
+    if (page < 0) {
+        const float none[8] = {};
+        for (int g = 0; g < groups; ++g) store8(dst + g * KV4_GROUP, none);
+        return;
     }
-    T* dst = out + ((((size_t)out_page * 2 + plane) * kv_heads + head) * out_page_size + index % out_page_size) * dim + word * 8;
-    if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
-    } else {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    const int slot = pos % page_size;
+    const uint8_t* run = pages + kv4_run_at(page, plane, head, slot, kv_heads, page_size, groups);
+    const uint8_t* codes = run + kv4_code_at(0, slot) + (lane & 3) * 4;
+    const uint8_t* pairs = run + kv4_pair_at(0, slot, groups);
+#pragma unroll 4
+    for (int g = 0; g < groups; ++g) {
+        float v[8];
+        eight_values(*reinterpret_cast<const unsigned*>(codes + g * 128), *reinterpret_cast<const unsigned*>(pairs + 4 * g), v);
+        store8(dst + g * KV4_GROUP, v);
     }
 }
 
@@ -266,10 +476,8 @@ extern "C" int qil_kv4_read(const void* pages, const void* block_table, int tabl
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8 || out_page_size <= 0) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments > 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
-    const long long blocks = ((long long)longest * (dim / 8) + READ_THREADS - 1) / READ_THREADS;
-    if (blocks > 0x7fffffff) QIL_REFUSE("segments of %d positions", longest);
-    const dim3 grid((unsigned)blocks, 2 * kv_heads, segments);
-    QIL_DISPATCH_1(act, qil_launch_chained(kv4_read_kernel<T>, grid, dim3(READ_THREADS), 0, stream, (const uint8_t*)pages,
+    const dim3 grid((longest / 8 + 2 + READ_WARPS - 1) / READ_WARPS, 2 * kv_heads, segments);          // a segment may begin and end inside a run
+    QIL_DISPATCH_1(act, qil_launch_chained(kv4_read_kernel<T>, grid, dim3(32 * READ_WARPS), 0, stream, (const uint8_t*)pages,
                                            (const int*)block_table, table_width, (const int*)info, (T*)out, out_pages, out_page_size,
                                            kv_heads, dim, page_size, num_pages));
     QIL_CHECK_LAUNCH();

@@ -14,14 +14,14 @@ package the functions launch on torch's current stream, on the current device, a
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int, c_longlong
+from ctypes import c_float, c_int, c_longlong, c_void_p
 from types import SimpleNamespace
 
 import numpy as np
 import torch
 
 from . import attention_f32, attention_mma, attention_tc, build, ops, tuning
-from .ops import F32, KernelError, _check, _need, _p, _stream, dtype_code
+from .ops import F32, KernelError, _check, _need, dtype_code
 
 GROUP = 32
 MOST_DIM = 256
@@ -38,27 +38,56 @@ _lib = None
 _few_libs: dict = {}
 
 
+# The C entries' arguments: with these ctypes converts numbers itself, which takes a third of the time that an object per argument
+# does (the host's work is most of what a call on a few tokens takes).
+_P, _I, _F = c_void_p, c_int, c_float
+_STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 9 * [_I] + [_P]
+_READ = [_P, _P, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
+_SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
+_FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]
+
+
 def few_library_name(head_dim):
     """(name, defines) of the tensor-core library for heads of ``head_dim``."""
     return f"qil_kv4_d{head_dim}", {"QIL_HEAD_DIM": head_dim}
 
 
 def few_library(head_dim):
-    lib = _few_libs.get(head_dim)
-    if lib is None:
+    """(the library, its most spans, blocks an SM takes by tiles of rows) for heads of ``head_dim``."""
+    held = _few_libs.get(head_dim)
+    if held is None:
         name, defines = few_library_name(head_dim)
         lib = build.load(name, ["kv4_attention_mma.cu"], defines, depends=DEPENDS)
         if lib.qil_kv4_few_head_dim() != head_dim:
             raise KernelError("the 4-bit attention library was built for another head size")
-        _few_libs[head_dim] = lib
-    return lib
+        lib.qil_kv4_few.argtypes = _FEW
+        held = _few_libs[head_dim] = (lib, lib.qil_kv4_few_most_spans(), {nt: lib.qil_kv4_few_blocks_a_sm(c_int(nt)) for nt in (1, 2, 4)})
+    return held
 
 
 def library():
     global _lib
     if _lib is None:
-        _lib = build.load("qil_kv4", SOURCES, depends=DEPENDS)
+        lib = build.load("qil_kv4", SOURCES, depends=DEPENDS)
+        lib.qil_kv4_store.argtypes, lib.qil_kv4_read.argtypes, lib.qil_kv4_singles.argtypes = _STORE, _READ, _SINGLES
+        _lib = lib
     return _lib
+
+
+def _at(tensor):
+    return tensor.data_ptr() if tensor is not None else None
+
+
+def _stream():
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _take(tensor, name, dtype, ndim, device):
+    """``ops._need`` with what every call here asks, and the device: quick where all is well."""
+    if not (isinstance(tensor, torch.Tensor) and tensor.is_cuda and tensor.dtype is dtype and tensor.dim() == ndim and tensor.is_contiguous()):
+        _need(tensor, name, dtype, ndim)
+    if tensor.get_device() != device:
+        raise KernelError(f"{name} is on {tensor.device} while the current device is cuda:{device}")
 
 
 def supports(head_dim, page_size) -> bool:
@@ -73,20 +102,12 @@ def page_shape(n_kv_heads, head_dim, page_size) -> tuple:
     return (2, int(n_kv_heads), page_size // 8, 160 * (head_dim // GROUP))
 
 
-def _check_pages(pages, n_kv_heads, head_dim, page_size, what):
-    _need(pages, "pages", torch.uint8)
-    if tuple(pages.shape[1:]) != page_shape(n_kv_heads, head_dim, page_size):
+def _check_pages(pages, n_kv_heads, head_dim, page_size, what, device):
+    _take(pages, "pages", torch.uint8, 5, device)
+    if pages.shape[1:] != page_shape(n_kv_heads, head_dim, page_size):
         raise KernelError(f"{what}: cache layout {tuple(pages.shape)} for {n_kv_heads} heads of {head_dim}, pages of {page_size}")
     if pages.data_ptr() % 16:
         raise KernelError(f"{what}: pages must start on a 16-byte boundary")
-
-
-def _here(what, *tensors):
-    """All on the current device: a launch goes to its stream."""
-    current = torch.cuda.current_device()
-    for tensor in tensors:
-        if tensor is not None and tensor.device.index != current:
-            raise KernelError(f"{what}: a tensor on {tensor.device} while the current device is cuda:{current}")
 
 
 def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_heads, n_kv_heads, head_dim, page_size, *,
@@ -101,27 +122,39 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
     ``q_out`` [N, n_q_heads * head_dim], rounded once; keys (64-bit arithmetic until they are coded) and values go to the token's page.  A
     token whose position has no page writes none.  Two tokens of one call must not share a position of a request.  With n_kv_heads ==
     0 only queries are processed (``pages`` and ``block_table`` may be None)."""
-    _need(proj, "proj", ndim=2); _need(q_out, "q_out", proj.dtype, 2)
-    _need(positions, "positions", torch.int32, 1); _need(token_row, "token_row", torch.int32, 1)
+    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    if not isinstance(proj, torch.Tensor):
+        _need(proj, "proj")
+    dtype = proj.dtype
+    act = dtype_code(dtype)
+    _take(proj, "proj", dtype, 2, device); _take(q_out, "q_out", dtype, 2, device)
+    _take(positions, "positions", torch.int32, 1, device); _take(token_row, "token_row", torch.int32, 1, device)
     n, width = proj.shape
-    q_at, k_at, v_at = (int(c) for c in columns)
-    if not supports(head_dim, page_size):
-        page_shape(n_kv_heads, head_dim, page_size)
-    if n_q_heads < 1 or n_kv_heads < 0:
-        raise KernelError("kv4.store: head counts")
-    if min(q_at, k_at, v_at) < 0 or q_out.shape != (n, n_q_heads * head_dim) or positions.shape[0] < n or token_row.shape[0] < n \
-            or max(q_at + n_q_heads * head_dim, k_at + n_kv_heads * head_dim, v_at + n_kv_heads * head_dim) > width:
+    q_at, k_at, v_at = columns
+    if n_q_heads < 1 or n_kv_heads < 0 or not supports(head_dim, page_size):
+        raise KernelError(f"kv4.store: {n_q_heads} and {n_kv_heads} heads of {head_dim}, pages of {page_size}")
+    q_width, k_width = n_q_heads * head_dim, n_kv_heads * head_dim
+    if min(q_at, k_at, v_at) < 0 or q_out.shape != (n, q_width) or positions.shape[0] < n or token_row.shape[0] < n \
+            or max(q_at + q_width, k_at + k_width, v_at + k_width) > width:
         raise KernelError("kv4.store: shapes do not match the head counts")
+    table_width = num_pages = table_rows = 0
     if n_kv_heads:
-        _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.store"); _need(block_table, "block_table", torch.int32, 2)
+        _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.store", device)
+        _take(block_table, "block_table", torch.int32, 2, device)
+        num_pages, table_width = pages.shape[0], block_table.shape[1]
+    else:
+        pages = block_table = None
     norm, norm_code = 0, F32
     if q_norm_w is not None or k_norm_w is not None:
         if unit_heads:
             raise KernelError("kv4.store: heads of unit size have no norm weights")
-        _need(q_norm_w, "q_norm_w", ndim=1); _need(k_norm_w, "k_norm_w", q_norm_w.dtype, 1)
-        if q_norm_w.shape[0] != head_dim or k_norm_w.shape[0] != head_dim:
-            raise KernelError("kv4.store: norm weights must have head_dim elements")
+        if not isinstance(q_norm_w, torch.Tensor):
+            _need(q_norm_w, "q_norm_w")
         norm, norm_code = 1, dtype_code(q_norm_w.dtype)
+        for weight, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+            _take(weight, name, q_norm_w.dtype, 1, device)
+            if weight.shape[0] != head_dim:
+                raise KernelError("kv4.store: norm weights must have head_dim elements")
     elif unit_heads:
         norm = 2
     if rot_dims % 2 or not 0 <= rot_dims <= head_dim or layout not in (ops.ROTARY_HALVES, ops.ROTARY_INTERLEAVED):
@@ -130,25 +163,23 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
         if (table is None) == (freq is None):
             raise KernelError("kv4.store: a rotation comes from a table or from frequencies")
         if table is not None:
-            _need(table, "table", torch.float32, 2)
-            if table.shape[1] != rot_dims or table.shape[0] < 1 or gain != 1.0:
+            _take(table, "table", torch.float32, 2, device)
+            table_rows = table.shape[0]
+            if table.shape[1] != rot_dims or table_rows < 1 or gain != 1.0:
                 raise KernelError("kv4.store: a table holds rot_dims columns, a gain included")
         else:
-            _need(freq, "freq", torch.float32, 1)
+            _take(freq, "freq", torch.float32, 1, device)
             if freq.shape[0] != rot_dims // 2:
                 raise KernelError("kv4.store: one frequency per rotated pair")
-    _here("kv4.store", proj, q_out, pages if n_kv_heads else None, positions, token_row, block_table if n_kv_heads else None, q_norm_w,
-          k_norm_w, table, freq)
+    else:
+        table = freq = None
     if n == 0:
         return q_out
     lib = library()
     _check(lib, lib.qil_kv4_store(
-        _p(proj), c_longlong(width), c_int(q_at), c_int(k_at), c_int(v_at), _p(q_out), _p(pages if n_kv_heads else None), _p(q_norm_w),
-        _p(k_norm_w), c_float(float(eps)), c_int(norm), _p(table if rot_dims else None), c_int(table.shape[0] if table is not None else 0),
-        _p(freq if rot_dims else None), c_float(float(gain)), c_int(rot_dims), c_int(layout), _p(positions), _p(token_row),
-        _p(block_table if n_kv_heads else None), c_int(block_table.shape[1] if n_kv_heads else 0), c_int(n), c_int(n_q_heads), c_int(n_kv_heads),
-        c_int(head_dim), c_int(page_size), c_int(pages.shape[0] if n_kv_heads else 0), c_int(dtype_code(proj.dtype)), c_int(norm_code), _stream()),
-        "kv4.store")
+        proj.data_ptr(), width, q_at, k_at, v_at, q_out.data_ptr(), _at(pages), _at(q_norm_w), _at(k_norm_w), eps, norm, _at(table), table_rows,
+        _at(freq), gain, rot_dims, layout, positions.data_ptr(), token_row.data_ptr(), _at(block_table), table_width, n, n_q_heads, n_kv_heads,
+        head_dim, page_size, num_pages, act, norm_code, _stream()), "kv4.store")
     return q_out
 
 
@@ -159,19 +190,23 @@ def read(pages, block_table, info, segments, longest, out, n_kv_heads, head_dim,
     ``info`` int32 [segments * 4]: (block-table row, first position, positions, first page of ``out``) a segment; ``longest``: no segment
     has more positions.  Position first + i goes to slot i % (positions a page) of page i // (positions a page) after the segment's
     first.  Positions without a page are read as zeros; slots behind a segment's last position are left as they are."""
-    _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.read")
-    _need(block_table, "block_table", torch.int32, 2); _need(info, "info", torch.int32, 1); _need(out, "out", ndim=5)
-    if info.shape[0] < 4 * segments or segments < 0:
-        raise KernelError("kv4.read: four numbers a segment")
-    if out.shape[1] != 2 or out.shape[2] != n_kv_heads or out.shape[4] != head_dim or out.data_ptr() % 16:
+    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.read", device)
+    _take(block_table, "block_table", torch.int32, 2, device); _take(info, "info", torch.int32, 1, device)
+    if not isinstance(out, torch.Tensor):
+        _need(out, "out")
+    act = dtype_code(out.dtype)
+    _take(out, "out", out.dtype, 5, device)
+    if info.shape[0] < 4 * segments or segments < 0 or info.data_ptr() % 16:
+        raise KernelError("kv4.read: four numbers a segment, from a 16-byte boundary on")
+    out_pages, planes, heads, out_page_size, dim = out.shape
+    if planes != 2 or heads != n_kv_heads or dim != head_dim or out.data_ptr() % 16:
         raise KernelError(f"kv4.read: output {tuple(out.shape)} for {n_kv_heads} heads of {head_dim}")
-    _here("kv4.read", pages, block_table, info, out)
-    if segments == 0 or longest <= 0 or out.numel() == 0:
+    if segments == 0 or longest <= 0 or out_pages * out_page_size == 0:
         return out
     lib = library()
-    _check(lib, lib.qil_kv4_read(_p(pages), _p(block_table), c_int(block_table.shape[1]), _p(info), c_int(segments), c_int(int(longest)),
-                                 _p(out), c_int(out.shape[0]), c_int(out.shape[3]), c_int(n_kv_heads), c_int(head_dim), c_int(page_size),
-                                 c_int(pages.shape[0]), c_int(dtype_code(out.dtype)), _stream()), "kv4.read")
+    _check(lib, lib.qil_kv4_read(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], info.data_ptr(), segments, longest, out.data_ptr(),
+                                 out_pages, out_page_size, n_kv_heads, head_dim, page_size, pages.shape[0], act, _stream()), "kv4.read")
     return out
 
 
@@ -242,6 +277,7 @@ class StepPlan:
     def __init__(self, array, count, max_context, min_context=0, most_tokens=0):
         self.array, self.count = array, count
         self.most_tokens = int(most_tokens)          # of a segment
+        self.tokens = sum(count[name] for name in ("single_tokens", "few_tokens", "portion_tokens")) // 4
         self.max_context, self.min_context = int(max_context), int(min_context)
         self.batches = 0
         while f"b{self.batches}.read" in count:
@@ -301,35 +337,39 @@ def _spans(blocks_per_span, slots, plan, window, most) -> int:
 
 
 def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
+    """``attention_mma.decode_scratch``, and quickly where it is there already."""
+    held = extras.get("attn_decode_scratch")
+    slots = tokens * n_q_heads * n_spans
+    if held is not None and held[0].numel() >= slots * head_dim and held[1].numel() >= 2 * slots and len(held) == 3 \
+            and held[2].numel() >= tokens * n_q_heads:
+        return held
     return attention_mma.decode_scratch(SimpleNamespace(extras=extras, device=device), tokens, n_q_heads, n_spans, head_dim,
                                         most=attention_f32.MOST_SCRATCH)
 
 
 def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
-    lib = few_library(head_dim)
+    lib, most, blocks_a_sm = few_library(head_dim)
     rows = most_tokens * (n_q_heads // n_kv_heads)
     nt = 1 if rows <= 8 else 2 if rows <= 16 or head_dim > 128 else 4
     blocks = n * n_kv_heads * -(-rows // (8 * nt))
     # the partial sums of all spans: fewer spans where they would outgrow their limit
-    most = min(lib.qil_kv4_few_most_spans(), attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
-    n_spans = _spans(blocks, _slots(lib.qil_kv4_few_blocks_a_sm(c_int(nt))), plan, window, most)
+    most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
+    n_spans = _spans(blocks, _slots(blocks_a_sm[nt]), plan, window, most)
     part_o, part_ml, tickets = _scratch(extras, q.device, tokens, n_q_heads, n_spans, head_dim)
-    _check(lib, lib.qil_kv4_few(_p(q), _p(pages), _p(out), _p(info), c_int(n), c_int(most_tokens), c_int(nt), _p(part_o), _p(part_ml), _p(tickets),
-                                c_int(n_spans), _p(block_table), c_int(block_table.shape[1]), c_int(n_q_heads), c_int(n_kv_heads), c_int(page_size),
-                                c_int(pages.shape[0]), c_int(window), c_float(scale), _stream()), "kv4.attend (few tokens)")
+    _check(lib, lib.qil_kv4_few(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, most_tokens, nt, part_o.data_ptr(),
+                                part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads,
+                                n_kv_heads, page_size, pages.shape[0], window, scale, _stream()), "kv4.attend (few tokens)")
 
 
 def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib = library()
-    share = n_q_heads // n_kv_heads
-    chunks = -(-share // lib.qil_kv4_singles_heads(c_int(share)))
+    chunks = -(-(n_q_heads // n_kv_heads) // lib.qil_kv4_singles_heads(n_q_heads // n_kv_heads))
     most = attention_f32.MOST_SCRATCH // (4 * n * n_q_heads * head_dim)
     n_spans = _spans(n * n_kv_heads * chunks, _slots(3), plan, window, most)
     part_o, part_ml, tickets = _scratch(extras, q.device, n, n_q_heads, n_spans, head_dim)
-    _check(lib, lib.qil_kv4_singles(_p(q), _p(pages), _p(out), _p(info), c_int(n), _p(part_o), _p(part_ml), _p(tickets), c_int(n_spans),
-                                    _p(block_table), c_int(block_table.shape[1]), c_int(n_q_heads), c_int(n_kv_heads), c_int(head_dim),
-                                    c_int(page_size), c_int(pages.shape[0]), c_int(window), c_float(scale), c_int(dtype_code(q.dtype)), _stream()),
-           "kv4.attend (single tokens)")
+    _check(lib, lib.qil_kv4_singles(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, part_o.data_ptr(), part_ml.data_ptr(),
+                                    tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads, n_kv_heads, head_dim,
+                                    page_size, pages.shape[0], window, scale, dtype_code(q.dtype), _stream()), "kv4.attend (single tokens)")
 
 
 def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
@@ -364,16 +404,20 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
     are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Positions whose page the block
     table does not have are not seen; a token that sees none gets zeros.  ``extras``: a dict that the caller keeps from call to call
     for the scratch memory; calls that may run at the same time (other streams) need one each."""
-    _need(q, "q", ndim=2); _need(out, "out", q.dtype, 2); _need(block_table, "block_table", torch.int32, 2)
+    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    if not isinstance(q, torch.Tensor):
+        _need(q, "q")
     dtype_code(q.dtype)
-    _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.attend")
+    _take(q, "q", q.dtype, 2, device); _take(out, "out", q.dtype, 2, device); _take(block_table, "block_table", torch.int32, 2, device)
+    _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.attend", device)
     if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads:
         raise KernelError(f"kv4.attend: {n_q_heads} query heads do not divide into {n_kv_heads} kv heads")
     if q.shape[1] != n_q_heads * head_dim or out.shape != q.shape:
         raise KernelError(f"kv4.attend: queries {tuple(q.shape)}, output {tuple(out.shape)}")
-    if window < 0:
-        raise KernelError("kv4.attend: a window cannot be negative")
-    _here("kv4.attend", q, pages, out, block_table, plan.array["singles"])
+    if window < 0 or not scale > 0:
+        raise KernelError("kv4.attend: a window cannot be negative, and a scale is a positive number")
+    if plan.array["singles"].get_device() != device or q.shape[0] < plan.tokens:
+        raise KernelError(f"kv4.attend: a plan of {plan.tokens} tokens on {plan.array['singles'].device} for queries {tuple(q.shape)}")
     shape = (q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, float(scale), int(window), extras)
     count, array = plan.count, plan.array
     if q.dtype == torch.float32:
