@@ -80,7 +80,7 @@ __device__ __forceinline__ unsigned max_pairs(unsigned a, unsigned b) {
 }
 __device__ __forceinline__ unsigned transposed(unsigned v) {
     unsigned r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ unsigned pack_bf16(float low, float high) {
@@ -185,30 +185,53 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) issue(s);
 
-    // ---- queries: a warp a row, a lane D / 32 dimensions; times 2^up the row's largest lies in [2^99, 2^100)
+    // ---- queries: a warp a row, a lane 4 neighbouring dimensions (twice beyond 128); times 2^up the row's largest lies in [2^99, 2^100)
     for (int of = warp; of < 8 * NT; of += WARPS) {
+        constexpr int QUADS = (D + 127) / 128;
         const int row = row0 + of;
-        float q[G], most_q = 0.f;
-        const bf16* src = a.q + ((size_t)(first_token + min(row, all_rows - 1) / share) * a.q_heads + kv * share + min(row, all_rows - 1) % share) * D;
+        if (row >= all_rows) {                              // nobody's: zeros
+            for (int i = lane; i < 4 * G; i += 32) q_frag[(i >> 2) * NT + of / 8][(of & 7) * 4 + (i & 3)] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = lane; i < 2 * G; i += 32) q_sums[of][i] = 0u;
+            if (lane == 0) q_unit[of] = 1.f;
+            continue;
+        }
+        float q[QUADS][4], most_q = 0.f;
+        const bf16* src = a.q + ((size_t)(first_token + row / share) * a.q_heads + kv * share + row % share) * D;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            q[g] = row < all_rows ? __bfloat162float(src[g * KV4_GROUP + lane]) : 0.f;
-            most_q = fmaxf(most_q, fabsf(q[g]));
+        for (int n = 0; n < QUADS; ++n) {
+            const int d = 4 * (lane + 32 * n);
+            const uint2 w = d < D ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0u, 0u);
+            q[n][0] = kv4_step(w.x); q[n][1] = kv4_base(w.x); q[n][2] = kv4_step(w.y); q[n][3] = kv4_base(w.y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most_q = fmaxf(most_q, fabsf(q[n][i]));
         }
         most_q = warp_max(most_q);
         const int up = most_q > 0.f && most_q < INFINITY ? 99 - ilogbf(most_q) : 0;
-        // lane's dimension is 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one
-        const float mine = lane & 1 ? 0.0625f : 1.f;
+        // 2^up in two factors: it may be beyond float32.  The sums are counted like the products of codes, 2^-133.
+        const float up1 = __uint_as_float((unsigned)(127 + up / 2) << 23), up2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float x = scalbnf(q[g], up);
-            const float sum = scalbnf(warp_sum(x), -133);
-            bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 3)]) + (lane & 3) * 2 + (lane >> 2 & 1);
-            *to = __float2bfloat16_rn(x * mine);
-            if (lane == 0) {
-                const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
-                q_sums[of][2 * g] = pack_bf16(first, second);
-                q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+        for (int n = 0; n < QUADS; ++n) {
+            const int d = 4 * (lane + 32 * n), g = d / KV4_GROUP;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[n][i] = q[n][i] * up1 * up2;
+            float sum = (q[n][0] + q[n][1]) + (q[n][2] + q[n][3]);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum = sum * 0x1p-100f * 0x1p-33f;
+            if (d < D) {
+                // dimension 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one; odd ones meet
+                // codes that lie four bits higher
+                bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 1 & 3)]) + (lane & 1);
+                to[0] = __float2bfloat16_rn(q[n][0]);
+                to[2] = __float2bfloat16_rn(q[n][1] * 0.0625f);
+                to[4] = __float2bfloat16_rn(q[n][2]);
+                to[6] = __float2bfloat16_rn(q[n][3] * 0.0625f);
+                if ((lane & 7) == 0) {
+                    const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
+                    q_sums[of][2 * g] = pack_bf16(first, second);
+                    q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+                }
             }
         }
         if (lane == 0) q_unit[of] = scalbnf(a.scale_log2, 133 - up);
@@ -234,8 +257,10 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         unit[nt][1] = q_unit[nt * 8 + 2 * c + 1];
     }
 
-    float acc[NT][G][2][4], side[NT][4], less[NT][4];
-    // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p (m + 8 s)), row 8 sum(p); less: row g -8 sum(p s), as acc's row
+    float acc[NT][G][2][4], side[NT][4], less[NT][(G + 1) / 2][4];
+    // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p (m + 8 s)), row 8 sum(p).
+    // less: -8 sum(p s) times 2^(lift - 133) with p s as the first operand: query row r, of two groups the even one in columns 0 .. 3 and
+    // the odd one in 4 .. 7, keys 0 .. 7 in row r and 8 .. 15 in row 8 + r
     float most[NT][2];                          // of rows 2 c, 2 c + 1
     int lift = MOST_LIFT;                       // p s stays below 2^108, so that it overflows nowhere, and far above 2^7
     unsigned lift_limit = (100 - MOST_LIFT + 128) << 7;                       // a step of that many bits or more (NaN too) asks for another lift
@@ -247,7 +272,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[nt][g][0][i] = acc[nt][g][1][i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) side[nt][i] = less[nt][i] = 0.f;
+        for (int i = 0; i < 4; ++i) {
+            side[nt][i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] = 0.f;
+        }
         most[nt][0] = most[nt][1] = -INFINITY;
         marked[nt][0] = marked[nt][1] = 0u;
     }
@@ -260,6 +289,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     for (int nt = 0; nt < NT; ++nt) minus[nt][0] = minus[nt][1] = (float)MOST_LIFT;
     unsigned sink = (127 - MOST_LIFT) << 7 | (127 - MOST_LIFT) << 23;         // 2^-lift, twice
     const unsigned one = r == 0 ? 0x3f803f80u : 0u;
+    const unsigned eight0 = r < 4 ? 0x80088008u : 0u, eight1 = r < 4 ? 0u : 0x80088008u;      // codes of -8
     // tiles of keys that every row sees begin in [plain_low, plain_low + plain_more]
     const int plain_low = max(span.first, a.window > 0 ? pos_high - a.window + 1 : 0);
     const int plain_more = min(pos_low - TILE + 1, span.last - TILE) - plain_low;
@@ -362,7 +392,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                             acc[nt][g][1][i] *= by;
                         }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) less[nt][i] *= by;
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= by;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) minus[nt][i] += (float)(lower - lift);
                 }
@@ -419,10 +451,12 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                         acc[nt][g][1][i] *= keep[i & 1];
                     }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    side[nt][i] *= keep[i & 1];
-                    less[nt][i] *= keep[i & 1];
-                }
+                for (int i = 0; i < 4; ++i) side[nt][i] *= keep[i & 1];
+                const float even = __shfl_sync(0xffffffffu, keep[0], r >> 1), odd = __shfl_sync(0xffffffffu, keep[1], r >> 1);     // of row r
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= r & 1 ? odd : even;
             }
         }
 #pragma unroll
@@ -460,6 +494,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma(side[nt], base0, one, base1, one, times_bf16(p0[u][nt], sink), times_bf16(p1[u][nt], sink));
+            unsigned ps[NT][G][2];                                 // p s of the groups
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const unsigned char* at0 = run0 + g * 128 + (r >> 1) * 4;
@@ -467,13 +502,14 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 const unsigned x = __byte_perm(*reinterpret_cast<const unsigned*>(at0 + c * 16), *reinterpret_cast<const unsigned*>(at0 + (c + 4) * 16), half);
                 const unsigned y = __byte_perm(*reinterpret_cast<const unsigned*>(at1 + c * 16), *reinterpret_cast<const unsigned*>(at1 + (c + 4) * 16), half);
                 const unsigned xs = x >> 8, ys = y >> 8;
-                const unsigned eight = r == g ? 0x80088008u : 0u;          // a code of -8 in row g
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const unsigned b0 = times_bf16(p0[u][nt], steps0[g]), b1 = times_bf16(p1[u][nt], steps1[g]);
-                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0, b1);
-                    mma(less[nt], eight, 0u, eight, 0u, b0, b1);
-                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, b0, b1);
+                    ps[nt][g][0] = times_bf16(p0[u][nt], steps0[g]);
+                    ps[nt][g][1] = times_bf16(p1[u][nt], steps1[g]);
+                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, ps[nt][g][0], ps[nt][g][1]);
+                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, ps[nt][g][0], ps[nt][g][1]);
+                    if (g & 1) mma(less[nt][g / 2], ps[nt][g - 1][0], ps[nt][g - 1][1], ps[nt][g][0], ps[nt][g][1], eight0, eight1);
+                    else if (g == G - 1) mma(less[nt][g / 2], ps[nt][g][0], ps[nt][g][1], 0u, 0u, eight0, eight1);
                 }
             }
         }
@@ -500,7 +536,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float middle = __shfl_sync(0xffffffffu, side[nt][i], 4 * g + c), eights = __shfl_sync(0xffffffffu, less[nt][i], 4 * g + c);
+                const float middle = __shfl_sync(0xffffffffu, side[nt][i], 4 * g + c), eights = __shfl_sync(0xffffffffu, less[nt][g / 2][0] + less[nt][g / 2][2], 4 * (2 * c + i) + 2 * (g & 1));
                 const float add = (marked[nt][i] >> g & 1) ? __int_as_float(0x7fc00000) : fmaf(eights * 0x1p100f, down, middle);
                 float4 o;                                  // 2^133 2^-lift is beyond float32 for a lift below 6: in two steps
                 o.x = fmaf(acc[nt][g][0][i] * 0x1p100f, down, add);

@@ -84,10 +84,23 @@ def _stream():
 
 def _take(tensor, name, dtype, ndim, device):
     """``ops._need`` with what every call here asks, and the device: quick where all is well."""
-    if not (isinstance(tensor, torch.Tensor) and tensor.is_cuda and tensor.dtype is dtype and tensor.dim() == ndim and tensor.is_contiguous()):
-        _need(tensor, name, dtype, ndim)
-    if tensor.get_device() != device:
-        raise KernelError(f"{name} is on {tensor.device} while the current device is cuda:{device}")
+    try:
+        if tensor.dtype is dtype and tensor.get_device() == device and tensor.dim() == ndim and tensor.is_contiguous():
+            return
+    except AttributeError:
+        pass
+    _need(tensor, name, dtype, ndim)
+    raise KernelError(f"{name} is on {tensor.device} while the current device is cuda:{device}")
+
+
+def _device_of(tensor, name):
+    """The current device, which ``tensor`` is on: a launch goes to its stream."""
+    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
+        _need(tensor, name)
+    device = tensor.get_device()
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} is on {tensor.device} while the current device is cuda:{torch._C._cuda_getDevice()}")
+    return device
 
 
 def supports(head_dim, page_size) -> bool:
@@ -122,9 +135,7 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
     ``q_out`` [N, n_q_heads * head_dim], rounded once; keys (64-bit arithmetic until they are coded) and values go to the token's page.  A
     token whose position has no page writes none.  Two tokens of one call must not share a position of a request.  With n_kv_heads ==
     0 only queries are processed (``pages`` and ``block_table`` may be None)."""
-    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
-    if not isinstance(proj, torch.Tensor):
-        _need(proj, "proj")
+    device = _device_of(proj, "proj")
     dtype = proj.dtype
     act = dtype_code(dtype)
     _take(proj, "proj", dtype, 2, device); _take(q_out, "q_out", dtype, 2, device)
@@ -190,7 +201,7 @@ def read(pages, block_table, info, segments, longest, out, n_kv_heads, head_dim,
     ``info`` int32 [segments * 4]: (block-table row, first position, positions, first page of ``out``) a segment; ``longest``: no segment
     has more positions.  Position first + i goes to slot i % (positions a page) of page i // (positions a page) after the segment's
     first.  Positions without a page are read as zeros; slots behind a segment's last position are left as they are."""
-    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    device = _device_of(pages, "pages")
     _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.read", device)
     _take(block_table, "block_table", torch.int32, 2, device); _take(info, "info", torch.int32, 1, device)
     if not isinstance(out, torch.Tensor):
@@ -404,9 +415,7 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
     are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Positions whose page the block
     table does not have are not seen; a token that sees none gets zeros.  ``extras``: a dict that the caller keeps from call to call
     for the scratch memory; calls that may run at the same time (other streams) need one each."""
-    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
-    if not isinstance(q, torch.Tensor):
-        _need(q, "q")
+    device = _device_of(q, "q")
     dtype_code(q.dtype)
     _take(q, "q", q.dtype, 2, device); _take(out, "out", q.dtype, 2, device); _take(block_table, "block_table", torch.int32, 2, device)
     _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.attend", device)
