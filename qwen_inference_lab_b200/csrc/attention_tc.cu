@@ -19,6 +19,11 @@
 //               and the rescale of O in tensor memory when the running maximum moved by more than
 //               2^8 (until then P is computed against the older maximum, which is exact algebra and
 //               safe in float32), in tiles of fewer tokens whenever it moved; finally O / l -> global memory.
+// With -DQIL_KEYS_F16=1 queries and keys are float16, each query row and each page of keys with a power of two of its own taken out, which
+// the softmax multiplies back (pages of 64: a tile's scores have one factor); values, P and the output are bfloat16 as ever.  Rows that were
+// held in fewer bits and are read back for this kernel have more than bfloat16's 8: as bfloat16 keys they are off by 2^-9, which
+// scores of some size turn into a weight's error several times that of its own rounding.  Value groups that are NaN come as zeros and
+// marks: a row that sees a mark gets NaN there, one that masks it does not.
 // K tiles are K-major operands and V tiles MN-major operands of the same shared-memory image
 // ([key][64 elements = 128 bytes] x the slabs of the head).
 //
@@ -51,6 +56,9 @@ static_assert(AT_D % 16 == 0 && AT_D >= 16 && AT_D <= 128 && AT_E % 16 == 0 && A
 #define AT_VTILE (AT_ES * AT_SLAB)    // a V tile
 #define AT_TMEM_COLS (AT_N == 64 ? 256 : 512)
 #define AT_STAGES 2
+#ifndef QIL_KEYS_F16
+#define QIL_KEYS_F16 0
+#endif
 
 __device__ __forceinline__ void at_tma_3d(void* smem, const CUtensorMap* map, unsigned long long* bar, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
@@ -147,6 +155,12 @@ struct AtParams {
     float tanh_arg, cap_log2;
     int* error_word;
     long long* trace;           // only read when compiled with AT_TRACE
+#if QIL_KEYS_F16
+    const float* q_factor;              // [N, Hq]: what a row of the float16 queries is multiplied by
+    const float* key_factor;            // [page][kv head]: what a page's float16 keys are
+    const int* value_marks;             // [page][kv head]: does any value group of the page have a mark?
+    const unsigned char* marks;         // [page][kv head][64]: bit g: group g of 32 columns of that position's value is NaN
+#endif
 };
 
 #define AT_VALUE_WARP 6                  // warps: 0 keys, 1 MMA issue, 2-5 softmax, 6 values
@@ -276,7 +290,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     } else if (warp == 1) {
         // bfloat16 -> float32, M = 128; scores: N = keys; output: N = the value slabs' columns, B (V) read MN-major
         const bool leader = elect_one();
-        const unsigned idesc_s = umma_idesc(AT_M, AT_N);
+        const unsigned idesc_s = umma_idesc(AT_M, AT_N) & (QIL_KEYS_F16 ? ~((1u << 7) | (1u << 10)) : ~0u);      // float16 operands: zeros there
         const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AT_ES * 64 >> 3) << 17) | ((unsigned)(AT_M >> 4) << 24);
         bool ok = warp_mbar_wait(&sh->q_full, 0);
         if (!ok && leader) atomicExch(p.error_word, 13);
@@ -331,7 +345,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const bool capped = p.cap_log2 > 0.f;
         const bool biased = p.slopes_log2 != nullptr;
         const float slope = biased ? p.slopes_log2[head] : 0.f;
+#if QIL_KEYS_F16
+        const float row_scale = p.scale_log2 * p.q_factor[(size_t)(n0 + min(row, rows - 1)) * p.n_q_heads + head];
+        float my_factor = 1.f;                                // of tile j / 32 * 32 + lane
+        int my_page = 0;
+        unsigned marked = 0u;                                 // groups of which this row sees a mark
+#else
         const float scale_later = (biased || capped) ? 1.0f : p.scale_log2;
+#endif
         // A tile of fewer than 128 tokens moves its maximum whenever it grows, as the 64-token kernel (attention_mma.cu)
         // that would take it does: a largest weight of exactly 1 has no rounding, and with the slack the error against 64
         // bits was up to 1.07 of that kernel's.
@@ -341,6 +362,20 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         for (int j = 0; j < n_tiles && ok; ++j) {
             const int buf = j & 1, stage = j % AT_STAGES;
             if (warp == 2 && lane == 0) AT_STAMP(2, 6 * j);
+#if QIL_KEYS_F16
+            if (j % 32 == 0) {
+                const int index = tile0 + j + lane;
+                const int page = (index <= hi / AT_N && index < p.table_stride) ? table[index] : -1;
+                my_page = page < 0 ? -1 : page * p.n_kv_heads + kv_head;
+                my_factor = my_page < 0 ? 1.f : p.key_factor[my_page];
+                if (my_page >= 0 && p.value_marks[my_page] == 0) my_page = -1;
+            }
+            const float scale_later = row_scale * __shfl_sync(0xffffffffu, my_factor, j % 32);
+            const int marks_at = __shfl_sync(0xffffffffu, my_page, j % 32);
+            if (marks_at >= 0)
+                for (int i = 0; i < AT_N; ++i)
+                    if ((tile0 + j) * AT_N + i <= pos && (tile0 + j) * AT_N + i >= lo) marked |= p.marks[(size_t)marks_at * AT_N + i];
+#endif
             if (!warp_mbar_wait(&sh->s_full[buf], (j >> 1) & 1)) { if (lane == 0) atomicExch(p.error_word, 21); ok = false; break; }
             if (warp == 2 && lane == 0) AT_STAMP(2, 6 * j + 1);
             tc_fence_after();
@@ -488,6 +523,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     bf16* o = reinterpret_cast<bf16*>(&packed);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(__uint_as_float(r[q * 8 + i]) * inv);
+#if QIL_KEYS_F16
+                    if (marked >> c & 1u) packed = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+#endif
                     if (row < rows) *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = packed;
                 }
             }
@@ -528,6 +566,7 @@ extern "C" int qil_attn_tc_keys_per_tile() { return AT_N; }
 // caller once.  trace: null, or 3 * 1024 int64 for the time stamps of block (0, 0) in a build with AT_TRACE.
 // slopes_log2: null, or float32 [n_q_heads] on the device: a distance bias per query head (see AtParams).
 // chunk, window, sink_log2 (null, or float32 [n_q_heads] on the device): see AtParams.  softcap > 0: capped scores.
+#if !QIL_KEYS_F16
 extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,
                                           int n_tokens, const int* block_table, int table_stride, int n_q_heads,
                                           int n_kv_heads, int page_size, int num_pages, float scale,
@@ -543,12 +582,12 @@ extern "C" int qil_attn_tc_prefill_masked(const void* q, const void* kv, void* o
                                       n_kv_heads, page_size, num_pages, scale, slopes_log2, chunk, sink_log2, 0.f,
                                       0, error_word, trace, stream);
 }
+#endif
 
-extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,
-                                          int n_tokens, const int* block_table, int table_stride, int n_q_heads,
-                                          int n_kv_heads, int page_size, int num_pages, float scale,
-                                          const float* slopes_log2, int chunk, const float* sink_log2, float softcap,
-                                          int window, int* error_word, long long* trace, cudaStream_t stream) {
+static int at_launch(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles, int n_tokens, const int* block_table,
+                     int table_stride, int n_q_heads, int n_kv_heads, int page_size, int num_pages, float scale,
+                     const float* slopes_log2, int chunk, const float* sink_log2, float softcap, int window, int* error_word,
+                     long long* trace, AtParams p, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
     if (chunk < 0 || softcap < 0.f || window < 0)
         QIL_REFUSE("attn_tc: chunks of %d positions, a cap of %g, a window of %d", chunk, (double)softcap, window);
@@ -584,7 +623,6 @@ extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* o
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) QIL_REFUSE("attn_tc: cuTensorMapEncodeTiled failed for the cache (%d)", (int)r);
     }
-    AtParams p;
     p.out = (bf16*)out; p.block_table = block_table; p.table_stride = table_stride;
     p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.page_size = page_size;
     p.scale_log2 = scale * 1.4426950408889634f;
@@ -608,6 +646,28 @@ extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* o
     QIL_CHECK_LAUNCH();
 }
 
+#if QIL_KEYS_F16
+// q and the keys of the pages (pages of 64) float16; see AtParams for the rest.
+extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles, int n_tokens,
+                                          const int* block_table, int table_stride, int n_q_heads, int n_kv_heads, int num_pages, float scale,
+                                          int window, const float* q_factor, const float* key_factor, const int* value_marks,
+                                          const unsigned char* marks, int* error_word, cudaStream_t stream) {
+    AtParams p = {};
+    p.q_factor = q_factor; p.key_factor = key_factor; p.value_marks = value_marks; p.marks = marks;
+    if (q_factor == nullptr || key_factor == nullptr || value_marks == nullptr || marks == nullptr) QIL_REFUSE("attn_tc: float16 keys come with their factors and marks");
+    return at_launch(q, kv, out, tile_info, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, AT_N, num_pages, scale,
+                     nullptr, 0, nullptr, 0.f, window, error_word, nullptr, p, stream);
+}
+#else
+extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,
+                                          int n_tokens, const int* block_table, int table_stride, int n_q_heads,
+                                          int n_kv_heads, int page_size, int num_pages, float scale,
+                                          const float* slopes_log2, int chunk, const float* sink_log2, float softcap,
+                                          int window, int* error_word, long long* trace, cudaStream_t stream) {
+    return at_launch(q, kv, out, tile_info, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, page_size, num_pages, scale,
+                     slopes_log2, chunk, sink_log2, softcap, window, error_word, trace, AtParams{}, stream);
+}
+
 extern "C" int qil_attn_tc_prefill_biased(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,
                                           int n_tokens, const int* block_table, int table_stride, int n_q_heads,
                                           int n_kv_heads, int page_size, int num_pages, float scale,
@@ -625,3 +685,4 @@ extern "C" int qil_attn_tc_prefill(const void* q, const void* kv, void* out, con
     return qil_attn_tc_prefill_biased(q, kv, out, tile_info, n_tiles, n_tokens, block_table, table_stride, n_q_heads,
                                       n_kv_heads, page_size, num_pages, scale, nullptr, error_word, trace, stream);
 }
+#endif

@@ -485,22 +485,19 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
             load_pairs(run1 + 128 * G + (c + 4) * 4 * G, pb);
 #pragma unroll
             for (int g = 0; g < G; ++g) steps1[g] = __byte_perm(pa[g], pb[g], 0x5410);
-            unsigned base0 = 0u, base1 = 0u;                       // row g of the side sums: m + 8 s of group r
-            if (r < G) {
-                const unsigned* at0 = reinterpret_cast<const unsigned*>(run0 + 128 * G + 4 * r);
-                const unsigned* at1 = reinterpret_cast<const unsigned*>(run1 + 128 * G + 4 * r);
-                base0 = middles(at0[c * G], at0[(c + 4) * G]);
-                base1 = middles(at1[c * G], at1[(c + 4) * G]);
-            }
+            // row g of the side sums: m + 8 s of group r (rows beyond the groups repeat them and are not looked at)
+            const unsigned* at0 = reinterpret_cast<const unsigned*>(run0 + 128 * G + 4 * (r % G));
+            const unsigned* at1 = reinterpret_cast<const unsigned*>(run1 + 128 * G + 4 * (r % G));
+            const unsigned middle0 = middles(at0[c * G], at0[(c + 4) * G]), middle1 = middles(at1[c * G], at1[(c + 4) * G]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(side[nt], base0, one, base1, one, times_bf16(p0[u][nt], sink), times_bf16(p1[u][nt], sink));
+            for (int nt = 0; nt < NT; ++nt) mma(side[nt], middle0, one, middle1, one, times_bf16(p0[u][nt], sink), times_bf16(p1[u][nt], sink));
             unsigned ps[NT][G][2];                                 // p s of the groups
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const unsigned char* at0 = run0 + g * 128 + (r >> 1) * 4;
-                const unsigned char* at1 = run1 + g * 128 + (r >> 1) * 4;
-                const unsigned x = __byte_perm(*reinterpret_cast<const unsigned*>(at0 + c * 16), *reinterpret_cast<const unsigned*>(at0 + (c + 4) * 16), half);
-                const unsigned y = __byte_perm(*reinterpret_cast<const unsigned*>(at1 + c * 16), *reinterpret_cast<const unsigned*>(at1 + (c + 4) * 16), half);
+                const unsigned char* from0 = run0 + g * 128 + (r >> 1) * 4;
+                const unsigned char* from1 = run1 + g * 128 + (r >> 1) * 4;
+                const unsigned x = __byte_perm(*reinterpret_cast<const unsigned*>(from0 + c * 16), *reinterpret_cast<const unsigned*>(from0 + (c + 4) * 16), half);
+                const unsigned y = __byte_perm(*reinterpret_cast<const unsigned*>(from1 + c * 16), *reinterpret_cast<const unsigned*>(from1 + (c + 4) * 16), half);
                 const unsigned xs = x >> 8, ys = y >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {

@@ -6,7 +6,7 @@ The kernel's mbarrier waits are bounded and report through an error word that ``
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int
+from ctypes import c_float, c_int, c_void_p
 
 import torch
 
@@ -40,6 +40,42 @@ def library(head_dim=MOST_DIM, v_dim=None):
             raise KernelError("attention_tc was built for other head sizes")
         _libs[(head_dim, v_dim)] = lib
     return lib
+
+
+KEYS16_PAGE = 64            # positions per page of float16 keys: a tile's
+_keys16_libs: dict = {}
+
+
+def keys16_library_name(head_dim):
+    """(name, defines) of the library for float16 queries and keys and bfloat16 values of ``head_dim``."""
+    return f"qil_attn_tc_d{head_dim}_keys16", {"QIL_HEAD_DIM": head_dim, "QIL_V_DIM": head_dim, "QIL_KEYS_F16": 1}
+
+
+def keys16_library(head_dim):
+    lib = _keys16_libs.get(head_dim)
+    if lib is None:
+        name, defines = keys16_library_name(head_dim)
+        lib = build.load(name, ["attention_tc.cu"], defines)
+        ops.register_post_step_check(check)
+        if lib.qil_attn_tc_head_dim() != head_dim or lib.qil_attn_tc_keys_per_tile() != KEYS16_PAGE:
+            raise KernelError("attention_tc was built for other head sizes")
+        _keys16_libs[head_dim] = lib
+    return lib
+
+
+def prefill_keys16(q16, q_factor, rows, key_factor, value_marks, marks, out, tile_info, n_tiles, table, n_pages, n_q_heads, n_kv_heads, head_dim,
+                   scale, window):
+    """``prefill`` over ``rows``, pages [n_pages, 2, Hkv, 64, head_dim] of float16 keys and bfloat16 values, and float16 queries [N, Hq * head_dim]:
+    ``q_factor`` float32 [N, Hq] and ``key_factor`` float32 [n_pages, Hkv] multiply them back; ``value_marks`` int32 [n_pages, Hkv] and ``marks``
+    uint8 [n_pages, Hkv, 64] say where a position's value groups of 32 are NaN (they hold zeros then).  The first six are addresses:
+    ``kernels.kv4`` lays them out in one buffer and is what calls this."""
+    lib = keys16_library(head_dim)
+    word = _fault.tensor(out.device)
+    _fault.mark()
+    _check(lib, lib.qil_attn_tc_prefill_keys16(
+        c_void_p(q16), c_void_p(rows), _p(out), _p(tile_info), c_int(n_tiles), c_int(out.shape[0]), _p(table), c_int(table.shape[1]), c_int(n_q_heads),
+        c_int(n_kv_heads), c_int(n_pages), c_float(scale), c_int(window), c_void_p(q_factor), c_void_p(key_factor), c_void_p(value_marks),
+        c_void_p(marks), _p(word), _stream()), "attention (128-token tiles, float16 keys)")
 
 
 def supports(head_dim, page_size, window, v_dim=None) -> bool:

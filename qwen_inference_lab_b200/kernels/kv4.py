@@ -43,6 +43,7 @@ _few_libs: dict = {}
 _P, _I, _F = c_void_p, c_int, c_float
 _STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 9 * [_I] + [_P]
 _READ = [_P, _P, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
+_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P] + 7 * [_I] + [_P]
 _SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
 _FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]
 
@@ -70,6 +71,7 @@ def library():
     if _lib is None:
         lib = build.load("qil_kv4", SOURCES, depends=DEPENDS)
         lib.qil_kv4_store.argtypes, lib.qil_kv4_read.argtypes, lib.qil_kv4_singles.argtypes = _STORE, _READ, _SINGLES
+        lib.qil_kv4_spread.argtypes = _SPREAD
         _lib = lib
     return _lib
 
@@ -230,8 +232,9 @@ def describe_segments(first, starts, lens, rows) -> dict:
                         position, tokens, block-table row, tokens of the segments before in this array, the longest context among these, 0, 0)
     ``single_tokens``, ``few_tokens``, ``portion_tokens``  the same token by token, four ints each, (token, its position, block-table row, the
                         longest context among these)
-    ``b0.read`` ...     the portions in batches whose contexts are read back together: ``kv4.read``'s info, the block table of the
-                        pages they are read to, and their query tiles over that table (``attention_mma.describe_segments``)
+    ``b0.read`` ...     the portions in batches whose contexts are read back together: ``kv4.read``'s info; the same with the segment's first
+                        position (``spread``); the block table of the pages they are read to; query tiles of 64 and of 128 tokens over that
+                        table, (first token, its position, tokens, row of it) each
     """
     lens, starts = np.asarray(lens, dtype=np.int64), np.asarray(starts, dtype=np.int64)
     first, rows = np.asarray(first, dtype=np.int64), np.asarray(rows, dtype=np.int64)
@@ -264,11 +267,13 @@ def describe_segments(first, starts, lens, rows) -> dict:
         taken = order[:max(1, MOST_READ // (width * READ_PAGE))]
         order = order[len(taken):]
         local = np.arange(len(taken), dtype=np.int64)
-        tiles = attention_mma.describe_segments(first[taken], starts[taken], lens[taken], local)
         arrays[f"b{batch}.read"] = np.stack([rows[taken], np.zeros_like(local), ends[taken], local * width], axis=1).reshape(-1)
+        arrays[f"b{batch}.spread"] = np.stack([rows[taken], starts[taken], ends[taken], local * width], axis=1).reshape(-1)
         arrays[f"b{batch}.table"] = np.arange(len(taken) * width, dtype=np.int64)
-        for name in ("tile_info", "big_tile_info", "rest_tile_info"):
-            arrays[f"b{batch}.{name}"] = tiles[name]
+        for name, tile in (("tiles", attention_mma.QUERY_TILE), ("big_tiles", attention_tc.TILE)):
+            found = [(first[i] + off, starts[i] + off, min(tile, lens[i] - off), j) for j, i in enumerate(taken) for off in range(0, int(lens[i]), tile)]
+            found.sort(key=lambda t: -(t[1] + t[2]))                # the longest contexts first: the short ones fill the gaps
+            arrays[f"b{batch}.{name}"] = np.array(found, dtype=np.int64).reshape(-1)
         batch += 1
     return arrays
 
@@ -384,28 +389,38 @@ def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, h
 
 
 def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
-    """A batch of portions: their contexts' rows as ordinary pages, then the attention over those."""
-    array = {name: plan.array[f"b{batch}.{name}"] for name in ("read", "table", "tile_info", "big_tile_info", "rest_tile_info")}
-    count = {name: plan.count[f"b{batch}.{name}"] for name in array}
-    segments = count["read"] // 4
-    width = count["table"] // segments
-    shape = (count["table"], 2, n_kv_heads, READ_PAGE, head_dim)
-    held = extras.get(("kv4_rows", q.dtype))
-    size = count["table"] * 2 * n_kv_heads * READ_PAGE * head_dim
-    if held is None or held.numel() < size:
-        held = extras[("kv4_rows", q.dtype)] = torch.empty(size, dtype=q.dtype, device=q.device)
-    rows = held[:size].view(shape)
-    read(pages, block_table, array["read"], segments, width * READ_PAGE, rows, n_kv_heads, head_dim, page_size)
-    table = array["table"][:count["table"]].view(segments, width)
-    if q.dtype == torch.bfloat16:
-        array["decode_info"], count["decode_info"] = None, 0
-        ctx = SimpleNamespace(plans={attention_mma.PLAN_KEY: SimpleNamespace(array=array, count=count)}, max_context=plan.max_context, min_context=0,
-                              extras=extras, device=q.device)
-        view = SimpleNamespace(pages=rows, block_table=table, page_size=READ_PAGE, window=window)
-        attention_mma.attend(ctx, q, view, out, n_q_heads, n_kv_heads, head_dim, window, scale)
-    else:
-        attention_f32.tiles(q, rows, out, array["tile_info"], count["tile_info"] // 4, table, n_q_heads, n_kv_heads, head_dim, READ_PAGE,
+    """A batch of portions: their contexts' rows as pages of 64 positions, then the attention over those."""
+    array, count = plan.array, plan.count
+    segments, n_pages = count[f"b{batch}.read"] // 4, count[f"b{batch}.table"]
+    table = array[f"b{batch}.table"][:n_pages].view(segments, n_pages // segments)
+    size = n_pages * 2 * n_kv_heads * READ_PAGE * head_dim
+    if q.dtype == torch.float32:
+        held = extras.get("kv4_rows")
+        if held is None or held.numel() < size:
+            held = extras["kv4_rows"] = torch.empty(size, dtype=torch.float32, device=q.device)
+        rows = held[:size].view(n_pages, 2, n_kv_heads, READ_PAGE, head_dim)
+        read(pages, block_table, array[f"b{batch}.read"], segments, n_pages // segments * READ_PAGE, rows, n_kv_heads, head_dim, page_size)
+        attention_f32.tiles(q, rows, out, array[f"b{batch}.tiles"], count[f"b{batch}.tiles"] // 4, table, n_q_heads, n_kv_heads, head_dim, READ_PAGE,
                             window, scale)
+        return
+    # rows, queries, and what goes with them, in one buffer: every part from a 16-byte boundary on
+    tokens, heads = q.shape[0], n_pages * n_kv_heads
+    parts = (2 * size, 2 * q.numel(), 4 * tokens * n_q_heads, 4 * heads, 4 * heads, heads * READ_PAGE)
+    at, total = [], 0
+    for nbytes in parts:
+        at.append(total)
+        total += -(-nbytes // 128) * 128
+    held = extras.get("kv4_spread")
+    if held is None or held.numel() < total:
+        held = extras["kv4_spread"] = torch.empty(total, dtype=torch.uint8, device=q.device)
+    base = held.data_ptr()
+    rows, q16, q_factor, key_factor, value_marks, marks = (base + offset for offset in at)
+    lib = library()
+    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], array[f"b{batch}.spread"].data_ptr(), segments,
+                                   n_pages // segments, rows, key_factor, value_marks, marks, q.data_ptr(), q16, q_factor, tokens, n_q_heads, n_kv_heads,
+                                   head_dim, page_size, pages.shape[0], window, _stream()), "kv4.attend (rows of portions)")
+    attention_tc.prefill_keys16(q16, q_factor, rows, key_factor, value_marks, marks, out, array[f"b{batch}.big_tiles"],
+                                count[f"b{batch}.big_tiles"] // 4, table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window)
 
 
 def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, *, window=0, extras):

@@ -282,11 +282,11 @@ def test_attend_spans_agree_with_one():
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
 def test_attend_nan_goes_to_those_who_see_it(dtype):
-    built = attend_case(4, 2, 64, 8, [40, 40, 40], [1, 1, 4], dtype)
+    built = attend_case(4, 2, 64, 8, [40, 40, 40, 0], [1, 1, 4, 30], dtype)
     key = built["table"]
     plane_bytes = built["pages"]
-    # request 0: the key at position 3 of head 0 is NaN; request 1: the value at position 3 of head 1
-    for row, plane, head, pos in ((0, 0, 0, 3), (1, 1, 1, 3)):
+    # request 0: the key at position 3 of head 0 is NaN; request 1: the value at position 3 of head 1; request 3: the value at position 20
+    for row, plane, head, pos in ((0, 0, 0, 3), (1, 1, 1, 3), (3, 1, 0, 20)):
         codes, pairs = plain.get(plane_bytes, int(key[row, pos // 8]), plane, head, pos % 8)
         pairs[0] = math.nan
         plain.put(plane_bytes, int(key[row, pos // 8]), plane, head, pos % 8, codes, pairs)
@@ -294,6 +294,9 @@ def test_attend_nan_goes_to_those_who_see_it(dtype):
     assert out[0, :2].isnan().all() and out[0, 2:].isfinite().all()
     assert out[1, 2:, :32].isnan().all() and out[1, 2:, 32:].isfinite().all() and out[1, :2].isfinite().all()
     assert out[2:6].isfinite().all()
+    portion = out[6:]
+    assert portion[20:, :2, :32].isnan().all() and portion[20:, :2, 32:].isfinite().all() and portion[:, 2:].isfinite().all()
+    assert portion[:20].isfinite().all()
     # a window that has passed position 3 does not see it
     assert attend_run(built, window=20).float().cpu().view(-1, 4, 64)[:6].isfinite().all()
 
