@@ -19,17 +19,21 @@
 //               and the rescale of O in tensor memory when the running maximum moved by more than
 //               2^8 (until then P is computed against the older maximum, which is exact algebra and
 //               safe in float32), in tiles of fewer tokens whenever it moved; finally O / l -> global memory.
-// With -DQIL_KEYS_F16=1 queries and keys are float16, each query row and each page of keys with a power of two of its own taken out, which
-// the softmax multiplies back (pages of 64: a tile's scores have one factor); values, P and the output are bfloat16 as ever.  Rows that were
+// With -DQIL_KEYS_F16=1 keys are float16, each page of them with a power of two taken out, which the softmax multiplies back (pages of 64:
+// a tile's scores have one factor); the softmax warps make float16 of the queries' rows where they lie, each with a power of two of its own;
+// values, P and the output are bfloat16 as ever.  Rows that were
 // held in fewer bits and are read back for this kernel have more than bfloat16's 8: as bfloat16 keys they are off by 2^-9, which
 // scores of some size turn into a weight's error several times that of its own rounding.  Value groups that are NaN come as zeros and
-// marks: a row that sees a mark gets NaN there, one that masks it does not.
+// marks: a row that sees a mark gets NaN there, one that masks it does not.  In this form a block's 128 rows are `pack` query heads of one kv
+// head times 128 / pack tokens (a short portion fills a tile, and a tile of fewer tokens masks less), and where the blocks would not fill
+// the GPU a context is cut over several blocks (`splits`), whose unnormed outputs a second kernel joins.
 // K tiles are K-major operands and V tiles MN-major operands of the same shared-memory image
 // ([key][64 elements = 128 bytes] x the slabs of the head).
 //
 // Every mbarrier wait is bounded (about a second), records its place in the error word when it runs
 // out and makes its role stop; the block then frees its tensor memory and returns.
 #include "tcgen05.cuh"
+#include <cuda_fp16.h>
 
 QIL_ERROR_STORAGE
 
@@ -125,6 +129,9 @@ __device__ __forceinline__ float at_exp2(float x) {
 
 struct AtShared {
     unsigned long long q_full;
+#if QIL_KEYS_F16
+    unsigned long long q_ready;         // the rows are float16
+#endif
     unsigned long long k_full[AT_STAGES], k_empty[AT_STAGES];
     unsigned long long v_full[AT_STAGES], v_empty[AT_STAGES];
     unsigned long long s_full[2];
@@ -156,12 +163,31 @@ struct AtParams {
     int* error_word;
     long long* trace;           // only read when compiled with AT_TRACE
 #if QIL_KEYS_F16
-    const float* q_factor;              // [N, Hq]: what a row of the float16 queries is multiplied by
     const float* key_factor;            // [page][kv head]: what a page's float16 keys are
     const int* value_marks;             // [page][kv head]: does any value group of the page have a mark?
     const unsigned char* marks;         // [page][kv head][64]: bit g: group g of 32 columns of that position's value is NaN
+    const int4* segments;               // (first token, its position, tokens, block-table row) each, the longest contexts first
+    int n_segments, pack;
+    float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum)
+    float2* part_ml;
 #endif
 };
+
+#if QIL_KEYS_F16
+// The tile that block `index` of the tiles of all segments takes: those of a segment's last tokens first.
+__device__ __forceinline__ int4 at_tile(const int4* __restrict__ segments, int n_segments, int index, int tokens) {
+    for (int i = 0; i < n_segments; ++i) {
+        const int4 s = segments[i];
+        const int tiles = (s.z + tokens - 1) / tokens;
+        if (index < tiles) {
+            const int off = (tiles - 1 - index) * tokens;
+            return make_int4(s.x + off, s.y + off, min(tokens, s.z - off), s.w);
+        }
+        index -= tiles;
+    }
+    return make_int4(0, 0, 0, 0);       // never: the grid is as large as the tiles are many
+}
+#endif
 
 #define AT_VALUE_WARP 6                  // warps: 0 keys, 1 MMA issue, 2-5 softmax, 6 values
 #define AT_THREADS 224
@@ -182,24 +208,44 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     AtShared* sh = reinterpret_cast<AtShared*>(sV + AT_STAGES * AT_VTILE);
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     // heads vary fastest, so all heads of the longest tile start first (tiles come sorted, longest first)
+#if QIL_KEYS_F16
+    const int pack = p.pack, head = blockIdx.x * pack;
+#else
+    constexpr int pack = 1;
     const int head = blockIdx.x;
+#endif
     const int kv_head = head / (p.n_q_heads / p.n_kv_heads);
     // tile_info: (first token in the flat batch, its absolute position, tokens, block-table row).  Rows past the tile's
     // tokens hold other tokens' queries or zeros; they see what its last token sees and are not stored.
+#if QIL_KEYS_F16
+    const int4 info = at_tile(p.segments, p.n_segments, blockIdx.y, AT_M / pack);
+    if (info.z <= 0) return;
+#else
     const int4 info = tile_info[blockIdx.y];
-    const int n0 = info.x, pos0 = info.y, rows = min(info.z, AT_M);
-    const int hi = pos0 + rows - 1;                          // last key any row of the tile may see
+#endif
+    const int n0 = info.x, pos0 = info.y, rows = min(info.z * pack, AT_M);
+    const int hi = pos0 + (rows - 1) / pack;                 // last key any row of the tile may see
     // the first key that the query at a position sees
     auto first_key_of = [&p](int position) {
         const int of_chunk = p.chunk > 0 ? position / p.chunk * p.chunk : 0;
         return p.window > 0 ? max(of_chunk, position - p.window + 1) : of_chunk;
     };
+#if QIL_KEYS_F16
+    const int whole0 = first_key_of(pos0) / AT_N, whole = hi / AT_N + 1 - whole0;
+    const int each = (whole + (int)gridDim.z - 1) / (int)gridDim.z;
+    const int tile0 = whole0 + (int)blockIdx.z * each, n_tiles = min(each, whole - (int)blockIdx.z * each);
+    if (n_tiles <= 0) return;                                // fewer tiles than splits: the join knows
+#else
     const int tile0 = first_key_of(pos0) / AT_N;             // the key tile that holds the first key any row sees
     const int n_tiles = hi / AT_N + 1 - tile0;
+#endif
     const int* table = p.block_table + (size_t)info.w * p.table_stride;
 
     if (threadIdx.x == 0) {
         mbar_init(&sh->q_full, 1);
+#if QIL_KEYS_F16
+        mbar_init(&sh->q_ready, 4);
+#endif
         for (int s = 0; s < AT_STAGES; ++s) {
             mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 1);
             mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 1);
@@ -219,6 +265,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = uniform(sh->tmem_base);
+#if QIL_KEYS_F16
+    qil_wait_for_producer();            // tiles and block table are older than the kernel that makes the rows
+#endif
     auto tmem_s = [tmem](int buffer) { return tmem + (unsigned)(buffer * AT_N); };    // the two score buffers
     const unsigned tmem_o = tmem + 2u * AT_N;
 
@@ -292,7 +341,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const bool leader = elect_one();
         const unsigned idesc_s = umma_idesc(AT_M, AT_N) & (QIL_KEYS_F16 ? ~((1u << 7) | (1u << 10)) : ~0u);      // float16 operands: zeros there
         const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AT_ES * 64 >> 3) << 17) | ((unsigned)(AT_M >> 4) << 24);
+#if QIL_KEYS_F16
+        bool ok = warp_mbar_wait(&sh->q_ready, 0);
+#else
         bool ok = warp_mbar_wait(&sh->q_full, 0);
+#endif
         if (!ok && leader) atomicExch(p.error_word, 13);
         auto issue_scores = [&](int j) -> bool {
             const int stage = j % AT_STAGES, buf = j & 1;
@@ -338,7 +391,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     } else if (warp < AT_VALUE_WARP) {
         const int quarter = warp & 3;
         const int row = quarter * 32 + lane;                 // query row of this thread = its TMEM lane
-        const int pos = min(pos0 + row, hi);
+        const int pos = min(pos0 + row / pack, hi);
         const int lo = first_key_of(pos);                     // the first key this row sees
         const unsigned lane_base = (unsigned)(quarter * 32) << 16;
         // With a distance bias the scores are scaled and biased first and the steps below take them as they are.
@@ -346,7 +399,40 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const bool biased = p.slopes_log2 != nullptr;
         const float slope = biased ? p.slopes_log2[head] : 0.f;
 #if QIL_KEYS_F16
-        const float row_scale = p.scale_log2 * p.q_factor[(size_t)(n0 + min(row, rows - 1)) * p.n_q_heads + head];
+        // this thread's row, 16 bytes at a time, neighbouring rows at different places of their 128 bytes (which element lies where
+        // does not matter): its largest into [256, 512)
+        if (!warp_mbar_wait(&sh->q_full, 0)) { if (lane == 0) atomicExch(p.error_word, 25); }
+        float row_scale = p.scale_log2;
+        {
+            unsigned char* q_row = sQ + row * 128;
+            float largest = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8 * AT_DS; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(q_row + i / 8 * AT_QSLAB + ((i + row) & 7) * 16);
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+            }
+            const int e = __float_as_int(largest) >> 23, by = e == 255 ? 0 : min(135 - e, 126);
+            const float up = __int_as_float((127 + by) << 23);
+            row_scale *= __int_as_float((127 - by) << 23);
+#pragma unroll
+            for (int i = 0; i < 8 * AT_DS; ++i) {
+                uint4* at = reinterpret_cast<uint4*>(q_row + i / 8 * AT_QSLAB + ((i + row) & 7) * 16);
+                const uint4 v = *at;
+                unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __half2 h = __floats2half2_rn(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
+                    w[k] = *reinterpret_cast<const unsigned*>(&h);
+                }
+                *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->q_ready);
+        }
         float my_factor = 1.f;                                // of tile j / 32 * 32 + lane
         int my_page = 0;
         unsigned marked = 0u;                                 // groups of which this row sees a mark
@@ -509,13 +595,27 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             tc_fence_after();
             if (p.sink_log2 != nullptr) l += (m_used == -INFINITY) ? 1.f : exp2f(p.sink_log2[head] - m_used);
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            bf16* dst = p.out + ((size_t)(n0 + row) * p.n_q_heads + head) * AT_E;
+            bf16* dst = p.out + ((size_t)(n0 + row / pack) * p.n_q_heads + head + row % pack) * AT_E;
+#if QIL_KEYS_F16
+            const size_t part = ((((size_t)blockIdx.y * gridDim.x + blockIdx.x) * gridDim.z + blockIdx.z) * AT_M + row);
+            if (gridDim.z > 1) p.part_ml[part] = make_float2(m_used, l);
+#endif
 #pragma unroll 1
             for (int c = 0; c < (AT_E + 31) / 32; ++c) {
                 unsigned r[32];
                 __syncwarp();
                 at_tmem_ld32(tmem_o + lane_base + c * 32, r);
                 at_wait_ld();
+#if QIL_KEYS_F16
+                if (gridDim.z > 1) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(p.part_o + part * AT_E + c * 32 + i) = (marked >> c & 1u)
+                            ? make_float4(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000), __int_as_float(0x7fc00000), __int_as_float(0x7fc00000))
+                            : make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+                    continue;
+                }
+#endif
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (AT_E % 32 != 0 && c * 32 + q * 8 >= AT_E) break;
@@ -538,6 +638,37 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"((unsigned)AT_TMEM_COLS) : "memory");
     }
 }
+
+#if QIL_KEYS_F16
+// out = sum over splits of O 2^(m - M) over the sum of l 2^(m - M), M their largest maximum.  A warp a row.
+__global__ void __launch_bounds__(256) at_join_kernel(AtParams p, int splits) {
+    const int row = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    qil_wait_for_producer();
+    const int4 info = at_tile(p.segments, p.n_segments, blockIdx.y, AT_M / p.pack);
+    if (row >= info.z * p.pack) return;
+    // the splits that hold anything, as the blocks counted them
+    const int hi = info.y + info.z - 1;
+    const int whole = hi / AT_N + 1 - (p.window > 0 ? max(0, info.y - p.window + 1) : 0) / AT_N;
+    const int each = (whole + splits - 1) / splits, used = (whole + each - 1) / each;
+    const size_t part = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits) * AT_M + row;
+    float most = -INFINITY, l = 0.f, o[AT_E / 32];
+    for (int z = 0; z < used; ++z) most = fmaxf(most, p.part_ml[part + (size_t)z * AT_M].x);
+    const float against = most == -INFINITY ? 0.f : most;
+#pragma unroll
+    for (int i = 0; i < AT_E / 32; ++i) o[i] = 0.f;
+    for (int z = 0; z < used; ++z) {
+        const float2 ml = p.part_ml[part + (size_t)z * AT_M];
+        const float keep = exp2f(ml.x - against);
+        l = fmaf(ml.y, keep, l);
+#pragma unroll
+        for (int i = 0; i < AT_E / 32; ++i) o[i] = fmaf(p.part_o[(part + (size_t)z * AT_M) * AT_E + i * 32 + lane], keep, o[i]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bf16* dst = p.out + ((size_t)(info.x + row / p.pack) * p.n_q_heads + blockIdx.x * p.pack + row % p.pack) * AT_E;
+#pragma unroll
+    for (int i = 0; i < AT_E / 32; ++i) dst[i * 32 + lane] = __float2bfloat16_rn(o[i] * inv);
+}
+#endif
 
 // ------------------------------------------------------------------ host side
 typedef CUresult (*AtEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -587,7 +718,7 @@ extern "C" int qil_attn_tc_prefill_masked(const void* q, const void* kv, void* o
 static int at_launch(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles, int n_tokens, const int* block_table,
                      int table_stride, int n_q_heads, int n_kv_heads, int page_size, int num_pages, float scale,
                      const float* slopes_log2, int chunk, const float* sink_log2, float softcap, int window, int* error_word,
-                     long long* trace, AtParams p, cudaStream_t stream) {
+                     long long* trace, AtParams p, int splits, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
     if (chunk < 0 || softcap < 0.f || window < 0)
         QIL_REFUSE("attn_tc: chunks of %d positions, a cap of %g, a window of %d", chunk, (double)softcap, window);
@@ -603,7 +734,11 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
     {
         const cuuint64_t dims[3] = {AT_D, (cuuint64_t)n_q_heads, (cuuint64_t)n_tokens};
         const cuuint64_t strides[2] = {AT_D * 2, (cuuint64_t)n_q_heads * AT_D * 2};
+#if QIL_KEYS_F16
+        const cuuint32_t box[3] = {64, (cuuint32_t)p.pack, (cuuint32_t)(AT_M / p.pack)};
+#else
         const cuuint32_t box[3] = {64, 1, AT_M};
+#endif
         const cuuint32_t elem[3] = {1, 1, 1};
         const CUresult r = encode(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem,
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -642,21 +777,32 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
         if (e != cudaSuccess) QIL_REFUSE("attn_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
         configured = true;
     }
+#if QIL_KEYS_F16
+    qil_launch_chained(attn_tc_kernel, dim3(n_q_heads / p.pack, n_tiles, splits), dim3(AT_THREADS), smem, stream, map_q, map_k, map_v, p, (const int4*)nullptr);
+    if (splits > 1) qil_launch_chained(at_join_kernel, dim3(n_q_heads / p.pack, n_tiles, AT_M / 8), dim3(256), 0, stream, p, splits);
+#else
     attn_tc_kernel<<<dim3(n_q_heads, n_tiles), AT_THREADS, smem, stream>>>(map_q, map_k, map_v, p, (const int4*)tile_info);
+#endif
     QIL_CHECK_LAUNCH();
 }
 
 #if QIL_KEYS_F16
-// q and the keys of the pages (pages of 64) float16; see AtParams for the rest.
-extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles, int n_tokens,
+// The keys of the pages (pages of 64) float16; see AtParams for the rest.  segments int32 [n_segments, 4]; n_tiles: of all segments,
+// 128 / pack tokens each; splits > 1: part_o float32 [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml as many pairs of rows.
+extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* segments, int n_segments, int n_tiles, int n_tokens,
                                           const int* block_table, int table_stride, int n_q_heads, int n_kv_heads, int num_pages, float scale,
-                                          int window, const float* q_factor, const float* key_factor, const int* value_marks,
-                                          const unsigned char* marks, int* error_word, cudaStream_t stream) {
+                                          int window, int pack, int splits, const float* key_factor, const int* value_marks,
+                                          const unsigned char* marks, float* part_o, float* part_ml, int* error_word, cudaStream_t stream) {
+    if (key_factor == nullptr || value_marks == nullptr || marks == nullptr) QIL_REFUSE("attn_tc: float16 keys come with factors and marks");
+    if (n_kv_heads <= 0 || pack <= 0 || AT_M % pack || (n_q_heads / n_kv_heads) % pack || splits < 1 || splits > 65535
+        || (splits > 1 && (part_o == nullptr || part_ml == nullptr)))
+        QIL_REFUSE("attn_tc: %d heads of %d over %d a tile, %d splits", pack, n_q_heads, n_kv_heads, splits);
     AtParams p = {};
-    p.q_factor = q_factor; p.key_factor = key_factor; p.value_marks = value_marks; p.marks = marks;
-    if (q_factor == nullptr || key_factor == nullptr || value_marks == nullptr || marks == nullptr) QIL_REFUSE("attn_tc: float16 keys come with their factors and marks");
-    return at_launch(q, kv, out, tile_info, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, AT_N, num_pages, scale,
-                     nullptr, 0, nullptr, 0.f, window, error_word, nullptr, p, stream);
+    p.key_factor = key_factor; p.value_marks = value_marks; p.marks = marks;
+    p.segments = (const int4*)segments; p.n_segments = n_segments; p.pack = pack;
+    p.part_o = part_o; p.part_ml = (float2*)part_ml;
+    return at_launch(q, kv, out, segments, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, AT_N, num_pages, scale,
+                     nullptr, 0, nullptr, 0.f, window, error_word, nullptr, p, splits, stream);
 }
 #else
 extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,
@@ -665,7 +811,7 @@ extern "C" int qil_attn_tc_prefill_capped(const void* q, const void* kv, void* o
                                           const float* slopes_log2, int chunk, const float* sink_log2, float softcap,
                                           int window, int* error_word, long long* trace, cudaStream_t stream) {
     return at_launch(q, kv, out, tile_info, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, page_size, num_pages, scale,
-                     slopes_log2, chunk, sink_log2, softcap, window, error_word, trace, AtParams{}, stream);
+                     slopes_log2, chunk, sink_log2, softcap, window, error_word, trace, AtParams{}, 1, stream);
 }
 
 extern "C" int qil_attn_tc_prefill_biased(const void* q, const void* kv, void* out, const int* tile_info, int n_tiles,

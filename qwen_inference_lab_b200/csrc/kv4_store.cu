@@ -14,9 +14,9 @@
 // neighbouring elements, so that a head of 128 is half a warp and a group's codes are one word of each of four lanes, and a token's
 // cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
 //
-// kv4_spread: the rows of a prompt portion's context and its queries for the kernel that attends to 16-bit operands (attention_tc.cu with
-// float16 keys): keys as float16 with a power of two taken out per page of 64 and head, values as bfloat16, queries as float16 with a
-// power of two per row; where a group of values is NaN, zeros and a mark.
+// kv4_spread: the rows of a prompt portion's context for the kernel that attends to 16-bit operands (attention_tc.cu with float16 keys):
+// keys as float16 with a power of two taken out per page of 64 and head, values as bfloat16; where a group of values is NaN, zeros and
+// a mark.
 //
 // kv4_read: rows of requests as ordinary pages [page][2][kv head][slot][d] of float32 or bfloat16.
 #include "kv4.h"
@@ -498,28 +498,25 @@ struct Kv4Spread {
     float* key_factor;              // [page][kv head]
     int* value_marks;               // [page][kv head]
     unsigned char* marks;           // [page][kv head][64]
-    const bf16* q;                  // [tokens, q_heads * dim]
-    __half* q16;
-    float* q_factor;                // [tokens, q_heads]
-    int table_width, segments, tokens, q_heads, kv_heads, dim, page_size, num_pages, window;
+    int table_width, kv_heads, dim, page_size, num_pages, window;
 };
-// Two factors whose product is the power of two that brings `largest` into [256, 512), and what undoes them.
-__device__ __forceinline__ float bring_up(float largest, float& up1, float& up2) {
-    const int up = largest > 0.f && largest < INFINITY ? 8 - ilogbf(largest) : 0;
-    up1 = __uint_as_float((unsigned)(127 + up / 2) << 23);
-    up2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
-    return scalbnf(1.f, -up);
+// The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.
+__device__ __forceinline__ float bring_up(float largest, float& up) {
+    const int e = __float_as_int(largest) >> 23;            // 0 of zero and of the smallest numbers, 255 of infinities
+    const int by = e == 255 ? 0 : min(135 - e, 126);
+    up = __int_as_float((127 + by) << 23);
+    return __int_as_float((127 - by) << 23);
 }
 __device__ __forceinline__ unsigned two_halves(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&v);
 }
-__device__ __forceinline__ void store8_half(__half* p, const float (&v)[8], float up1, float up2) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(two_halves(v[0] * up1 * up2, v[1] * up1 * up2), two_halves(v[2] * up1 * up2, v[3] * up1 * up2),
-                                              two_halves(v[4] * up1 * up2, v[5] * up1 * up2), two_halves(v[6] * up1 * up2, v[7] * up1 * up2));
+__device__ __forceinline__ void store8_half(__half* p, const float (&v)[8], float up) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(two_halves(v[0] * up, v[1] * up), two_halves(v[2] * up, v[3] * up),
+                                              two_halves(v[4] * up, v[5] * up), two_halves(v[6] * up, v[7] * up));
 }
 
-// A block: a page of 64 positions of a head's keys or values, a run of 8 a warp (as in kv4_read); the last layer of blocks: the queries.
+// A block: a page of 64 positions of a head's keys or values, a run of 8 a warp (as in kv4_read).
 template <int GROUPS>
 __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Spread a) {
     __shared__ float largest_of[READ_WARPS];
@@ -527,35 +524,6 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     qil_release_consumer();
     constexpr int dim = GROUPS * KV4_GROUP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if ((int)blockIdx.z == a.segments) {
-        // a row is dim / 8 lanes of 8 elements: 4, 8, 12 or 16, several rows a warp
-        constexpr int LANES = dim / 8, ROWS = 32 / LANES;
-        const int sub = lane / LANES, l = lane % LANES;
-        const long long rows = (long long)a.tokens * a.q_heads, blocks = (long long)gridDim.x * gridDim.y;
-        const long long first = (blockIdx.y * (long long)gridDim.x + blockIdx.x) * READ_WARPS + warp;
-        for (long long base = first * ROWS; base < rows; base += blocks * READ_WARPS * ROWS) {
-            const long long row = base + sub;
-            const bool mine = sub < ROWS && row < rows;
-            EightBf16 own;
-            own.zero();
-            if (mine) own.load(a.q + row * dim + 8 * l);
-            float x[8], largest = 0.f;
-            own.floats(x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
-            const float own_largest = largest;
-#pragma unroll
-            for (int i = 0; i < LANES; ++i)                 // 12 lanes of a row of 96 are no power of two
-                largest = fmaxf(largest, __shfl_sync(0xffffffffu, own_largest, (min(sub, ROWS - 1) * LANES + i) & 31));
-            float up1, up2;
-            const float factor = bring_up(largest, up1, up2);
-            if (mine) {
-                store8_half(a.q16 + row * dim + 8 * l, x, up1, up2);
-                if (l == 0) a.q_factor[row] = factor;
-            }
-        }
-        return;
-    }
     const int4 mine = reinterpret_cast<const int4*>(a.info)[blockIdx.z];
     const int plane = blockIdx.y / a.kv_heads, head = blockIdx.y % a.kv_heads;
     const int page0 = blockIdx.x * SPREAD_PAGE;
@@ -589,14 +557,14 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
         largest = largest_of[0];
 #pragma unroll
         for (int w = 1; w < READ_WARPS; ++w) largest = fmaxf(largest, largest_of[w]);
-        float up1, up2;
-        const float factor = bring_up(largest, up1, up2);
+        float up;
+        const float factor = bring_up(largest, up);
         if (threadIdx.x == 0) a.key_factor[at] = factor;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
             float v[8];
             eight_values(codes[g], pairs[g], v);
-            store8_half(dst + g * KV4_GROUP, v, up1, up2);
+            store8_half(dst + g * KV4_GROUP, v, up);
         }
         return;
     }
@@ -618,16 +586,15 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
 }
 
 extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int table_width, const void* info, int segments, int width, void* rows,
-                              void* key_factor, void* value_marks, void* marks, const void* q, void* q16, void* q_factor, int tokens, int q_heads,
-                              int kv_heads, int dim, int page_size, int num_pages, int window, cudaStream_t stream) {
+                              void* key_factor, void* value_marks, void* marks, int kv_heads, int dim, int page_size, int num_pages, int window,
+                              cudaStream_t stream) {
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments >= 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
     const Kv4Spread a = {(const uint8_t*)pages, (const int*)block_table, (const int*)info, (__half*)rows, (float*)key_factor, (int*)value_marks,
-                         (unsigned char*)marks, (const bf16*)q, (__half*)q16, (float*)q_factor, table_width, segments, tokens, q_heads, kv_heads, dim,
-                         page_size, num_pages, window};
-    const dim3 grid(width, 2 * kv_heads, segments + (q != nullptr ? 1 : 0));
+                         (unsigned char*)marks, table_width, kv_heads, dim, page_size, num_pages, window};
+    const dim3 grid(width, 2 * kv_heads, segments);
     void (*kernel)(Kv4Spread) = dim == 32 ? kv4_spread_kernel<1> : dim == 64 ? kv4_spread_kernel<2> : dim == 96 ? kv4_spread_kernel<3> : kv4_spread_kernel<4>;
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);
     QIL_CHECK_LAUNCH();

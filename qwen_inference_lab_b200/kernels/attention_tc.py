@@ -63,19 +63,33 @@ def keys16_library(head_dim):
     return lib
 
 
-def prefill_keys16(q16, q_factor, rows, key_factor, value_marks, marks, out, tile_info, n_tiles, table, n_pages, n_q_heads, n_kv_heads, head_dim,
-                   scale, window):
-    """``prefill`` over ``rows``, pages [n_pages, 2, Hkv, 64, head_dim] of float16 keys and bfloat16 values, and float16 queries [N, Hq * head_dim]:
-    ``q_factor`` float32 [N, Hq] and ``key_factor`` float32 [n_pages, Hkv] multiply them back; ``value_marks`` int32 [n_pages, Hkv] and ``marks``
-    uint8 [n_pages, Hkv, 64] say where a position's value groups of 32 are NaN (they hold zeros then).  The first six are addresses:
-    ``kernels.kv4`` lays them out in one buffer and is what calls this."""
+def keys16_pack(n_q_heads, n_kv_heads) -> int:
+    """Query heads of one kv head that share a tile: the largest power of two that divides their number, 128 at most."""
+    share = n_q_heads // n_kv_heads
+    return min(share & -share, TILE)
+
+
+def keys16_splits(blocks, tiles) -> int:
+    """Blocks that a context of ``tiles`` tiles of 64 keys is cut over: as fill the GPU's two blocks an SM, of 8 tiles or more each.  (One
+    portion of 509 tokens behind 6001, 32 heads of 128 over 8: 128 blocks alone take 106 us.)"""
+    return max(1, min(2 * 148 // blocks, tiles // 8))
+
+
+def prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, segments, n_segments, n_tiles, table, n_pages,
+                   n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits):
+    """``prefill`` over ``rows``, pages [n_pages, 2, Hkv, 64, head_dim] of float16 keys and bfloat16 values: ``key_factor`` float32 [n_pages, Hkv]
+    multiplies the keys back; ``value_marks`` int32 [n_pages, Hkv] and ``marks`` uint8 [n_pages, Hkv, 64] say where a position's value groups of 32 are NaN (they hold zeros then).  ``segments`` int32 [n_segments * 4] =
+    (first token, its position, tokens, row of ``table``), the longest contexts first; ``n_tiles``: of 128 / ``pack`` tokens over all of them.
+    ``splits`` > 1: ``part_o`` and ``part_ml`` hold 128 rows of head_dim and of 2 floats for every tile, head group and split.
+    From ``rows`` to ``part_ml`` they are addresses: ``kernels.kv4`` lays them out in one buffer and is what calls this."""
     lib = keys16_library(head_dim)
     word = _fault.tensor(out.device)
     _fault.mark()
     _check(lib, lib.qil_attn_tc_prefill_keys16(
-        c_void_p(q16), c_void_p(rows), _p(out), _p(tile_info), c_int(n_tiles), c_int(out.shape[0]), _p(table), c_int(table.shape[1]), c_int(n_q_heads),
-        c_int(n_kv_heads), c_int(n_pages), c_float(scale), c_int(window), c_void_p(q_factor), c_void_p(key_factor), c_void_p(value_marks),
-        c_void_p(marks), _p(word), _stream()), "attention (128-token tiles, float16 keys)")
+        _p(q), c_void_p(rows), _p(out), _p(segments), c_int(n_segments), c_int(n_tiles), c_int(out.shape[0]), _p(table), c_int(table.shape[1]),
+        c_int(n_q_heads), c_int(n_kv_heads), c_int(n_pages), c_float(scale), c_int(window), c_int(pack), c_int(splits), c_void_p(key_factor),
+        c_void_p(value_marks), c_void_p(marks), c_void_p(part_o), c_void_p(part_ml), _p(word), _stream()),
+        "attention (portions, float16 keys)", kernels=2 if splits > 1 else 1)
 
 
 def supports(head_dim, page_size, window, v_dim=None) -> bool:

@@ -43,7 +43,7 @@ _few_libs: dict = {}
 _P, _I, _F = c_void_p, c_int, c_float
 _STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 9 * [_I] + [_P]
 _READ = [_P, _P, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
-_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P] + 7 * [_I] + [_P]
+_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P] + 5 * [_I] + [_P]
 _SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
 _FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]
 
@@ -233,8 +233,8 @@ def describe_segments(first, starts, lens, rows) -> dict:
     ``single_tokens``, ``few_tokens``, ``portion_tokens``  the same token by token, four ints each, (token, its position, block-table row, the
                         longest context among these)
     ``b0.read`` ...     the portions in batches whose contexts are read back together: ``kv4.read``'s info; the same with the segment's first
-                        position (``spread``); the block table of the pages they are read to; query tiles of 64 and of 128 tokens over that
-                        table, (first token, its position, tokens, row of it) each
+                        position (``spread``); the block table of the pages they are read to; the segments and tiles of 64 of their tokens
+                        over that table, (first token, its position, tokens, row of it) each
     """
     lens, starts = np.asarray(lens, dtype=np.int64), np.asarray(starts, dtype=np.int64)
     first, rows = np.asarray(first, dtype=np.int64), np.asarray(rows, dtype=np.int64)
@@ -259,23 +259,32 @@ def describe_segments(first, starts, lens, rows) -> dict:
                                ("portions", "portion_tokens", lens > FEW_TOKENS)):
         indices = np.nonzero(some)[0]
         arrays[name], arrays[tokens] = segments(indices), one_by_one(indices)
-    portions = np.nonzero(lens > FEW_TOKENS)[0]
-    order = portions[np.argsort(-ends[portions], kind="stable")]
-    batch = 0
-    while len(order):
-        width = -(-int(ends[order[0]]) // READ_PAGE)               # pages a segment: of the longest, so that segment i's begin at i * width
-        taken = order[:max(1, MOST_READ // (width * READ_PAGE))]
-        order = order[len(taken):]
+    for batch, taken in enumerate(portion_batches(starts, lens)):
+        width = -(-int(ends[taken[0]]) // READ_PAGE)               # pages a segment: of the longest, so that segment i's begin at i * width
         local = np.arange(len(taken), dtype=np.int64)
         arrays[f"b{batch}.read"] = np.stack([rows[taken], np.zeros_like(local), ends[taken], local * width], axis=1).reshape(-1)
         arrays[f"b{batch}.spread"] = np.stack([rows[taken], starts[taken], ends[taken], local * width], axis=1).reshape(-1)
+        arrays[f"b{batch}.segments"] = np.stack([first[taken], starts[taken], lens[taken], local], axis=1).reshape(-1)
         arrays[f"b{batch}.table"] = np.arange(len(taken) * width, dtype=np.int64)
-        for name, tile in (("tiles", attention_mma.QUERY_TILE), ("big_tiles", attention_tc.TILE)):
-            found = [(first[i] + off, starts[i] + off, min(tile, lens[i] - off), j) for j, i in enumerate(taken) for off in range(0, int(lens[i]), tile)]
-            found.sort(key=lambda t: -(t[1] + t[2]))                # the longest contexts first: the short ones fill the gaps
-            arrays[f"b{batch}.{name}"] = np.array(found, dtype=np.int64).reshape(-1)
-        batch += 1
+        tile = attention_mma.QUERY_TILE
+        found = [(first[i] + off, starts[i] + off, min(tile, lens[i] - off), j) for j, i in enumerate(taken) for off in range(0, int(lens[i]), tile)]
+        found.sort(key=lambda t: -(t[1] + t[2]))                    # the longest contexts first: the short ones fill the gaps
+        arrays[f"b{batch}.tiles"] = np.array(found, dtype=np.int64).reshape(-1)
     return arrays
+
+
+def portion_batches(starts, lens) -> list:
+    """The segments of more than FEW_TOKENS in batches whose contexts are read back together, as arrays of their indices, the
+    longest contexts first."""
+    portions = np.nonzero(lens > FEW_TOKENS)[0]
+    ends = starts + lens
+    order, batches = portions[np.argsort(-ends[portions], kind="stable")], []
+    while len(order):
+        width = -(-int(ends[order[0]]) // READ_PAGE)
+        taken = max(1, MOST_READ // (width * READ_PAGE))
+        batches.append(order[:taken])
+        order = order[taken:]
+    return batches
 
 
 def refresh_single_tokens(arrays, starts) -> None:
@@ -290,14 +299,15 @@ class StepPlan:
     """A step's segments on the device, as ``attend`` reads them.  ``max_context``: the longest context; of a recorded step the
     longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest."""
 
-    def __init__(self, array, count, max_context, min_context=0, most_tokens=0):
+    def __init__(self, array, count, starts, lens, max_context, min_context=0):
+        """``starts`` and ``lens``: the segments' on the host (numpy)."""
         self.array, self.count = array, count
+        self.portion_lens = [lens[taken] for taken in portion_batches(starts, lens)]          # of the batches' segments
+        most_tokens = lens.max(initial=0)
         self.most_tokens = int(most_tokens)          # of a segment
         self.tokens = sum(count[name] for name in ("single_tokens", "few_tokens", "portion_tokens")) // 4
         self.max_context, self.min_context = int(max_context), int(min_context)
-        self.batches = 0
-        while f"b{self.batches}.read" in count:
-            self.batches += 1
+        self.batches = len(self.portion_lens)
 
     @classmethod
     def of_segments(cls, rows, starts, lens, device):
@@ -308,14 +318,13 @@ class StepPlan:
             raise KernelError("kv4.StepPlan: a row, a start and at least one token a segment")
         arrays = describe_segments(np.cumsum(lens) - lens, starts, lens, rows)
         array = {name: torch.from_numpy(values.astype(np.int32)).to(device) for name, values in arrays.items()}
-        return cls(array, {name: len(values) for name, values in arrays.items()}, int((starts + lens).max(initial=0)),
-                   most_tokens=lens.max(initial=0))
+        return cls(array, {name: len(values) for name, values in arrays.items()}, starts, lens, int((starts + lens).max(initial=0)))
 
     @classmethod
     def of_step(cls, ctx):
         """Of the step in flight, from the arrays that the planner made for it."""
         view = ctx.plans[PLAN_KEY]
-        return cls(view.array, view.count, ctx.max_context, ctx.min_context, most_tokens=max(ctx.h_seg_len))
+        return cls(view.array, view.count, ctx.h_seg_pos0, ctx.h_seg_len, ctx.max_context, ctx.min_context)
 
 
 # ------------------------------------------------------------------ attention
@@ -403,33 +412,37 @@ def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, he
         attention_f32.tiles(q, rows, out, array[f"b{batch}.tiles"], count[f"b{batch}.tiles"] // 4, table, n_q_heads, n_kv_heads, head_dim, READ_PAGE,
                             window, scale)
         return
-    # rows, queries, and what goes with them, in one buffer: every part from a 16-byte boundary on
-    tokens, heads = q.shape[0], n_pages * n_kv_heads
-    parts = (2 * size, 2 * q.numel(), 4 * tokens * n_q_heads, 4 * heads, 4 * heads, heads * READ_PAGE)
+    pack = attention_tc.keys16_pack(n_q_heads, n_kv_heads)
+    groups, n_tiles = n_q_heads // pack, int((-(-plan.portion_lens[batch] // (attention_tc.TILE // pack))).sum())
+    most = n_pages // segments
+    splits = attention_tc.keys16_splits(n_tiles * groups, min(most, -(-window // READ_PAGE) + 1) if window else most)
+    # rows, what goes with them and partial outputs, in one buffer: every part from a 128-byte boundary on
+    heads, parts = n_pages * n_kv_heads, n_tiles * groups * splits * attention_tc.TILE if splits > 1 else 0
     at, total = [], 0
-    for nbytes in parts:
+    for nbytes in (2 * size, 4 * heads, 4 * heads, heads * READ_PAGE, 4 * parts * head_dim, 8 * parts):
         at.append(total)
         total += -(-nbytes // 128) * 128
     held = extras.get("kv4_spread")
     if held is None or held.numel() < total:
         held = extras["kv4_spread"] = torch.empty(total, dtype=torch.uint8, device=q.device)
     base = held.data_ptr()
-    rows, q16, q_factor, key_factor, value_marks, marks = (base + offset for offset in at)
+    rows, key_factor, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
     lib = library()
-    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], array[f"b{batch}.spread"].data_ptr(), segments,
-                                   n_pages // segments, rows, key_factor, value_marks, marks, q.data_ptr(), q16, q_factor, tokens, n_q_heads, n_kv_heads,
-                                   head_dim, page_size, pages.shape[0], window, _stream()), "kv4.attend (rows of portions)")
-    attention_tc.prefill_keys16(q16, q_factor, rows, key_factor, value_marks, marks, out, array[f"b{batch}.big_tiles"],
-                                count[f"b{batch}.big_tiles"] // 4, table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window)
+    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], array[f"b{batch}.spread"].data_ptr(), segments, most,
+                                   rows, key_factor, value_marks, marks, n_kv_heads, head_dim, page_size, pages.shape[0], window, _stream()),
+           "kv4.attend (rows of portions)")
+    attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, n_tiles,
+                                table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits)
 
 
 def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, *, window=0, extras):
     """Causal attention of the tokens of ``plan`` (a :class:`StepPlan`) over 4-bit pages that hold their own keys and values already.
 
     q and out [N, n_q_heads * head_dim], bfloat16 or float32, the plan's tokens' rows of the flat batch; rows of other tokens are left as they
-    are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Positions whose page the block
-    table does not have are not seen; a token that sees none gets zeros.  ``extras``: a dict that the caller keeps from call to call
-    for the scratch memory; calls that may run at the same time (other streams) need one each."""
+    are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Segments of up to FEW_TOKENS
+    do not see positions whose page the block table does not have (a token that sees none gets zeros); longer ones need the pages of all
+    that they see.  A value that is NaN reaches the tokens that see it and no others.  ``extras``: a dict that the caller keeps from call
+    to call for the scratch memory; calls that may run at the same time (other streams, recorded graphs too) need one each."""
     device = _device_of(q, "q")
     dtype_code(q.dtype)
     _take(q, "q", q.dtype, 2, device); _take(out, "out", q.dtype, 2, device); _take(block_table, "block_table", torch.int32, 2, device)

@@ -95,7 +95,7 @@ def test_the_plan_of_a_step():
         read, table = arrays[f"b{batch}.read"].reshape(-1, 4), arrays[f"b{batch}.table"]
         spread, width = arrays[f"b{batch}.spread"].reshape(-1, 4), len(table) // len(read)
         assert (spread[:, (0, 2, 3)] == read[:, (0, 2, 3)]).all() and (read[:, 1] == 0).all()
-        for name, most in (("tiles", 64), ("big_tiles", 128)):
+        for name, most in (("tiles", 64), ("segments", 1 << 20)):
             for token, pos, count, local in arrays[f"b{batch}.{name}"].reshape(-1, 4):
                 row, begin, end, page = spread[local]
                 assert begin <= pos and count <= most and pos + count <= end <= width * kv4.READ_PAGE and page == local * width
@@ -103,7 +103,7 @@ def test_the_plan_of_a_step():
                     assert (name, token + i) not in seen
                     seen[name, token + i] = (row, pos + i)
         batch += 1
-    assert seen == {(name, t): at for name in ("tiles", "big_tiles")
+    assert seen == {(name, t): at for name in ("tiles", "segments")
                     for t, at in {**{6 + i: (2, 100 + i) for i in range(300)}, **{307 + i: (4, i) for i in range(64)}}.items()}
     # consecutive steps of the same single tokens: positions change, nothing else
     old = kv4.describe_segments([0, 1], [5, 9], [1, 1], [4, 2])
