@@ -168,6 +168,7 @@ struct AtParams {
     const unsigned char* marks;         // [page][kv head][64]: bit g: group g of 32 columns of that position's value is NaN
     const int4* segments;               // (first token, its position, tokens, block-table row) each, the longest contexts first
     int n_segments, pack;
+    int least;                          // segments of fewer tokens are left alone
     float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum)
     float2* part_ml;
 #endif
@@ -175,10 +176,10 @@ struct AtParams {
 
 #if QIL_KEYS_F16
 // The tile that block `index` of the tiles of all segments takes: those of a segment's last tokens first.
-__device__ __forceinline__ int4 at_tile(const int4* __restrict__ segments, int n_segments, int index, int tokens) {
-    for (int i = 0; i < n_segments; ++i) {
-        const int4 s = segments[i];
-        const int tiles = (s.z + tokens - 1) / tokens;
+__device__ __forceinline__ int4 at_tile(const AtParams& p, int index, int tokens) {
+    for (int i = 0; i < p.n_segments; ++i) {
+        const int4 s = p.segments[i];
+        const int tiles = s.z < p.least ? 0 : (s.z + tokens - 1) / tokens;
         if (index < tiles) {
             const int off = (tiles - 1 - index) * tokens;
             return make_int4(s.x + off, s.y + off, min(tokens, s.z - off), s.w);
@@ -218,7 +219,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     // tile_info: (first token in the flat batch, its absolute position, tokens, block-table row).  Rows past the tile's
     // tokens hold other tokens' queries or zeros; they see what its last token sees and are not stored.
 #if QIL_KEYS_F16
-    const int4 info = at_tile(p.segments, p.n_segments, blockIdx.y, AT_M / pack);
+    const int4 info = at_tile(p, blockIdx.y, AT_M / pack);
     if (info.z <= 0) return;
 #else
     const int4 info = tile_info[blockIdx.y];
@@ -644,7 +645,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 __global__ void __launch_bounds__(256) at_join_kernel(AtParams p, int splits) {
     const int row = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     qil_wait_for_producer();
-    const int4 info = at_tile(p.segments, p.n_segments, blockIdx.y, AT_M / p.pack);
+    const int4 info = at_tile(p, blockIdx.y, AT_M / p.pack);
     if (row >= info.z * p.pack) return;
     // the splits that hold anything, as the blocks counted them
     const int hi = info.y + info.z - 1;
@@ -787,9 +788,9 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
 }
 
 #if QIL_KEYS_F16
-// The keys of the pages (pages of 64) float16; see AtParams for the rest.  segments int32 [n_segments, 4]; n_tiles: of all segments,
-// 128 / pack tokens each; splits > 1: part_o float32 [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml as many pairs of rows.
-extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* segments, int n_segments, int n_tiles, int n_tokens,
+// The keys of the pages (pages of 64) float16; see AtParams for the rest.  segments int32 [n_segments, 4]; n_tiles: of all segments of at
+// least `least` tokens, 128 / pack tokens each; splits > 1: part_o float32 [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml as many pairs of rows.
+extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* segments, int n_segments, int least, int n_tiles, int n_tokens,
                                           const int* block_table, int table_stride, int n_q_heads, int n_kv_heads, int num_pages, float scale,
                                           int window, int pack, int splits, const float* key_factor, const int* value_marks,
                                           const unsigned char* marks, float* part_o, float* part_ml, int* error_word, cudaStream_t stream) {
@@ -799,7 +800,7 @@ extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* o
         QIL_REFUSE("attn_tc: %d heads of %d over %d a tile, %d splits", pack, n_q_heads, n_kv_heads, splits);
     AtParams p = {};
     p.key_factor = key_factor; p.value_marks = value_marks; p.marks = marks;
-    p.segments = (const int4*)segments; p.n_segments = n_segments; p.pack = pack;
+    p.segments = (const int4*)segments; p.n_segments = n_segments; p.least = least; p.pack = pack;
     p.part_o = part_o; p.part_ml = (float2*)part_ml;
     return at_launch(q, kv, out, segments, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, AT_N, num_pages, scale,
                      nullptr, 0, nullptr, 0.f, window, error_word, nullptr, p, splits, stream);

@@ -45,9 +45,6 @@ static constexpr int WARPS = 4, TILE = 32, STAGES = 2;
 static constexpr int STAGE_BYTES = 8 * RUN;            // 4 runs of keys, 4 of values
 static constexpr int MOST_SPANS = 128;
 static constexpr int MOST_LIFT = 90;
-#ifndef KV4_B1
-#define KV4_B1 4
-#endif
 
 struct Kv4Few {
     const bf16* q;                  // [tokens, q_heads * D]
@@ -58,7 +55,7 @@ struct Kv4Few {
     float* part_ml;                 // [few tokens][q_heads][n_spans][2]
     int* tickets;                   // [few tokens][q_heads], zero between launches
     const int* block_table;
-    int table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window;
+    int table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, most_tokens;
     float scale_log2;
 };
 
@@ -116,8 +113,9 @@ __device__ __forceinline__ void load_pairs(const uint8_t* at, unsigned (&w)[G]) 
     }
 }
 
-// How many blocks of this kernel share an SM (registers): what the launch bounds ask for.
-constexpr int blocks_a_sm(int nt) { return nt == 1 ? (D <= 128 ? KV4_B1 : 2) : nt == 2 ? (D <= 64 ? 4 : D <= 128 ? 3 : 1) : (D <= 32 ? 4 : D <= 64 ? 3 : 2); }
+// How many blocks of this kernel share an SM: what the launch bounds ask for.  Of heads of 128 and one tile of rows 4 blocks have 128
+// registers a thread and next to no spills; 2 with all the registers they want stream 4.2 TB/s where 4 stream 4.6, 5 spill (2.7).
+constexpr int blocks_a_sm(int nt) { return nt == 1 ? (D <= 128 ? 4 : 2) : (D <= 64 ? 4 : D <= 128 ? 3 : 1); }
 
 template <int NT>
 __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(const Kv4Few a) {
@@ -133,7 +131,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     const int4 more = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z + 1];
     const int first_token = info.x, pos0 = info.y, all_rows = info.z * share, longest = more.y;
     const int kv = blockIdx.y % a.kv_heads, row0 = blockIdx.y / a.kv_heads * 8 * NT;
-    if (row0 >= all_rows) return;
+    if (row0 >= all_rows || info.z > a.most_tokens) return;            // a segment of more tokens is somebody else's
     const int rows = min(8 * NT, all_rows - row0);
     const int pos_low = pos0 + row0 / share, pos_high = pos0 + (row0 + rows - 1) / share;        // of the block's rows
     const int low = a.window > 0 ? max(0, pos_low + 1 - a.window) : 0;
@@ -644,7 +642,7 @@ extern "C" int qil_kv4_few_head_dim() { return D; }
 extern "C" int qil_kv4_few_most_spans() { return MOST_SPANS; }
 extern "C" int qil_kv4_few_blocks_a_sm(int nt) { return blocks_a_sm(nt); }
 
-// info: see Kv4Few; most_tokens: of a segment; nt: 8-row tiles a block takes (1, 2 or 4; 1 or 2 of heads beyond 128).
+// info: see Kv4Few; most_tokens: segments of more are left alone; nt: 8-row tiles a block takes, 1 or 2.
 extern "C" int qil_kv4_few(const void* q, const void* pages, void* out, const void* info, int n, int most_tokens, int nt, void* part_o, void* part_ml,
                            void* tickets, int n_spans, const void* block_table, int table_width, int q_heads, int kv_heads, int page_size, int num_pages,
                            int window, float scale, cudaStream_t stream) {
@@ -654,12 +652,9 @@ extern "C" int qil_kv4_few(const void* q, const void* pages, void* out, const vo
         QIL_REFUSE("%d query heads, %d kv heads, %d spans", q_heads, kv_heads, n_spans);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages | (uintptr_t)info | (uintptr_t)part_o) & 15) QIL_REFUSE("kv4: operands must be 16-byte aligned");
     const Kv4Few a = {(const bf16*)q, (const uint8_t*)pages, (bf16*)out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
-                      (const int*)block_table, table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, scale * 1.4426950408889634f};
+                      (const int*)block_table, table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, most_tokens, scale * 1.4426950408889634f};
     const int rows = most_tokens * (q_heads / kv_heads);
     if (nt == 1) return launch<1>(a, n, rows, stream);
     if (nt == 2) return launch<2>(a, n, rows, stream);
-#if QIL_HEAD_DIM <= 128
-    if (nt == 4) return launch<4>(a, n, rows, stream);
-#endif
     QIL_REFUSE("kv4: %d tiles of rows a block", nt);
 }

@@ -498,7 +498,7 @@ struct Kv4Spread {
     float* key_factor;              // [page][kv head]
     int* value_marks;               // [page][kv head]
     unsigned char* marks;           // [page][kv head][64]
-    int table_width, kv_heads, dim, page_size, num_pages, window;
+    int table_width, kv_heads, dim, page_size, num_pages, window, least;
 };
 // The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.
 __device__ __forceinline__ float bring_up(float largest, float& up) {
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     const int4 mine = reinterpret_cast<const int4*>(a.info)[blockIdx.z];
     const int plane = blockIdx.y / a.kv_heads, head = blockIdx.y % a.kv_heads;
     const int page0 = blockIdx.x * SPREAD_PAGE;
-    if (page0 >= mine.z || (a.window > 0 && page0 + SPREAD_PAGE <= mine.y + 1 - a.window)) return;       // nobody will look
+    if (mine.z - mine.y < a.least || page0 >= mine.z || (a.window > 0 && page0 + SPREAD_PAGE <= mine.y + 1 - a.window)) return;       // nobody will look
     const int slot_out = warp * 8 + (lane >> 2), pos = page0 + slot_out;
     const size_t at = (size_t)(mine.w + blockIdx.x) * a.kv_heads + head;
     __half* dst = a.rows + ((((size_t)(mine.w + blockIdx.x) * 2 + plane) * a.kv_heads + head) * SPREAD_PAGE + slot_out) * dim + (lane & 3) * 8;
@@ -586,14 +586,14 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
 }
 
 extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int table_width, const void* info, int segments, int width, void* rows,
-                              void* key_factor, void* value_marks, void* marks, int kv_heads, int dim, int page_size, int num_pages, int window,
+                              void* key_factor, void* value_marks, void* marks, int kv_heads, int dim, int page_size, int num_pages, int window, int least,
                               cudaStream_t stream) {
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments >= 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
     const Kv4Spread a = {(const uint8_t*)pages, (const int*)block_table, (const int*)info, (__half*)rows, (float*)key_factor, (int*)value_marks,
-                         (unsigned char*)marks, table_width, kv_heads, dim, page_size, num_pages, window};
+                         (unsigned char*)marks, table_width, kv_heads, dim, page_size, num_pages, window, least};
     const dim3 grid(width, 2 * kv_heads, segments);
     void (*kernel)(Kv4Spread) = dim == 32 ? kv4_spread_kernel<1> : dim == 64 ? kv4_spread_kernel<2> : dim == 96 ? kv4_spread_kernel<3> : kv4_spread_kernel<4>;
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);

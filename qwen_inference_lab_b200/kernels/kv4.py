@@ -26,8 +26,12 @@ from .ops import F32, KernelError, _check, _need, dtype_code
 GROUP = 32
 MOST_DIM = 256
 PLAN_KEY = "kv4_attention"        # the step planner whose arrays ``attend`` reads (``describe_segments`` makes them)
-#: Tokens of a segment up to which the kernels that walk the codes take it; longer portions' rows are read back once and attended to
-#: as ordinary pages.
+#: Rows (tokens of a segment times query heads of a kv head) up to which the kernel that walks the codes takes more than one token; of
+#: more the rows are read back once and attended to as 16-bit pages.  Measured (us, this kernel / the other one; 4 heads of 128 a kv head):
+#: 8 segments behind 4000 of 2, 4, 8, 16 tokens 21 / 72, 40 / 72, 59 / 72, 94 / 74; one segment 11 / 25, 18 / 25, 23 / 25, 27 / 26; 8
+#: segments behind 500 8.7 / 19, 13 / 19, 14 / 19, 22 / 22.
+FEW_ROWS = 32
+#: Tokens of a segment up to which the 32-bit path takes them one by one.
 FEW_TOKENS = 8
 #: Positions per page of rows that are read back for a portion, and the most of them at a time (of several portions; a single
 #: one may be longer): 8 heads of 128 in bfloat16 take 4 KB a position.
@@ -43,7 +47,7 @@ _few_libs: dict = {}
 _P, _I, _F = c_void_p, c_int, c_float
 _STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 9 * [_I] + [_P]
 _READ = [_P, _P, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
-_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P] + 5 * [_I] + [_P]
+_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P] + 6 * [_I] + [_P]
 _SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
 _FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]
 
@@ -62,7 +66,7 @@ def few_library(head_dim):
         if lib.qil_kv4_few_head_dim() != head_dim:
             raise KernelError("the 4-bit attention library was built for another head size")
         lib.qil_kv4_few.argtypes = _FEW
-        held = _few_libs[head_dim] = (lib, lib.qil_kv4_few_most_spans(), {nt: lib.qil_kv4_few_blocks_a_sm(c_int(nt)) for nt in (1, 2, 4)})
+        held = _few_libs[head_dim] = (lib, lib.qil_kv4_few_most_spans(), {nt: lib.qil_kv4_few_blocks_a_sm(c_int(nt)) for nt in (1, 2)})
     return held
 
 
@@ -228,13 +232,13 @@ def describe_segments(first, starts, lens, rows) -> dict:
     """A step's segments as ``attend`` wants them (numpy int64 arrays in, one entry per segment: first token in the flat batch,
     its absolute position, tokens, block-table row).
 
-    ``singles``, ``few``, ``portions``  the segments of one token, of up to FEW_TOKENS and the others: eight ints each, (first token, its
+    ``singles``, ``few``, ``multi``  the segments of one token, of 2 to FEW_ROWS and of any more than one: eight ints each, (first token, its
                         position, tokens, block-table row, tokens of the segments before in this array, the longest context among these, 0, 0)
-    ``single_tokens``, ``few_tokens``, ``portion_tokens``  the same token by token, four ints each, (token, its position, block-table row, the
-                        longest context among these)
-    ``b0.read`` ...     the portions in batches whose contexts are read back together: ``kv4.read``'s info; the same with the segment's first
-                        position (``spread``); the block table of the pages they are read to; the segments and tiles of 64 of their tokens
-                        over that table, (first token, its position, tokens, row of it) each
+    ``single_tokens``, ``few_tokens``, ``portion_tokens``  the segments of one token, of 2 to FEW_TOKENS and the others token by token, four
+                        ints each, (token, its position, block-table row, the longest context among these)
+    ``b0.spread`` ...   the segments of more than one token in batches whose contexts are read back together: (block-table row, first position,
+                        end, first page); ``kv4.read``'s info of those beyond FEW_TOKENS; the block table of the pages they are read to; the
+                        segments, and tiles of 64 of their tokens beyond FEW_TOKENS, over that table: (first token, its position, tokens, row of it)
     """
     lens, starts = np.asarray(lens, dtype=np.int64), np.asarray(starts, dtype=np.int64)
     first, rows = np.asarray(first, dtype=np.int64), np.asarray(rows, dtype=np.int64)
@@ -255,28 +259,30 @@ def describe_segments(first, starts, lens, rows) -> dict:
         return np.stack([first[of] + offset, starts[of] + offset, rows[of], np.full_like(of, ends[indices].max())], axis=1).reshape(-1)
 
     arrays = {}
-    for name, tokens, some in (("singles", "single_tokens", lens == 1), ("few", "few_tokens", (lens > 1) & (lens <= FEW_TOKENS)),
-                               ("portions", "portion_tokens", lens > FEW_TOKENS)):
-        indices = np.nonzero(some)[0]
-        arrays[name], arrays[tokens] = segments(indices), one_by_one(indices)
+    for name, some in (("singles", lens == 1), ("few", (lens > 1) & (lens <= FEW_ROWS)), ("multi", lens > 1)):
+        arrays[name] = segments(np.nonzero(some)[0])
+    for name, some in (("single_tokens", lens == 1), ("few_tokens", (lens > 1) & (lens <= FEW_TOKENS)), ("portion_tokens", lens > FEW_TOKENS)):
+        arrays[name] = one_by_one(np.nonzero(some)[0])
     for batch, taken in enumerate(portion_batches(starts, lens)):
         width = -(-int(ends[taken[0]]) // READ_PAGE)               # pages a segment: of the longest, so that segment i's begin at i * width
         local = np.arange(len(taken), dtype=np.int64)
-        arrays[f"b{batch}.read"] = np.stack([rows[taken], np.zeros_like(local), ends[taken], local * width], axis=1).reshape(-1)
+        counts = np.where(lens[taken] > FEW_TOKENS, ends[taken], 0)
+        arrays[f"b{batch}.read"] = np.stack([rows[taken], np.zeros_like(local), counts, local * width], axis=1).reshape(-1)
         arrays[f"b{batch}.spread"] = np.stack([rows[taken], starts[taken], ends[taken], local * width], axis=1).reshape(-1)
         arrays[f"b{batch}.segments"] = np.stack([first[taken], starts[taken], lens[taken], local], axis=1).reshape(-1)
         arrays[f"b{batch}.table"] = np.arange(len(taken) * width, dtype=np.int64)
         tile = attention_mma.QUERY_TILE
-        found = [(first[i] + off, starts[i] + off, min(tile, lens[i] - off), j) for j, i in enumerate(taken) for off in range(0, int(lens[i]), tile)]
+        found = [(first[i] + off, starts[i] + off, min(tile, lens[i] - off), j) for j, i in enumerate(taken) if lens[i] > FEW_TOKENS
+                 for off in range(0, int(lens[i]), tile)]
         found.sort(key=lambda t: -(t[1] + t[2]))                    # the longest contexts first: the short ones fill the gaps
         arrays[f"b{batch}.tiles"] = np.array(found, dtype=np.int64).reshape(-1)
     return arrays
 
 
 def portion_batches(starts, lens) -> list:
-    """The segments of more than FEW_TOKENS in batches whose contexts are read back together, as arrays of their indices, the
-    longest contexts first."""
-    portions = np.nonzero(lens > FEW_TOKENS)[0]
+    """The segments of more than one token in batches whose contexts are read back together, as arrays of their indices, the longest
+    contexts first."""
+    portions = np.nonzero(lens > 1)[0]
     ends = starts + lens
     order, batches = portions[np.argsort(-ends[portions], kind="stable")], []
     while len(order):
@@ -303,12 +309,9 @@ class StepPlan:
         """``starts`` and ``lens``: the segments' on the host (numpy)."""
         self.array, self.count = array, count
         self.portion_lens = [lens[taken] for taken in portion_batches(starts, lens)]          # of the batches' segments
-        most_tokens = lens.max(initial=0)
-        self.most_tokens = int(most_tokens)          # of a segment
-        self.tokens = sum(count[name] for name in ("single_tokens", "few_tokens", "portion_tokens")) // 4
+        self.multi_lens = lens[lens > 1]
+        self.tokens = int(lens.sum())
         self.max_context, self.min_context = int(max_context), int(min_context)
-        self.batches = len(self.portion_lens)
-
     @classmethod
     def of_segments(cls, rows, starts, lens, device):
         """Of a flat batch of segments one after another: their block-table rows, the absolute position of each one's first token and
@@ -328,37 +331,39 @@ class StepPlan:
 
 
 # ------------------------------------------------------------------ attention
-_sms = None
-
-
-def _slots(blocks_per_sm) -> int:
-    global _sms
-    if _sms is None:
-        _sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count if torch.cuda.is_available() else 148
-    return _sms * blocks_per_sm
-
-
 #: Keys that a block of the span kernels takes at a time: a tile of 32 for each of its four warps.
 STEP = 128
+#: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 and one tile of rows (one B200, a
+#: recorded chain of the kernel; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
+STEP_US, SINGLES_STEP_US = (1.18, 1.58, 2.5, 2.6), (2.0, 2.4, 3.0)
+#: ... a launch and a block's start, what the join costs at all and what every span adds.  Measured against the model (us): one request
+#: behind 8191 and 8, 16, 22, 32, 64 spans 15.1, 10.7, 13.3, 10.9, 12.9 (16.6, 12.6, 13.1, 12.3, 12.9); 8 requests and 4, 6, 8, 12 spans
+#: 32.8, 35.7, 28.6, 37.1; 48 requests and 1, 2, 3, 4 spans 157, 131, 118, 124.
+START_US, JOIN_US, SPAN_US = tuning.KV4_START_US, tuning.KV4_JOIN_US, tuning.KV4_SPAN_US
+SMS = 148
 
 
 @functools.lru_cache(maxsize=4096)
-def _plan(blocks_per_span, slots, lo, hi, most) -> int:
-    """The number of spans with the lowest cost per step of keys at both ends of [lo, hi] steps of longest context.  A wave of blocks takes
-    the steps of a span and a start-up; every span costs the join something."""
+def _plan(blocks_per_span, step_us, size, lo, hi, most) -> int:
+    """The number of spans that costs least per step of keys at both ends of [lo, hi] steps of longest context."""
+    full = SMS * len(step_us)
+
     def cost(steps, n):
         each = -(-steps // n)
-        n = -(-steps // each)
-        return (-(-blocks_per_span * n // slots) * (each + tuning.KV4_SPAN_STARTUP) + tuning.KV4_SPAN_JOIN * n) / steps
+        n = -(-steps // each)                           # spans that hold anything
+        waves, rest = divmod(blocks_per_span * n, full)
+        time = each * size * (waves * step_us[-1] + (step_us[-(-rest // SMS) - 1] if rest else 0.0)) + START_US * (waves + (rest > 0))
+        return (time + (JOIN_US + SPAN_US * n if n > 1 else 0.0)) / steps
     return min(range(1, min(hi, most) + 1), key=lambda n: cost(hi, n) + (cost(lo, min(n, lo)) if lo != hi else 0.0))
 
 
-def _spans(blocks_per_span, slots, plan, window, most) -> int:
+def _spans(blocks_per_span, step_us, size, plan, window, most) -> int:
     """Parts to cut the contexts into."""
-    reach = lambda context: min(context, window + STEP) if window else context
-    hi = max(1, -(-reach(plan.max_context) // STEP))
-    lo = max(1, min(hi, -(-reach(plan.min_context or plan.max_context) // STEP)))
-    return _plan(blocks_per_span, slots, lo, hi, max(1, most))
+    hi, lo = plan.max_context, plan.min_context or plan.max_context
+    if window:
+        hi, lo = min(hi, window + STEP), min(lo, window + STEP)
+    hi = max(1, -(-hi // STEP))
+    return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most))
 
 
 def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
@@ -375,11 +380,11 @@ def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
 def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib, most, blocks_a_sm = few_library(head_dim)
     rows = most_tokens * (n_q_heads // n_kv_heads)
-    nt = 1 if rows <= 8 else 2 if rows <= 16 or head_dim > 128 else 4
+    nt = 1 if rows <= 8 else 2
     blocks = n * n_kv_heads * -(-rows // (8 * nt))
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
-    n_spans = _spans(blocks, _slots(blocks_a_sm[nt]), plan, window, most)
+    n_spans = _spans(blocks, STEP_US[:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
     part_o, part_ml, tickets = _scratch(extras, q.device, tokens, n_q_heads, n_spans, head_dim)
     _check(lib, lib.qil_kv4_few(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, most_tokens, nt, part_o.data_ptr(),
                                 part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads,
@@ -390,20 +395,22 @@ def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, h
     lib = library()
     chunks = -(-(n_q_heads // n_kv_heads) // lib.qil_kv4_singles_heads(n_q_heads // n_kv_heads))
     most = attention_f32.MOST_SCRATCH // (4 * n * n_q_heads * head_dim)
-    n_spans = _spans(n * n_kv_heads * chunks, _slots(3), plan, window, most)
+    n_spans = _spans(n * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, plan, window, most)
     part_o, part_ml, tickets = _scratch(extras, q.device, n, n_q_heads, n_spans, head_dim)
     _check(lib, lib.qil_kv4_singles(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, part_o.data_ptr(), part_ml.data_ptr(),
                                     tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads, n_kv_heads, head_dim,
                                     page_size, pages.shape[0], window, scale, dtype_code(q.dtype), _stream()), "kv4.attend (single tokens)")
 
 
-def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
-    """A batch of portions: their contexts' rows as pages of 64 positions, then the attention over those."""
+def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
+    """A batch of portions of at least ``least`` tokens: their contexts' rows as pages of 64 positions, then the attention over those."""
     array, count = plan.array, plan.count
     segments, n_pages = count[f"b{batch}.read"] // 4, count[f"b{batch}.table"]
     table = array[f"b{batch}.table"][:n_pages].view(segments, n_pages // segments)
     size = n_pages * 2 * n_kv_heads * READ_PAGE * head_dim
     if q.dtype == torch.float32:
+        if not count[f"b{batch}.tiles"]:
+            return
         held = extras.get("kv4_rows")
         if held is None or held.numel() < size:
             held = extras["kv4_rows"] = torch.empty(size, dtype=torch.float32, device=q.device)
@@ -413,7 +420,10 @@ def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, he
                             window, scale)
         return
     pack = attention_tc.keys16_pack(n_q_heads, n_kv_heads)
-    groups, n_tiles = n_q_heads // pack, int((-(-plan.portion_lens[batch] // (attention_tc.TILE // pack))).sum())
+    lens = plan.portion_lens[batch]
+    groups, n_tiles = n_q_heads // pack, int((-(-lens[lens >= least] // (attention_tc.TILE // pack))).sum())
+    if not n_tiles:
+        return
     most = n_pages // segments
     splits = attention_tc.keys16_splits(n_tiles * groups, min(most, -(-window // READ_PAGE) + 1) if window else most)
     # rows, what goes with them and partial outputs, in one buffer: every part from a 128-byte boundary on
@@ -429,9 +439,9 @@ def _portions(plan, batch, q, pages, out, block_table, n_q_heads, n_kv_heads, he
     rows, key_factor, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
     lib = library()
     _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], array[f"b{batch}.spread"].data_ptr(), segments, most,
-                                   rows, key_factor, value_marks, marks, n_kv_heads, head_dim, page_size, pages.shape[0], window, _stream()),
+                                   rows, key_factor, value_marks, marks, n_kv_heads, head_dim, page_size, pages.shape[0], window, least, _stream()),
            "kv4.attend (rows of portions)")
-    attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, n_tiles,
+    attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
                                 table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits)
 
 
@@ -463,19 +473,22 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
                 _singles(array[name], count[name] // 4, plan, *shape)
         if count["portion_tokens"]:
             if attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads):
-                for batch in range(plan.batches):
-                    _portions(plan, batch, *shape)
+                for batch in range(len(plan.portion_lens)):
+                    _portions(plan, batch, FEW_TOKENS + 1, *shape)
             else:       # heads of a size that the tile kernel does not take: token by token
                 _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan, *shape)
         return out
     if count["singles"]:
         _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, *shape)
-    if count["few"]:
-        _few(array["few"], count["few"] // 8, count["few_tokens"] // 4, FEW_TOKENS, plan, *shape)
-    if count["portions"]:
-        if attention_tc.supports(head_dim, READ_PAGE, window):
-            for batch in range(plan.batches):
-                _portions(plan, batch, *shape)
-        else:           # heads beyond 128
-            _few(array["portions"], count["portions"] // 8, count["portion_tokens"] // 4, plan.most_tokens, plan, *shape)
+    if len(plan.multi_lens):
+        if not attention_tc.supports(head_dim, READ_PAGE, window):          # heads beyond 128
+            _few(array["multi"], len(plan.multi_lens), int(plan.multi_lens.sum()), int(plan.multi_lens.max()), plan, *shape)
+            return out
+        most = FEW_ROWS // (n_q_heads // n_kv_heads)           # tokens
+        few = plan.multi_lens[plan.multi_lens <= most]
+        if len(few):
+            _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, *shape)
+        if len(few) < len(plan.multi_lens):
+            for batch in range(len(plan.portion_lens)):
+                _portions(plan, batch, max(most, 1) + 1, *shape)
     return out

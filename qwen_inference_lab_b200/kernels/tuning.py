@@ -61,6 +61,8 @@ QKV_TAIL_MIN_ROWS = _tuned("QKV_TAIL_MIN_ROWS", 512)
 #: 8192 (batch 8: 4.84 ms with 5 or 6 spans, 4.97 with 4, 5.1 with 7 to 9; batch 1 flat from 16 to 43 spans).
 SPAN_STARTUP_TILES = _tuned("SPAN_STARTUP_TILES", 2.0)
 SPAN_MERGE_TILES = _tuned("SPAN_MERGE_TILES", 0.15)
-#: The same of the attention over 4-bit pages, in units of the time a block takes for its 128 keys.
-KV4_SPAN_STARTUP = _tuned("KV4_SPAN_STARTUP", 3.0)
-KV4_SPAN_JOIN = _tuned("KV4_SPAN_JOIN", 0.1)
+#: The attention over 4-bit pages (``kernels.kv4``), in us: a launch and a block's start, what joining the spans of a context costs, and
+#: what every span adds to it.
+KV4_START_US = _tuned("KV4_START_US", 3.6)
+KV4_JOIN_US = _tuned("KV4_JOIN_US", 3.0)
+KV4_SPAN_US = _tuned("KV4_SPAN_US", 0.08)

@@ -86,15 +86,16 @@ def test_the_plan_of_a_step():
     arrays = kv4.describe_segments(first, starts, lens, rows)
     assert arrays["singles"].reshape(-1, 8).tolist() == [[0, 5, 1, 0, 0, 71, 0, 0], [306, 70, 1, 1, 1, 71, 0, 0]]
     assert arrays["few"].reshape(-1, 8).tolist() == [[1, 9, 5, 3, 0, 14, 0, 0]]
-    assert arrays["portions"].reshape(-1, 8)[:, :5].tolist() == [[6, 100, 300, 2, 0], [307, 0, 64, 4, 300]]
+    assert arrays["multi"].reshape(-1, 8)[:, :5].tolist() == [[1, 9, 5, 3, 0], [6, 100, 300, 2, 5], [307, 0, 64, 4, 305]]
     assert arrays["few_tokens"].reshape(-1, 4).tolist() == [[1 + i, 9 + i, 3, 14] for i in range(5)]
-    # every token of a portion lies in one tile of its batch, whose row is that of the segment's pages
+    # every token of a portion lies in one segment and, beyond a few tokens, in one tile of its batch, whose row is that of the segment's pages
     seen = {}
     batch = 0
     while f"b{batch}.read" in arrays:
         read, table = arrays[f"b{batch}.read"].reshape(-1, 4), arrays[f"b{batch}.table"]
         spread, width = arrays[f"b{batch}.spread"].reshape(-1, 4), len(table) // len(read)
-        assert (spread[:, (0, 2, 3)] == read[:, (0, 2, 3)]).all() and (read[:, 1] == 0).all()
+        assert (spread[:, (0, 3)] == read[:, (0, 3)]).all() and (read[:, 1] == 0).all()
+        assert (read[:, 2] == np.where(spread[:, 2] - spread[:, 1] > kv4.FEW_TOKENS, spread[:, 2], 0)).all()
         for name, most in (("tiles", 64), ("segments", 1 << 20)):
             for token, pos, count, local in arrays[f"b{batch}.{name}"].reshape(-1, 4):
                 row, begin, end, page = spread[local]
@@ -103,8 +104,9 @@ def test_the_plan_of_a_step():
                     assert (name, token + i) not in seen
                     seen[name, token + i] = (row, pos + i)
         batch += 1
-    assert seen == {(name, t): at for name in ("tiles", "segments")
-                    for t, at in {**{6 + i: (2, 100 + i) for i in range(300)}, **{307 + i: (4, i) for i in range(64)}}.items()}
+    tiled = {**{6 + i: (2, 100 + i) for i in range(300)}, **{307 + i: (4, i) for i in range(64)}}
+    assert seen == {**{(name, t): at for name in ("tiles", "segments") for t, at in tiled.items()},
+                    **{("segments", 1 + i): (3, 9 + i) for i in range(5)}}
     # consecutive steps of the same single tokens: positions change, nothing else
     old = kv4.describe_segments([0, 1], [5, 9], [1, 1], [4, 2])
     kv4.refresh_single_tokens(old, np.array([6, 31]))
@@ -122,9 +124,19 @@ def test_long_contexts_are_read_in_batches():
     assert all(sum(len(arrays[f"b{i}.read"]) // 4 for i in range(k)) <= 4 for k in (1, 2))
 
 
+def test_spans_fill_the_gpu():
+    """More requests, fewer spans; a context of one step is not cut; never more spans than there is room for."""
+    plan = lambda context: kv4.StepPlan.of_segments([0], [context - 1], [1], "cpu")
+    spans = lambda blocks, context, window=0, most=128: kv4._spans(blocks, kv4.STEP_US, 1.0, plan(context), window, most)
+    assert spans(8, 100) == 1 and spans(8, 8192) >= 16 and spans(64, 8192) == 8 and spans(2000, 8192) <= 2
+    assert spans(8, 8192, most=3) == 3 and spans(8, 100000, window=100) == spans(8, 228)
+    counts = [spans(blocks, 16384) for blocks in (8, 32, 128, 600)]
+    assert counts == sorted(counts, reverse=True)
+
+
 def test_a_plan_of_host_segments():
     plan = kv4.StepPlan.of_segments([2, 0], [7, 0], [1, 20], "cpu")
-    assert plan.max_context == 20 and plan.most_tokens == 20 and plan.batches == 1 and plan.count["singles"] == 8
+    assert plan.max_context == 20 and plan.tokens == 21 and len(plan.portion_lens) == 1 and plan.count["singles"] == 8
     empty = kv4.StepPlan.of_segments([], [], [], "cpu")
     assert empty.max_context == 0 and not any(empty.count.values())
     for wrong in (([0], [0], [0]), ([0], [-1], [1]), ([-1], [0], [1]), ([0, 1], [0], [1])):
