@@ -333,9 +333,10 @@ class StepPlan:
 # ------------------------------------------------------------------ attention
 #: Keys that a block of the span kernels takes at a time: a tile of 32 for each of its four warps.
 STEP = 128
-#: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 and one tile of rows (one B200, a
+#: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 by its tiles of rows (one B200, a
 #: recorded chain of the kernel; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
-STEP_US, SINGLES_STEP_US = (1.18, 1.58, 2.5, 2.6), (2.0, 2.4, 3.0)
+STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 3.2, 4.0, 4.6)}
+SINGLES_STEP_US = (2.0, 2.4, 3.0)
 #: ... a launch and a block's start, what the join costs at all and what every span adds.  Measured against the model (us): one request
 #: behind 8191 and 8, 16, 22, 32, 64 spans 15.1, 10.7, 13.3, 10.9, 12.9 (16.6, 12.6, 13.1, 12.3, 12.9); 8 requests and 4, 6, 8, 12 spans
 #: 32.8, 35.7, 28.6, 37.1; 48 requests and 1, 2, 3, 4 spans 157, 131, 118, 124.
@@ -384,7 +385,7 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
     blocks = n * n_kv_heads * -(-rows // (8 * nt))
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
-    n_spans = _spans(blocks, STEP_US[:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
+    n_spans = _spans(blocks, STEP_US[nt][:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
     part_o, part_ml, tickets = _scratch(extras, q.device, tokens, n_q_heads, n_spans, head_dim)
     _check(lib, lib.qil_kv4_few(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, most_tokens, nt, part_o.data_ptr(),
                                 part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads,

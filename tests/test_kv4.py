@@ -127,7 +127,7 @@ def test_long_contexts_are_read_in_batches():
 def test_spans_fill_the_gpu():
     """More requests, fewer spans; a context of one step is not cut; never more spans than there is room for."""
     plan = lambda context: kv4.StepPlan.of_segments([0], [context - 1], [1], "cpu")
-    spans = lambda blocks, context, window=0, most=128: kv4._spans(blocks, kv4.STEP_US, 1.0, plan(context), window, most)
+    spans = lambda blocks, context, window=0, most=128: kv4._spans(blocks, kv4.STEP_US[1], 1.0, plan(context), window, most)
     assert spans(8, 100) == 1 and spans(8, 8192) >= 16 and spans(64, 8192) == 8 and spans(2000, 8192) <= 2
     assert spans(8, 8192, most=3) == 3 and spans(8, 100000, window=100) == spans(8, 228)
     counts = [spans(blocks, 16384) for blocks in (8, 32, 128, 600)]
