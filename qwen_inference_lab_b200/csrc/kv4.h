@@ -28,12 +28,18 @@ __device__ __forceinline__ int kv4_pair_at(int group, int slot, int groups) { re
 __device__ __forceinline__ float kv4_step(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float kv4_base(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// The physical page of a position, or -1 where the table has none (never one outside the pool).
-__device__ __forceinline__ int kv4_page(const int* __restrict__ table_row, int table_width, int position, int page_size, int num_pages) {
-    const int index = position / page_size;
-    const int page = (position >= 0 && index < table_width) ? table_row[index] : -1;
-    return page < num_pages ? page : -1;
-}
+// Block tables [rows][width] of physical pages by position / page size.
+struct Kv4Table {
+    const int* pages;
+    int rows, width, page_size, num_pages;
+    // The page of a request's position, or -1 where the table has none: never one outside the pool, whatever row and position are.
+    __device__ __forceinline__ int page(int row, int position) const {
+        const int index = position / page_size;
+        if (row < 0 || row >= rows || position < 0 || index >= width) return -1;
+        const int found = pages[(size_t)row * width + index];
+        return found < num_pages ? found : -1;
+    }
+};
 
 // The share of a context that a span kernel's block takes.  The longest context of the step is cut into at most n_spans parts of
 // equal length, a multiple of `tile`; a token's own keys [low, end) start at a tile's border.  Empty when the context is over before.
@@ -54,3 +60,11 @@ __device__ __forceinline__ Kv4Span kv4_span(int span, int n_spans, int longest, 
     s.last = (span == s.count - 1 || at + length > end) ? end : (int)(at + length);
     return s;
 }
+
+// What has to be done once on every device: a flag for each.
+struct Kv4PerDevice {
+    bool flags[64] = {};
+    int device = 0;
+    bool here() { return cudaGetDevice(&device) == cudaSuccess && device < 64 && flags[device]; }
+    void done() { if (device < 64) flags[device] = true; }
+};

@@ -21,8 +21,8 @@ struct Kv4Singles {
     float* part_o;                  // [n][q_heads][n_spans][dim]
     float* part_ml;                 // [n][q_heads][n_spans][2]
     int* tickets;                   // [n][kv_heads * head chunks], zero between launches
-    const int* block_table;
-    int table_width, n_spans, q_heads, kv_heads, dim, page_size, num_pages, window;
+    Kv4Table table;
+    int n_spans, q_heads, kv_heads, dim, window;
     float scale_log2;
 };
 
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
     const int reach = a.window > 0 ? min(longest, a.window + TILE - 1) : longest;       // a window begins anywhere in its first tile
     const Kv4Span span = kv4_span(blockIdx.x, a.n_spans, reach, low, pos + 1, TILE);
     if ((int)blockIdx.x >= span.count) return;
-    const int* table = a.block_table + (size_t)row * a.table_width;
+    const int page_size = a.table.page_size;
     for (int i = threadIdx.x; i < HEADS * dim; i += 32 * WARPS) {
         const int h = i / dim;
         qs[i] = h < heads ? to_f32<T>(reinterpret_cast<const T*>(a.q)[((size_t)token * a.q_heads + head0 + h) * dim + i % dim]) * a.scale_log2 : 0.f;
@@ -69,12 +69,12 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
     for (int k0 = span.first / TILE * TILE + warp * TILE; k0 < span.last; k0 += WARPS * TILE) {
         const int key = k0 + lane;
         const bool seen = key >= span.first && key < span.last;
-        const int page = seen ? kv4_page(table, a.table_width, key, a.page_size, a.num_pages) : -1;
+        const int page = seen ? a.table.page(row, key) : -1;
         float score[HEADS];
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) score[h] = page >= 0 ? 0.f : -INFINITY;
         if (page >= 0) {
-            const uint8_t* run = a.pages + kv4_run_at(page, 0, kv, key % a.page_size, a.kv_heads, a.page_size, groups);
+            const uint8_t* run = a.pages + kv4_run_at(page, 0, kv, key % page_size, a.kv_heads, page_size, groups);
             for (int g = 0; g < groups; ++g) {
                 const uint4 codes = *reinterpret_cast<const uint4*>(run + kv4_code_at(g, key));
                 const unsigned pair = *reinterpret_cast<const unsigned*>(run + kv4_pair_at(g, key, groups));
@@ -114,8 +114,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
             const int j = j0 + my_side;
             const int at = __shfl_sync(0xffffffffu, page, j & 31);
             if (!owns || j >= TILE || at < 0) continue;
-            const int slot = (k0 + j) % a.page_size;
-            const uint8_t* run = a.pages + kv4_run_at(at, 1, kv, slot, a.kv_heads, a.page_size, groups);
+            const int slot = (k0 + j) % page_size;
+            const uint8_t* run = a.pages + kv4_run_at(at, 1, kv, slot, a.kv_heads, page_size, groups);
 #pragma unroll
             for (int n = 0; n < QUADS; ++n) {
                 const int quad = my_quad + 32 * n;
@@ -208,8 +208,12 @@ template <typename T, int HEADS, int QUADS>
 static cudaError_t launch_singles(const Kv4Singles& a, int n, cudaStream_t stream) {
     const int share = a.q_heads / a.kv_heads, chunks = (share + HEADS - 1) / HEADS;
     const size_t smem = sizeof(float) * (HEADS * a.dim + WARPS * TILE * HEADS + WARPS * HEADS * a.dim + WARPS * HEADS * 2);
-    static cudaError_t ready = cudaFuncSetAttribute(kv4_singles_kernel<T, HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-    if (ready != cudaSuccess) return ready;
+    static Kv4PerDevice ready;
+    if (!ready.here()) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_singles_kernel<T, HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        if (e != cudaSuccess) return e;
+        ready.done();
+    }
     return qil_launch_chained(kv4_singles_kernel<T, HEADS, QUADS>, dim3(a.n_spans, a.kv_heads * chunks, n), dim3(32 * WARPS), smem, stream, a);
 }
 
@@ -219,14 +223,14 @@ static int heads_a_block(int share) { return share >= 5 ? 8 : share >= 3 ? 4 : s
 extern "C" int qil_kv4_singles_heads(int share) { return heads_a_block(share); }
 
 extern "C" int qil_kv4_singles(const void* q, const void* pages, void* out, const void* info, int n, void* part_o, void* part_ml, void* tickets,
-                               int n_spans, const void* block_table, int table_width, int q_heads, int kv_heads, int dim, int page_size,
+                               int n_spans, const void* block_table, int table_height, int table_width, int q_heads, int kv_heads, int dim, int page_size,
                                int num_pages, int window, float scale, int act, cudaStream_t stream) {
     if (n <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n > 65535 || n_spans < 1) QIL_REFUSE("%d query heads, %d kv heads, %d tokens, %d spans", q_heads, kv_heads, n, n_spans);
     const Kv4Singles a = {q, (const uint8_t*)pages, out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
-                          (const int*)block_table, table_width, n_spans, q_heads, kv_heads, dim, page_size, num_pages, window,
+                          {(const int*)block_table, table_height, table_width, page_size, num_pages}, n_spans, q_heads, kv_heads, dim, window,
                           scale * 1.4426950408889634f};
     const int heads = heads_a_block(q_heads / kv_heads);
     cudaError_t e = cudaSuccess;

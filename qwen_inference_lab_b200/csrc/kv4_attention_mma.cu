@@ -54,8 +54,9 @@ struct Kv4Few {
     float* part_o;                  // [few tokens][q_heads][n_spans][D]
     float* part_ml;                 // [few tokens][q_heads][n_spans][2]
     int* tickets;                   // [few tokens][q_heads], zero between launches
-    const int* block_table;
-    int table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, most_tokens;
+    Kv4Table table;
+    int n_spans, q_heads, kv_heads, window, most_tokens;
+    int settled;                    // info and the table are older than the kernel before this one
     float scale_log2;
 };
 
@@ -127,36 +128,36 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     __shared__ int last_block;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int share = a.q_heads / a.kv_heads;
+    if (!a.settled) qil_wait_for_producer();                 // 0.9 us of a launch's 4.7 when it is chained to the one before
     const int4 info = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z];
     const int4 more = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z + 1];
     const int first_token = info.x, pos0 = info.y, all_rows = info.z * share, longest = more.y;
-    const int kv = blockIdx.y % a.kv_heads, row0 = blockIdx.y / a.kv_heads * 8 * NT;
+    const int kv = blockIdx.y, my_span = blockIdx.x % a.n_spans, row0 = blockIdx.x / a.n_spans * 8 * NT;
     if (row0 >= all_rows || info.z > a.most_tokens) return;            // a segment of more tokens is somebody else's
     const int rows = min(8 * NT, all_rows - row0);
     const int pos_low = pos0 + row0 / share, pos_high = pos0 + (row0 + rows - 1) / share;        // of the block's rows
     const int low = a.window > 0 ? max(0, pos_low + 1 - a.window) : 0;
     const int reach = a.window > 0 ? min(longest, a.window + info.z + TILE - 1) : longest;
-    const Kv4Span span = kv4_span(blockIdx.x, a.n_spans, reach, low, pos_high + 1, TILE);
-    if ((int)blockIdx.x >= span.count) return;
-    const int* table = a.block_table + (size_t)info.w * a.table_width;
+    const Kv4Span span = kv4_span(my_span, a.n_spans, reach, low, pos_high + 1, TILE);
+    if (my_span >= span.count) return;
 
     // ---- copies: this warp's tiles are first_tile, first_tile + WARPS, ...
     const int first_tile = span.first / TILE + warp, end_tile = (span.last + TILE - 1) / TILE;
     const int tiles = end_tile > first_tile ? (end_tile - first_tile + WARPS - 1) / WARPS : 0;
-    const int page_runs = a.page_size >> 3;
+    const int page_runs = a.table.page_size >> 3;
     // the number of the run of keys of lane's (tile lane / 4 of eight, run lane % 4) among all runs of the layer, or -1
     auto runs_of = [&](int tile0) -> int {
         const int key = (first_tile + WARPS * (tile0 + (lane >> 2))) * TILE + (lane & 3) * 8;
         if (key >= span.last) return -1;
-        const int page = kv4_page(table, a.table_width, key, a.page_size, a.num_pages);
-        return page < 0 ? -1 : (page * 2 * a.kv_heads + kv) * page_runs + (key % a.page_size >> 3);
+        const int page = a.table.page(info.w, key);
+        return page < 0 ? -1 : (page * 2 * a.kv_heads + kv) * page_runs + (key % a.table.page_size >> 3);
     };
     const unsigned char* ring_at = shared + warp * STAGES * STAGE_BYTES;
     const unsigned ring = (unsigned)__cvta_generic_to_shared(ring_at) + (lane >> 3) * RUN + (lane & 7) * 16;
     int runs_now = tiles ? runs_of(0) : -1, runs_next = tiles > 8 ? runs_of(8) : -1, issued = 0;
     const size_t value_plane = (size_t)a.kv_heads * page_runs * RUN;
     const unsigned char* my_pages = a.pages + (lane & 7) * 16;
-    qil_wait_for_producer();                                 // the description and the table are older than the kernel before this one
+    qil_wait_for_producer();
     qil_release_consumer();
     auto issue = [&](int stage) {
         if (issued < tiles) {
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 *reinterpret_cast<uint2*>(a.out + ((size_t)(first_token + row / share) * a.q_heads + head) * D + d)
                     = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
             } else {
-                const size_t slot = ((size_t)(more.x + row / share) * a.q_heads + head) * a.n_spans + blockIdx.x;
+                const size_t slot = ((size_t)(more.x + row / share) * a.q_heads + head) * a.n_spans + my_span;
                 *reinterpret_cast<float4*>(a.part_o + slot * D + d) = sum;
                 if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(peak, l);
             }
@@ -621,14 +622,14 @@ template <int NT>
 static int launch(const Kv4Few& a, int n, int most_rows, cudaStream_t stream) {
     const int ring = WARPS * STAGES * STAGE_BYTES, rows = WARPS * 8 * D * 4, weights = 8 * NT * a.n_spans * 4;
     const int smem = ring > rows ? (ring > weights ? ring : weights) : (rows > weights ? rows : weights);
-    static bool configured = false;
-    if (!configured) {
+    static Kv4PerDevice configured;
+    if (!configured.here()) {
         const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory: %s", cudaGetErrorString(e));
-        configured = true;
+        configured.done();
     }
-    const dim3 grid(a.n_spans, a.kv_heads * ((most_rows + 8 * NT - 1) / (8 * NT)), n);
-    if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments, %d rows a kv head", n, most_rows);
+    const dim3 grid(a.n_spans * ((most_rows + 8 * NT - 1) / (8 * NT)), a.kv_heads, n);
+    if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments of %d kv heads", n, a.kv_heads);
     const cudaError_t e = qil_launch_chained(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, stream, a);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
@@ -644,15 +645,16 @@ extern "C" int qil_kv4_few_blocks_a_sm(int nt) { return blocks_a_sm(nt); }
 
 // info: see Kv4Few; most_tokens: segments of more are left alone; nt: 8-row tiles a block takes, 1 or 2.
 extern "C" int qil_kv4_few(const void* q, const void* pages, void* out, const void* info, int n, int most_tokens, int nt, void* part_o, void* part_ml,
-                           void* tickets, int n_spans, const void* block_table, int table_width, int q_heads, int kv_heads, int page_size, int num_pages,
-                           int window, float scale, cudaStream_t stream) {
+                           void* tickets, int n_spans, const void* block_table, int table_height, int table_width, int q_heads, int kv_heads, int page_size, int num_pages,
+                           int window, float scale, int settled, cudaStream_t stream) {
     if (n <= 0) return 0;
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n_spans < 1 || n_spans > MOST_SPANS || most_tokens < 1 || window < 0)
         QIL_REFUSE("%d query heads, %d kv heads, %d spans", q_heads, kv_heads, n_spans);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages | (uintptr_t)info | (uintptr_t)part_o) & 15) QIL_REFUSE("kv4: operands must be 16-byte aligned");
     const Kv4Few a = {(const bf16*)q, (const uint8_t*)pages, (bf16*)out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
-                      (const int*)block_table, table_width, n_spans, q_heads, kv_heads, page_size, num_pages, window, most_tokens, scale * 1.4426950408889634f};
+                      {(const int*)block_table, table_height, table_width, page_size, num_pages}, n_spans, q_heads, kv_heads, window, most_tokens, settled,
+                      scale * 1.4426950408889634f};
     const int rows = most_tokens * (q_heads / kv_heads);
     if (nt == 1) return launch<1>(a, n, rows, stream);
     if (nt == 2) return launch<2>(a, n, rows, stream);

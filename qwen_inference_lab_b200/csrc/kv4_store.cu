@@ -43,8 +43,8 @@ struct Kv4Store {
     int rot_dims, interleaved;
     const int* positions;
     const int* token_row;
-    const int* block_table;
-    int table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages;
+    Kv4Table table_of;
+    int tokens, q_heads, kv_heads, dim;
     int vectors;                    // four elements are read and written at a time: columns, strides and pointers allow it
 };
 
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
     const int pos = a.positions[token], half = a.rot_dims >> 1, groups = a.dim / KV4_GROUP;
     const Turn turn = {a.rot_dims, half, a.interleaved};
     int page = -1;
-    if (a.kv_heads) page = kv4_page(a.block_table + (size_t)a.token_row[token] * a.table_width, a.table_width, pos, a.page_size, a.num_pages);
+    if (a.kv_heads) page = a.table_of.page(a.token_row[token], pos);
     for (int d = threadIdx.x; d < 8 * LANES; d += 32 * STORE_WARPS) {
         double cosine = 1.0, sine = 0.0;
         if (d < a.rot_dims) angle_of(a, pos, turn.pair_at(d), cosine, sine);
@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
             pair = found.y;
         }
         if (mine) {
-            const int slot = pos % a.page_size;
-            uint8_t* run = a.pages + kv4_run_at(page, now - 1, head, slot, a.kv_heads, a.page_size, groups);
+            const int slot = pos % a.table_of.page_size;
+            uint8_t* run = a.pages + kv4_run_at(page, now - 1, head, slot, a.kv_heads, a.table_of.page_size, groups);
             *reinterpret_cast<unsigned*>(run + kv4_code_at(l >> 2, slot) + (l & 3) * 4) = codes;
             if ((l & 3) == 0) *reinterpret_cast<unsigned*>(run + kv4_pair_at(l >> 2, slot, groups)) = pair;
         }
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
 extern "C" int qil_kv4_store(const void* proj, long long ld, int q_col, int k_col, int v_col, void* q_out, void* pages,
                              const void* q_weight, const void* k_weight, float eps, int norm, const void* table, int table_rows,
                              const void* freq, float gain, int rot_dims, int interleaved, const void* positions, const void* token_row,
-                             const void* block_table, int table_width, int tokens, int q_heads, int kv_heads, int dim, int page_size,
-                             int num_pages, int act, int weight, cudaStream_t stream) {
+                             const void* block_table, int table_height, int table_width, int tokens, int q_heads, int kv_heads, int dim,
+                             int page_size, int num_pages, int act, int weight, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
@@ -406,8 +406,8 @@ extern "C" int qil_kv4_store(const void* proj, long long ld, int q_col, int k_co
         QIL_REFUSE("%d rotated dimensions of %d", rot_dims, dim);
     if (q_heads < 0 || kv_heads < 0 || q_heads + kv_heads == 0) QIL_REFUSE("no heads");
     Kv4Store a = {proj, ld, q_col, k_col, v_col, q_out, (uint8_t*)pages, q_weight, k_weight, eps, norm, (const float*)table, table_rows,
-                  (const float*)freq, gain, rot_dims, interleaved, (const int*)positions, (const int*)token_row, (const int*)block_table,
-                  table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages, 0};
+                  (const float*)freq, gain, rot_dims, interleaved, (const int*)positions, (const int*)token_row,
+                  {(const int*)block_table, table_height, table_width, page_size, num_pages}, tokens, q_heads, kv_heads, dim, 0};
     const int eight = act == QIL_BF16 ? 8 : 4;               // elements of 16 bytes
     a.vectors = ld % eight == 0 && q_col % eight == 0 && k_col % eight == 0 && v_col % eight == 0 && (uintptr_t)proj % 16 == 0;
     if ((uintptr_t)q_out % 16) QIL_REFUSE("queries out must start on a 16-byte boundary");
@@ -442,8 +442,8 @@ __device__ __forceinline__ void eight_values(unsigned word, unsigned pair, float
 }
 template <typename T>
 __global__ void __launch_bounds__(32 * READ_WARPS)
-kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ block_table, int table_width, const int* __restrict__ info,
-                T* __restrict__ out, int out_pages, int out_page_size, int kv_heads, int dim, int page_size, int num_pages) {
+kv4_read_kernel(const uint8_t* __restrict__ pages, const Kv4Table table, const int* __restrict__ info,
+                T* __restrict__ out, int out_pages, int out_page_size, int kv_heads, int dim) {
     qil_wait_for_producer();
     qil_release_consumer();
     const int4 mine = reinterpret_cast<const int4*>(info)[blockIdx.z];
@@ -455,15 +455,15 @@ kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ block
     if (index < 0 || index >= count) return;
     const int out_page = out_first + index / out_page_size;
     if (out_page < 0 || out_page >= out_pages) return;
-    const int page = kv4_page(block_table + (size_t)row * table_width, table_width, pos, page_size, num_pages);
+    const int page = table.page(row, pos);
     T* dst = out + ((((size_t)out_page * 2 + plane) * kv_heads + head) * out_page_size + index % out_page_size) * dim + (lane & 3) * 8;
     if (page < 0) {
         const float none[8] = {};
         for (int g = 0; g < groups; ++g) store8(dst + g * KV4_GROUP, none);
         return;
     }
-    const int slot = pos % page_size;
-    const uint8_t* run = pages + kv4_run_at(page, plane, head, slot, kv_heads, page_size, groups);
+    const int slot = pos % table.page_size;
+    const uint8_t* run = pages + kv4_run_at(page, plane, head, slot, kv_heads, table.page_size, groups);
     const uint8_t* codes = run + kv4_code_at(0, slot) + (lane & 3) * 4;
     const uint8_t* pairs = run + kv4_pair_at(0, slot, groups);
 #pragma unroll 4
@@ -474,7 +474,7 @@ kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ block
     }
 }
 
-extern "C" int qil_kv4_read(const void* pages, const void* block_table, int table_width, const void* info, int segments, int longest,
+extern "C" int qil_kv4_read(const void* pages, const void* block_table, int table_height, int table_width, const void* info, int segments, int longest,
                             void* out, int out_pages, int out_page_size, int kv_heads, int dim, int page_size, int num_pages, int act,
                             cudaStream_t stream) {
     if (segments <= 0 || longest <= 0) return 0;
@@ -483,8 +483,8 @@ extern "C" int qil_kv4_read(const void* pages, const void* block_table, int tabl
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments > 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
     const dim3 grid((longest / 8 + 2 + READ_WARPS - 1) / READ_WARPS, 2 * kv_heads, segments);          // a segment may begin and end inside a run
     QIL_DISPATCH_1(act, qil_launch_chained(kv4_read_kernel<T>, grid, dim3(32 * READ_WARPS), 0, stream, (const uint8_t*)pages,
-                                           (const int*)block_table, table_width, (const int*)info, (T*)out, out_pages, out_page_size,
-                                           kv_heads, dim, page_size, num_pages));
+                                           Kv4Table{(const int*)block_table, table_height, table_width, page_size, num_pages}, (const int*)info,
+                                           (T*)out, out_pages, out_page_size, kv_heads, dim));
     QIL_CHECK_LAUNCH();
 }
 
@@ -492,13 +492,13 @@ extern "C" int qil_kv4_read(const void* pages, const void* block_table, int tabl
 static constexpr int SPREAD_PAGE = 64;
 struct Kv4Spread {
     const uint8_t* pages;
-    const int* block_table;
+    Kv4Table table;
     const int* info;                // [segments][4]: table row, the segment's first position, its end, first page of rows
     __half* rows;                   // [page][2][kv head][64][dim]: float16 keys, then bfloat16 values
     float* key_factor;              // [page][kv head]
     int* value_marks;               // [page][kv head]
     unsigned char* marks;           // [page][kv head][64]
-    int table_width, kv_heads, dim, page_size, num_pages, window, least;
+    int kv_heads, dim, window, least;
 };
 // The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.
 __device__ __forceinline__ float bring_up(float largest, float& up) {
@@ -531,13 +531,13 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     const int slot_out = warp * 8 + (lane >> 2), pos = page0 + slot_out;
     const size_t at = (size_t)(mine.w + blockIdx.x) * a.kv_heads + head;
     __half* dst = a.rows + ((((size_t)(mine.w + blockIdx.x) * 2 + plane) * a.kv_heads + head) * SPREAD_PAGE + slot_out) * dim + (lane & 3) * 8;
-    const int page = pos < mine.z ? kv4_page(a.block_table + (size_t)mine.x * a.table_width, a.table_width, pos, a.page_size, a.num_pages) : -1;
+    const int page = pos < mine.z ? a.table.page(mine.x, pos) : -1;
     unsigned codes[GROUPS], pairs[GROUPS];
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) codes[g] = pairs[g] = 0u;
     if (page >= 0) {
-        const int slot = pos % a.page_size;
-        const uint8_t* run = a.pages + kv4_run_at(page, plane, head, slot, a.kv_heads, a.page_size, GROUPS);
+        const int slot = pos % a.table.page_size;
+        const uint8_t* run = a.pages + kv4_run_at(page, plane, head, slot, a.kv_heads, a.table.page_size, GROUPS);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
             codes[g] = *reinterpret_cast<const unsigned*>(run + kv4_code_at(g, slot) + (lane & 3) * 4);
@@ -585,15 +585,15 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     if (any && (lane & 3) == 0) a.marks[at * SPREAD_PAGE + slot_out] = (unsigned char)nan;
 }
 
-extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int table_width, const void* info, int segments, int width, void* rows,
+extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int table_height, int table_width, const void* info, int segments, int width, void* rows,
                               void* key_factor, void* value_marks, void* marks, int kv_heads, int dim, int page_size, int num_pages, int window, int least,
                               cudaStream_t stream) {
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments >= 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
-    const Kv4Spread a = {(const uint8_t*)pages, (const int*)block_table, (const int*)info, (__half*)rows, (float*)key_factor, (int*)value_marks,
-                         (unsigned char*)marks, table_width, kv_heads, dim, page_size, num_pages, window, least};
+    const Kv4Spread a = {(const uint8_t*)pages, {(const int*)block_table, table_height, table_width, page_size, num_pages}, (const int*)info,
+                         (__half*)rows, (float*)key_factor, (int*)value_marks, (unsigned char*)marks, kv_heads, dim, window, least};
     const dim3 grid(width, 2 * kv_heads, segments);
     void (*kernel)(Kv4Spread) = dim == 32 ? kv4_spread_kernel<1> : dim == 64 ? kv4_spread_kernel<2> : dim == 96 ? kv4_spread_kernel<3> : kv4_spread_kernel<4>;
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);

@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
-from types import SimpleNamespace
 
 import numpy as np
 import torch
@@ -45,11 +44,11 @@ _few_libs: dict = {}
 # The C entries' arguments: with these ctypes converts numbers itself, which takes a third of the time that an object per argument
 # does (the host's work is most of what a call on a few tokens takes).
 _P, _I, _F = c_void_p, c_int, c_float
-_STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 9 * [_I] + [_P]
-_READ = [_P, _P, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
-_SPREAD = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P] + 6 * [_I] + [_P]
-_SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
-_FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]
+_STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 10 * [_I] + [_P]
+_READ = [_P, _P, _I, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
+_SPREAD = [_P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P] + 6 * [_I] + [_P]
+_SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
+_FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
 
 
 def few_library_name(head_dim):
@@ -154,11 +153,11 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
     if min(q_at, k_at, v_at) < 0 or q_out.shape != (n, q_width) or positions.shape[0] < n or token_row.shape[0] < n \
             or max(q_at + q_width, k_at + k_width, v_at + k_width) > width:
         raise KernelError("kv4.store: shapes do not match the head counts")
-    table_width = num_pages = table_rows = 0
+    table_height = table_width = num_pages = table_rows = 0
     if n_kv_heads:
         _check_pages(pages, n_kv_heads, head_dim, page_size, "kv4.store", device)
         _take(block_table, "block_table", torch.int32, 2, device)
-        num_pages, table_width = pages.shape[0], block_table.shape[1]
+        num_pages, (table_height, table_width) = pages.shape[0], block_table.shape
     else:
         pages = block_table = None
     norm, norm_code = 0, F32
@@ -195,7 +194,7 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
     lib = library()
     _check(lib, lib.qil_kv4_store(
         proj.data_ptr(), width, q_at, k_at, v_at, q_out.data_ptr(), _at(pages), _at(q_norm_w), _at(k_norm_w), eps, norm, _at(table), table_rows,
-        _at(freq), gain, rot_dims, layout, positions.data_ptr(), token_row.data_ptr(), _at(block_table), table_width, n, n_q_heads, n_kv_heads,
+        _at(freq), gain, rot_dims, layout, positions.data_ptr(), token_row.data_ptr(), _at(block_table), table_height, table_width, n, n_q_heads, n_kv_heads,
         head_dim, page_size, num_pages, act, norm_code, _stream()), "kv4.store")
     return q_out
 
@@ -222,7 +221,7 @@ def read(pages, block_table, info, segments, longest, out, n_kv_heads, head_dim,
     if segments == 0 or longest <= 0 or out_pages * out_page_size == 0:
         return out
     lib = library()
-    _check(lib, lib.qil_kv4_read(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], info.data_ptr(), segments, longest, out.data_ptr(),
+    _check(lib, lib.qil_kv4_read(pages.data_ptr(), block_table.data_ptr(), *block_table.shape, info.data_ptr(), segments, longest, out.data_ptr(),
                                  out_pages, out_page_size, n_kv_heads, head_dim, page_size, pages.shape[0], act, _stream()), "kv4.read")
     return out
 
@@ -303,15 +302,17 @@ def refresh_single_tokens(arrays, starts) -> None:
 
 class StepPlan:
     """A step's segments on the device, as ``attend`` reads them.  ``max_context``: the longest context; of a recorded step the
-    longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest."""
+    longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest.  ``settled``: no kernel right
+    before an ``attend`` writes these arrays or the block table, so that it may read them while that one finishes."""
 
-    def __init__(self, array, count, starts, lens, max_context, min_context=0):
+    def __init__(self, array, count, starts, lens, max_context, min_context=0, settled=False):
         """``starts`` and ``lens``: the segments' on the host (numpy)."""
         self.array, self.count = array, count
         self.portion_lens = [lens[taken] for taken in portion_batches(starts, lens)]          # of the batches' segments
         self.multi_lens = lens[lens > 1]
         self.tokens = int(lens.sum())
-        self.max_context, self.min_context = int(max_context), int(min_context)
+        self.max_context, self.min_context, self.settled = int(max_context), int(min_context), int(settled)
+
     @classmethod
     def of_segments(cls, rows, starts, lens, device):
         """Of a flat batch of segments one after another: their block-table rows, the absolute position of each one's first token and
@@ -325,9 +326,9 @@ class StepPlan:
 
     @classmethod
     def of_step(cls, ctx):
-        """Of the step in flight, from the arrays that the planner made for it."""
+        """Of the step in flight, from the arrays that the planner made for it: the step's ``store`` comes after they are there."""
         view = ctx.plans[PLAN_KEY]
-        return cls(view.array, view.count, ctx.h_seg_pos0, ctx.h_seg_len, ctx.max_context, ctx.min_context)
+        return cls(view.array, view.count, ctx.h_seg_pos0, ctx.h_seg_len, ctx.max_context, ctx.min_context, settled=True)
 
 
 # ------------------------------------------------------------------ attention
@@ -367,15 +368,56 @@ def _spans(blocks_per_span, step_us, size, plan, window, most) -> int:
     return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most))
 
 
+def _capturing() -> bool:
+    return torch._C._cuda_isCurrentStreamCapturing()
+
+
+def _keep(extras, tensors) -> None:
+    """What a recorded graph points to stays for as long as ``extras`` does, whatever other calls replace there."""
+    kept = extras.setdefault("kv4_recorded", [])
+    if not any(held is tensors for held in kept):
+        kept.append(tensors)
+
+
+def _replaced(old) -> None:
+    """Memory that goes back to the stream it came from may still be in use on the current one."""
+    for tensor in old or ():
+        if tensor.is_cuda:
+            tensor.record_stream(torch.cuda.current_stream())
+
+
 def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
-    """``attention_mma.decode_scratch``, and quickly where it is there already."""
-    held = extras.get("attn_decode_scratch")
-    slots = tokens * n_q_heads * n_spans
-    if held is not None and held[0].numel() >= slots * head_dim and held[1].numel() >= 2 * slots and len(held) == 3 \
-            and held[2].numel() >= tokens * n_q_heads:
-        return held
-    return attention_mma.decode_scratch(SimpleNamespace(extras=extras, device=device), tokens, n_q_heads, n_spans, head_dim,
-                                        most=attention_f32.MOST_SCRATCH)
+    """Partial sums, their (maximum, sum) pairs and the counters of the blocks that are done, which are zero between launches.  One
+    span needs no partial sums."""
+    if n_spans == 1:
+        tokens, n_q_heads = 1, 1
+    key = ("kv4_scratch", device)
+    held, slots, heads = extras.get(key), tokens * n_q_heads * n_spans, tokens * n_q_heads
+    if held is None or held[0].numel() < slots * head_dim or held[1].numel() < 2 * slots or held[2].numel() < heads:
+        room = [2 * t.numel() for t in held] if held else [0, 0, 0]
+        new = (torch.empty(max(slots * head_dim, min(room[0], attention_f32.MOST_SCRATCH // 4)), dtype=torch.float32, device=device),
+               torch.empty(max(2 * slots, room[1]), dtype=torch.float32, device=device),
+               torch.zeros(max(heads, room[2]), dtype=torch.int32, device=device))
+        if _capturing():            # the counters are zeroed when the graph runs: no other call may count on it
+            _keep(extras, new)
+            return new
+        _replaced(held)
+        held = extras[key] = new
+    elif _capturing():
+        _keep(extras, held)
+    return held
+
+
+def _rows(extras, device, nbytes):
+    """Memory for the rows of portions."""
+    key = ("kv4_rows", device)
+    held = extras.get(key)
+    if held is None or held[0].numel() < nbytes:
+        _replaced(held)
+        held = extras[key] = (torch.empty(nbytes, dtype=torch.uint8, device=device),)
+    if _capturing():
+        _keep(extras, held)
+    return held[0]
 
 
 def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
@@ -386,21 +428,24 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
     n_spans = _spans(blocks, STEP_US[nt][:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
-    part_o, part_ml, tickets = _scratch(extras, q.device, tokens, n_q_heads, n_spans, head_dim)
+    part_o, part_ml, tickets = _scratch(extras, q.get_device(), tokens, n_q_heads, n_spans, head_dim)
     _check(lib, lib.qil_kv4_few(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, most_tokens, nt, part_o.data_ptr(),
-                                part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads,
-                                n_kv_heads, page_size, pages.shape[0], window, scale, _stream()), "kv4.attend (few tokens)")
+                                part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), *block_table.shape, n_q_heads,
+                                n_kv_heads, page_size, pages.shape[0], window, scale, plan.settled, _stream()), "kv4.attend (few tokens)")
 
 
 def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib = library()
     chunks = -(-(n_q_heads // n_kv_heads) // lib.qil_kv4_singles_heads(n_q_heads // n_kv_heads))
-    most = attention_f32.MOST_SCRATCH // (4 * n * n_q_heads * head_dim)
-    n_spans = _spans(n * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, plan, window, most)
-    part_o, part_ml, tickets = _scratch(extras, q.device, n, n_q_heads, n_spans, head_dim)
-    _check(lib, lib.qil_kv4_singles(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, part_o.data_ptr(), part_ml.data_ptr(),
-                                    tickets.data_ptr(), n_spans, block_table.data_ptr(), block_table.shape[1], n_q_heads, n_kv_heads, head_dim,
-                                    page_size, pages.shape[0], window, scale, dtype_code(q.dtype), _stream()), "kv4.attend (single tokens)")
+    for begin in range(0, n, 65535):                       # a grid's third size
+        some = min(65535, n - begin)
+        most = attention_f32.MOST_SCRATCH // (4 * some * n_q_heads * head_dim)
+        n_spans = _spans(some * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, plan, window, most)
+        part_o, part_ml, tickets = _scratch(extras, q.get_device(), some, n_q_heads, n_spans, head_dim)
+        _check(lib, lib.qil_kv4_singles(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr() + 16 * begin, some, part_o.data_ptr(),
+                                        part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), *block_table.shape, n_q_heads,
+                                        n_kv_heads, head_dim, page_size, pages.shape[0], window, scale, dtype_code(q.dtype), _stream()),
+               "kv4.attend (single tokens)")
 
 
 def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
@@ -412,10 +457,7 @@ def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_he
     if q.dtype == torch.float32:
         if not count[f"b{batch}.tiles"]:
             return
-        held = extras.get("kv4_rows")
-        if held is None or held.numel() < size:
-            held = extras["kv4_rows"] = torch.empty(size, dtype=torch.float32, device=q.device)
-        rows = held[:size].view(n_pages, 2, n_kv_heads, READ_PAGE, head_dim)
+        rows = _rows(extras, q.get_device(), 4 * size)[:4 * size].view(torch.float32).view(n_pages, 2, n_kv_heads, READ_PAGE, head_dim)
         read(pages, block_table, array[f"b{batch}.read"], segments, n_pages // segments * READ_PAGE, rows, n_kv_heads, head_dim, page_size)
         attention_f32.tiles(q, rows, out, array[f"b{batch}.tiles"], count[f"b{batch}.tiles"] // 4, table, n_q_heads, n_kv_heads, head_dim, READ_PAGE,
                             window, scale)
@@ -433,13 +475,10 @@ def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_he
     for nbytes in (2 * size, 4 * heads, 4 * heads, heads * READ_PAGE, 4 * parts * head_dim, 8 * parts):
         at.append(total)
         total += -(-nbytes // 128) * 128
-    held = extras.get("kv4_spread")
-    if held is None or held.numel() < total:
-        held = extras["kv4_spread"] = torch.empty(total, dtype=torch.uint8, device=q.device)
-    base = held.data_ptr()
+    base = _rows(extras, q.get_device(), total).data_ptr()
     rows, key_factor, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
     lib = library()
-    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], array[f"b{batch}.spread"].data_ptr(), segments, most,
+    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), *block_table.shape, array[f"b{batch}.spread"].data_ptr(), segments, most,
                                    rows, key_factor, value_marks, marks, n_kv_heads, head_dim, page_size, pages.shape[0], window, least, _stream()),
            "kv4.attend (rows of portions)")
     attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
@@ -453,7 +492,8 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
     are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Segments of up to FEW_TOKENS
     do not see positions whose page the block table does not have (a token that sees none gets zeros); longer ones need the pages of all
     that they see.  A value that is NaN reaches the tokens that see it and no others.  ``extras``: a dict that the caller keeps from call
-    to call for the scratch memory; calls that may run at the same time (other streams, recorded graphs too) need one each."""
+    to call for the scratch memory, and for as long as a graph that recorded the call; calls that may run at the same time (other
+    streams, recorded graphs too) need one each."""
     device = _device_of(q, "q")
     dtype_code(q.dtype)
     _take(q, "q", q.dtype, 2, device); _take(out, "out", q.dtype, 2, device); _take(block_table, "block_table", torch.int32, 2, device)

@@ -134,6 +134,27 @@ def test_spans_fill_the_gpu():
     assert counts == sorted(counts, reverse=True)
 
 
+def test_scratch_that_a_recorded_graph_points_to(monkeypatch):
+    """Grown scratch replaces the old one; what was handed out while a graph was recorded stays; counters that are zeroed by the graph
+    serve no other call; devices have their own."""
+    recording = [False]
+    monkeypatch.setattr(kv4, "_capturing", lambda: recording[0])
+    extras, cpu = {}, torch.device("cpu")
+    small = kv4._scratch(extras, cpu, 2, 4, 3, 32)
+    assert kv4._scratch(extras, cpu, 2, 4, 2, 32) is small and "kv4_recorded" not in extras and not small[2].any()
+    recording[0] = True
+    assert kv4._scratch(extras, cpu, 1, 4, 3, 32) is small and extras["kv4_recorded"] == [small]
+    own = kv4._scratch(extras, cpu, 20, 4, 3, 32)
+    assert own is not small and len(extras["kv4_recorded"]) == 2 and kv4._scratch(extras, cpu, 20, 4, 3, 32) is not own
+    rows = kv4._rows(extras, cpu, 100)
+    recording[0] = False
+    assert kv4._scratch(extras, cpu, 2, 4, 3, 32) is small
+    assert kv4._scratch(extras, cpu, 20, 4, 3, 32) is not own and kv4._rows(extras, cpu, 200) is not rows
+    kept = [tensor.data_ptr() for tensors in extras["kv4_recorded"] for tensor in tensors]
+    assert small[0].data_ptr() in kept and own[2].data_ptr() in kept and rows.data_ptr() in kept
+    assert kv4._scratch(extras, torch.device("meta"), 2, 4, 3, 32)[0].device.type == "meta"
+
+
 def test_a_plan_of_host_segments():
     plan = kv4.StepPlan.of_segments([2, 0], [7, 0], [1, 20], "cpu")
     assert plan.max_context == 20 and plan.tokens == 21 and len(plan.portion_lens) == 1 and plan.count["singles"] == 8
