@@ -12,6 +12,7 @@
 // one group are 128 neighbouring bytes, so 32 lanes read them in one access, from global or from shared memory.
 #pragma once
 #include "common.cuh"
+#include <string.h>
 
 #define KV4_GROUP 32
 #define KV4_MAX_DIM 256
@@ -59,6 +60,14 @@ __device__ __forceinline__ Kv4Span kv4_span(int span, int n_spans, int longest, 
     // the last span takes what is left, should a description have understated its longest context
     s.last = (span == s.count - 1 || at + length > end) ? end : (int)(at + length);
     return s;
+}
+
+// The entries take one struct each, pointers first and 32-bit numbers behind them, which the caller packs: converting thirty
+// arguments one by one takes the host 4.6 us a call, packing them 1.0.
+template <typename Call> static inline Call kv4_call(const void* packed) {
+    Call call;
+    memcpy(&call, packed, sizeof(Call));
+    return call;
 }
 
 // What has to be done once on every device: a flag for each.

@@ -222,9 +222,20 @@ static int heads_a_block(int share) { return share >= 5 ? 8 : share >= 3 ? 4 : s
 
 extern "C" int qil_kv4_singles_heads(int share) { return heads_a_block(share); }
 
-extern "C" int qil_kv4_singles(const void* q, const void* pages, void* out, const void* info, int n, void* part_o, void* part_ml, void* tickets,
-                               int n_spans, const void* block_table, int table_height, int table_width, int q_heads, int kv_heads, int dim, int page_size,
-                               int num_pages, int window, float scale, int act, cudaStream_t stream) {
+struct Kv4SinglesCall {
+    const void *q, *pages;
+    void* out;
+    const void* info;
+    void *part_o, *part_ml, *tickets;
+    const void* block_table;
+    cudaStream_t stream;
+    float scale;
+    int n, n_spans, table_height, table_width, q_heads, kv_heads, dim, page_size, num_pages, window, act;
+};
+extern "C" int qil_kv4_singles_call_bytes() { return sizeof(Kv4SinglesCall); }
+extern "C" int qil_kv4_singles(const void* packed) {
+    const auto [q, pages, out, info, part_o, part_ml, tickets, block_table, stream, scale, n, n_spans, table_height, table_width, q_heads, kv_heads, dim,
+                page_size, num_pages, window, act] = kv4_call<Kv4SinglesCall>(packed);
     if (n <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);

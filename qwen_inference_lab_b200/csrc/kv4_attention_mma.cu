@@ -644,9 +644,20 @@ extern "C" int qil_kv4_few_most_spans() { return MOST_SPANS; }
 extern "C" int qil_kv4_few_blocks_a_sm(int nt) { return blocks_a_sm(nt); }
 
 // info: see Kv4Few; most_tokens: segments of more are left alone; nt: 8-row tiles a block takes, 1 or 2.
-extern "C" int qil_kv4_few(const void* q, const void* pages, void* out, const void* info, int n, int most_tokens, int nt, void* part_o, void* part_ml,
-                           void* tickets, int n_spans, const void* block_table, int table_height, int table_width, int q_heads, int kv_heads, int page_size, int num_pages,
-                           int window, float scale, int settled, cudaStream_t stream) {
+struct Kv4FewCall {
+    const void *q, *pages;
+    void* out;
+    const void* info;
+    void *part_o, *part_ml, *tickets;
+    const void* block_table;
+    cudaStream_t stream;
+    float scale;
+    int n, most_tokens, nt, n_spans, table_height, table_width, q_heads, kv_heads, page_size, num_pages, window, settled;
+};
+extern "C" int qil_kv4_few_call_bytes() { return sizeof(Kv4FewCall); }
+extern "C" int qil_kv4_few(const void* packed) {
+    const auto [q, pages, out, info, part_o, part_ml, tickets, block_table, stream, scale, n, most_tokens, nt, n_spans, table_height, table_width,
+                q_heads, kv_heads, page_size, num_pages, window, settled] = kv4_call<Kv4FewCall>(packed);
     if (n <= 0) return 0;
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n_spans < 1 || n_spans > MOST_SPANS || most_tokens < 1 || window < 0)

@@ -393,11 +393,20 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
     }
 }
 
-extern "C" int qil_kv4_store(const void* proj, long long ld, int q_col, int k_col, int v_col, void* q_out, void* pages,
-                             const void* q_weight, const void* k_weight, float eps, int norm, const void* table, int table_rows,
-                             const void* freq, float gain, int rot_dims, int interleaved, const void* positions, const void* token_row,
-                             const void* block_table, int table_height, int table_width, int tokens, int q_heads, int kv_heads, int dim,
-                             int page_size, int num_pages, int act, int weight, cudaStream_t stream) {
+struct Kv4StoreCall {
+    const void* proj;
+    long long ld;
+    void *q_out, *pages;
+    const void *q_weight, *k_weight, *table, *freq, *positions, *token_row, *block_table;
+    cudaStream_t stream;
+    float eps, gain;
+    int q_col, k_col, v_col, norm, table_rows, rot_dims, interleaved, table_height, table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages,
+        act, weight;
+};
+extern "C" int qil_kv4_store(const void* packed) {
+    const auto [proj, ld, q_out, pages, q_weight, k_weight, table, freq, positions, token_row, block_table, stream, eps, gain, q_col, k_col, v_col,
+                norm, table_rows, rot_dims, interleaved, table_height, table_width, tokens, q_heads, kv_heads, dim, page_size, num_pages, act,
+                weight] = kv4_call<Kv4StoreCall>(packed);
     if (tokens <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
@@ -474,9 +483,15 @@ kv4_read_kernel(const uint8_t* __restrict__ pages, const Kv4Table table, const i
     }
 }
 
-extern "C" int qil_kv4_read(const void* pages, const void* block_table, int table_height, int table_width, const void* info, int segments, int longest,
-                            void* out, int out_pages, int out_page_size, int kv_heads, int dim, int page_size, int num_pages, int act,
-                            cudaStream_t stream) {
+struct Kv4ReadCall {
+    const void *pages, *block_table, *info;
+    void* out;
+    cudaStream_t stream;
+    int table_height, table_width, segments, longest, out_pages, out_page_size, kv_heads, dim, page_size, num_pages, act;
+};
+extern "C" int qil_kv4_read(const void* packed) {
+    const auto [pages, block_table, info, out, stream, table_height, table_width, segments, longest, out_pages, out_page_size, kv_heads, dim, page_size,
+                num_pages, act] = kv4_call<Kv4ReadCall>(packed);
     if (segments <= 0 || longest <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8 || out_page_size <= 0) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
@@ -585,9 +600,15 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     if (any && (lane & 3) == 0) a.marks[at * SPREAD_PAGE + slot_out] = (unsigned char)nan;
 }
 
-extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int table_height, int table_width, const void* info, int segments, int width, void* rows,
-                              void* key_factor, void* value_marks, void* marks, int kv_heads, int dim, int page_size, int num_pages, int window, int least,
-                              cudaStream_t stream) {
+struct Kv4SpreadCall {
+    const void *pages, *block_table, *info;
+    void *rows, *key_factor, *value_marks, *marks;
+    cudaStream_t stream;
+    int table_height, table_width, segments, width, kv_heads, dim, page_size, num_pages, window, least;
+};
+extern "C" int qil_kv4_spread(const void* packed) {
+    const auto [pages, block_table, info, rows, key_factor, value_marks, marks, stream, table_height, table_width, segments, width, kv_heads, dim,
+                page_size, num_pages, window, least] = kv4_call<Kv4SpreadCall>(packed);
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
@@ -599,3 +620,5 @@ extern "C" int qil_kv4_spread(const void* pages, const void* block_table, int ta
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);
     QIL_CHECK_LAUNCH();
 }
+
+extern "C" int qil_kv4_call_bytes(int which) { return which == 0 ? sizeof(Kv4StoreCall) : which == 1 ? sizeof(Kv4ReadCall) : sizeof(Kv4SpreadCall); }

@@ -14,7 +14,8 @@ package the functions launch on torch's current stream, on the current device, a
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_int
+from struct import Struct
 
 import numpy as np
 import torch
@@ -41,14 +42,16 @@ _lib = None
 _few_libs: dict = {}
 
 
-# The C entries' arguments: with these ctypes converts numbers itself, which takes a third of the time that an object per argument
-# does (the host's work is most of what a call on a few tokens takes).
-_P, _I, _F = c_void_p, c_int, c_float
-_STORE = [_P, c_longlong, _I, _I, _I, _P, _P, _P, _P, _F, _I, _P, _I, _P, _F, _I, _I, _P, _P, _P] + 10 * [_I] + [_P]
-_READ = [_P, _P, _I, _I, _P, _I, _I, _P] + 7 * [_I] + [_P]
-_SPREAD = [_P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P] + 6 * [_I] + [_P]
-_SINGLES = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
-_FEW = [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P]
+# The C entries' arguments, packed: pointers, then 32-bit numbers (the structs beside the entries), padded to whole pointers.
+_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P10i", "9Pf11i", "9Pf12i"))
+
+
+def _entry(lib, name, struct, size):
+    """A C entry that takes ``struct``."""
+    if size != struct.size:
+        raise KernelError(f"{name} takes {size} bytes of arguments, not {struct.size}")
+    entry = getattr(lib, name)
+    entry.argtypes = [c_char_p]
 
 
 def few_library_name(head_dim):
@@ -64,7 +67,7 @@ def few_library(head_dim):
         lib = build.load(name, ["kv4_attention_mma.cu"], defines, depends=DEPENDS)
         if lib.qil_kv4_few_head_dim() != head_dim:
             raise KernelError("the 4-bit attention library was built for another head size")
-        lib.qil_kv4_few.argtypes = _FEW
+        _entry(lib, "qil_kv4_few", _FEW, lib.qil_kv4_few_call_bytes())
         held = _few_libs[head_dim] = (lib, lib.qil_kv4_few_most_spans(), {nt: lib.qil_kv4_few_blocks_a_sm(c_int(nt)) for nt in (1, 2)})
     return held
 
@@ -73,18 +76,18 @@ def library():
     global _lib
     if _lib is None:
         lib = build.load("qil_kv4", SOURCES, depends=DEPENDS)
-        lib.qil_kv4_store.argtypes, lib.qil_kv4_read.argtypes, lib.qil_kv4_singles.argtypes = _STORE, _READ, _SINGLES
-        lib.qil_kv4_spread.argtypes = _SPREAD
+        for which, (name, struct) in enumerate((("qil_kv4_store", _STORE), ("qil_kv4_read", _READ), ("qil_kv4_spread", _SPREAD))):
+            _entry(lib, name, struct, lib.qil_kv4_call_bytes(which))
+        _entry(lib, "qil_kv4_singles", _SINGLES, lib.qil_kv4_singles_call_bytes())
         _lib = lib
     return _lib
 
 
 def _at(tensor):
-    return tensor.data_ptr() if tensor is not None else None
+    return tensor.data_ptr() if tensor is not None else 0
 
 
-def _stream():
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)        # of a device
 
 
 def _take(tensor, name, dtype, ndim, device):
@@ -192,10 +195,10 @@ def store(proj, columns, q_out, pages, positions, token_row, block_table, n_q_he
     if n == 0:
         return q_out
     lib = library()
-    _check(lib, lib.qil_kv4_store(
-        proj.data_ptr(), width, q_at, k_at, v_at, q_out.data_ptr(), _at(pages), _at(q_norm_w), _at(k_norm_w), eps, norm, _at(table), table_rows,
-        _at(freq), gain, rot_dims, layout, positions.data_ptr(), token_row.data_ptr(), _at(block_table), table_height, table_width, n, n_q_heads, n_kv_heads,
-        head_dim, page_size, num_pages, act, norm_code, _stream()), "kv4.store")
+    _check(lib, lib.qil_kv4_store(_STORE.pack(
+        proj.data_ptr(), width, q_out.data_ptr(), _at(pages), _at(q_norm_w), _at(k_norm_w), _at(table), _at(freq), positions.data_ptr(),
+        token_row.data_ptr(), _at(block_table), _stream(device), eps, gain, q_at, k_at, v_at, norm, table_rows, rot_dims, layout, table_height,
+        table_width, n, n_q_heads, n_kv_heads, head_dim, page_size, num_pages, act, norm_code)), "kv4.store")
     return q_out
 
 
@@ -221,8 +224,9 @@ def read(pages, block_table, info, segments, longest, out, n_kv_heads, head_dim,
     if segments == 0 or longest <= 0 or out_pages * out_page_size == 0:
         return out
     lib = library()
-    _check(lib, lib.qil_kv4_read(pages.data_ptr(), block_table.data_ptr(), *block_table.shape, info.data_ptr(), segments, longest, out.data_ptr(),
-                                 out_pages, out_page_size, n_kv_heads, head_dim, page_size, pages.shape[0], act, _stream()), "kv4.read")
+    _check(lib, lib.qil_kv4_read(_READ.pack(
+        pages.data_ptr(), block_table.data_ptr(), info.data_ptr(), out.data_ptr(), _stream(device), *block_table.shape, segments, longest, out_pages,
+        out_page_size, n_kv_heads, head_dim, page_size, pages.shape[0], act)), "kv4.read")
     return out
 
 
@@ -428,10 +432,12 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
     n_spans = _spans(blocks, STEP_US[nt][:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
-    part_o, part_ml, tickets = _scratch(extras, q.get_device(), tokens, n_q_heads, n_spans, head_dim)
-    _check(lib, lib.qil_kv4_few(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), n, most_tokens, nt, part_o.data_ptr(),
-                                part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), *block_table.shape, n_q_heads,
-                                n_kv_heads, page_size, pages.shape[0], window, scale, plan.settled, _stream()), "kv4.attend (few tokens)")
+    device = q.get_device()
+    part_o, part_ml, tickets = _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim)
+    _check(lib, lib.qil_kv4_few(_FEW.pack(
+        q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(),
+        block_table.data_ptr(), _stream(device), scale, n, most_tokens, nt, n_spans, *block_table.shape, n_q_heads, n_kv_heads, page_size,
+        pages.shape[0], window, plan.settled)), "kv4.attend (few tokens)")
 
 
 def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
@@ -441,11 +447,12 @@ def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, h
         some = min(65535, n - begin)
         most = attention_f32.MOST_SCRATCH // (4 * some * n_q_heads * head_dim)
         n_spans = _spans(some * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, plan, window, most)
-        part_o, part_ml, tickets = _scratch(extras, q.get_device(), some, n_q_heads, n_spans, head_dim)
-        _check(lib, lib.qil_kv4_singles(q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr() + 16 * begin, some, part_o.data_ptr(),
-                                        part_ml.data_ptr(), tickets.data_ptr(), n_spans, block_table.data_ptr(), *block_table.shape, n_q_heads,
-                                        n_kv_heads, head_dim, page_size, pages.shape[0], window, scale, dtype_code(q.dtype), _stream()),
-               "kv4.attend (single tokens)")
+        device = q.get_device()
+        part_o, part_ml, tickets = _scratch(extras, device, some, n_q_heads, n_spans, head_dim)
+        _check(lib, lib.qil_kv4_singles(_SINGLES.pack(
+            q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr() + 16 * begin, part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(),
+            block_table.data_ptr(), _stream(device), scale, some, n_spans, *block_table.shape, n_q_heads, n_kv_heads, head_dim, page_size,
+            pages.shape[0], window, dtype_code(q.dtype))), "kv4.attend (single tokens)")
 
 
 def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
@@ -478,9 +485,9 @@ def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_he
     base = _rows(extras, q.get_device(), total).data_ptr()
     rows, key_factor, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
     lib = library()
-    _check(lib, lib.qil_kv4_spread(pages.data_ptr(), block_table.data_ptr(), *block_table.shape, array[f"b{batch}.spread"].data_ptr(), segments, most,
-                                   rows, key_factor, value_marks, marks, n_kv_heads, head_dim, page_size, pages.shape[0], window, least, _stream()),
-           "kv4.attend (rows of portions)")
+    _check(lib, lib.qil_kv4_spread(_SPREAD.pack(
+        pages.data_ptr(), block_table.data_ptr(), array[f"b{batch}.spread"].data_ptr(), rows, key_factor, value_marks, marks, _stream(q.get_device()),
+        *block_table.shape, segments, most, n_kv_heads, head_dim, page_size, pages.shape[0], window, least)), "kv4.attend (rows of portions)")
     attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
                                 table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits)
 
