@@ -69,7 +69,8 @@ __device__ __forceinline__ unsigned pair_of(bf16 step, bf16 base) {
 }
 static constexpr unsigned NAN_PAIR = 0x7fc07fc0u;
 
-// Eight elements a lane, exact: the definition.
+// Eight elements a lane, exact: the definition.  A code is the quotient's nearest whole number without a division: a step has 8
+// bits, so the products with it are exact, and 32 bits are enough to be next to it.
 __device__ __forceinline__ void code_exact(const double (&y)[8], unsigned& codes, unsigned& pair) {
     double lo, hi;
     range_of(y, lo, hi);
@@ -83,8 +84,16 @@ __device__ __forceinline__ void code_exact(const double (&y)[8], unsigned& codes
     good = good && isfinite(m) && isfinite(s);
     codes = 0;
     if (good && s > 0.0) {
+        const double middling = s < 0x1p-64 ? 0x1p80 : s > 0x1p64 ? 0x1p-80 : 1.0;           // where steps and distances are ordinary floats
+        const float inverse = 1.f / (float)(s * middling);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) codes |= (unsigned)fmin(fmax(rint((y[i] - m) / s), 0.0), 15.0) << (4 * i);
+        for (int i = 0; i < 8; ++i) {
+            const double d = y[i] - m;
+            int n = min(max(__float2int_rn((float)(d * middling) * inverse), 0), 15);
+            const double above = fma(-((double)n + 0.5), s, d), below = fma(-((double)n - 0.5), s, d);
+            n += above > 0.0 || (above == 0.0 && (n & 1)) ? 1 : below < 0.0 || (below == 0.0 && (n & 1)) ? -1 : 0;
+            codes |= (unsigned)min(max(n, 0), 15) << (4 * i);
+        }
     }
     pair = good ? pair_of(step, base) : NAN_PAIR;
 }
@@ -217,7 +226,7 @@ __device__ __forceinline__ void angle_of(const Kv4Store& a, int pos, int pair, d
 struct EightPairs { float x[8], partner[8]; };
 // A warp's keys in 64 bits, and their codes.  Out of line: few rows come here, and its registers are twice the others'.
 template <typename W, int LANES>
-__device__ __noinline__ uint2 keys_exact(const Kv4Store* p, EightPairs e, int pos, int d0) {
+__device__ __noinline__ uint2 keys_exact(const Kv4Store* p, const double2* angles, EightPairs e, int d0) {
     const Kv4Store& a = *p;
     const Turn turn = {a.rot_dims, a.rot_dims >> 1, a.interleaved};
     const W* weight = reinterpret_cast<const W*>(a.k_weight);
@@ -225,7 +234,7 @@ __device__ __noinline__ uint2 keys_exact(const Kv4Store* p, EightPairs e, int po
     if (a.norm == 1) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq += (double)e.x[i] * (double)e.x[i];
-        r = 1.0 / sqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+        r = rsqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
         sq = 0.0;
     }
 #pragma unroll
@@ -237,15 +246,14 @@ __device__ __noinline__ uint2 keys_exact(const Kv4Store* p, EightPairs e, int po
             v = v * r * (double)to_f32<W>(weight[turn.other_of(d)]);
         }
         if (d < a.rot_dims) {
-            double c, s;
-            angle_of(a, pos, turn.pair_at(d), c, s);
-            u = turn.second(d) ? u * c + v * s : u * c - v * s;
+            const double2 at = angles[turn.pair_at(d)];
+            u = turn.second(d) ? u * at.x + v * at.y : u * at.x - v * at.y;
         }
         exact[i] = u;
         sq += u * u;
     }
     if (a.norm == 2) {
-        r = 1.0 / sqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+        r = rsqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) exact[i] *= r;
     }
@@ -269,6 +277,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
     constexpr int HEADS = 32 / LANES;
     // what an element and its partner are multiplied by: cosines times own weights, signed sines times partners', of queries and of keys
     __shared__ __align__(16) float factor[2][2][8 * LANES];
+    __shared__ double2 angles[4 * LANES];                  // cosine and sine of the pairs
     qil_wait_for_producer();
     qil_release_consumer();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, token = blockIdx.x;
@@ -278,7 +287,10 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
     if (a.kv_heads) page = a.table_of.page(a.token_row[token], pos);
     for (int d = threadIdx.x; d < 8 * LANES; d += 32 * STORE_WARPS) {
         double cosine = 1.0, sine = 0.0;
-        if (d < a.rot_dims) angle_of(a, pos, turn.pair_at(d), cosine, sine);
+        if (d < a.rot_dims) {
+            angle_of(a, pos, turn.pair_at(d), cosine, sine);
+            if (!turn.second(d)) angles[turn.pair_at(d)] = make_double2(cosine, sine);
+        }
         const float c = (float)cosine, s = turn.second(d) ? (float)sine : -(float)sine;
         const bool weighs = a.norm == 1 && d < a.dim;
         const W* q_weight = reinterpret_cast<const W*>(a.q_weight);
@@ -380,7 +392,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
                 e.x[i] = x[i];
                 e.partner[i] = now == 1 ? xp[i] : 0.f;
             }
-            const uint2 found = now == 1 ? keys_exact<W, LANES>(&a, e, pos, d0) : values_exact(e);
+            const uint2 found = now == 1 ? keys_exact<W, LANES>(&a, angles, e, d0) : values_exact(e);
             codes = found.x;
             pair = found.y;
         }
