@@ -457,7 +457,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 my_factor = my_page < 0 ? 1.f : p.key_factor[my_page];
                 if (my_page >= 0 && p.value_marks[my_page] == 0) my_page = -1;
             }
-            const float scale_later = row_scale * __shfl_sync(0xffffffffu, my_factor, j % 32);
+            float scale_later = row_scale * __shfl_sync(0xffffffffu, my_factor, j % 32);
             const int marks_at = __shfl_sync(0xffffffffu, my_page, j % 32);
             if (marks_at >= 0)
                 for (int i = 0; i < AT_N; ++i)
@@ -518,6 +518,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const float factor = (grow && j > 0) ? at_exp2(m_used - tmax) : 1.0f;
             if (grow) m_used = tmax;
             const float minus_m = (m_used == -INFINITY) ? 0.f : -m_used;
+#if QIL_KEYS_F16
+            // scores beyond 2^20: rounded together with the subtraction, the largest minus itself would be up to 2^-25 of it
+            if (__any_sync(0xffffffffu, fabsf(minus_m) > 0x1p20f)) {
+#pragma unroll
+                for (int i = 0; i < AT_N; ++i) s[i] = __fmul_rn(s[i], scale_later);
+                scale_later = 1.f;
+            }
+#endif
             // P = exp2(s * scale - m) as bfloat16, kept in registers until it is stored
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
             uint4 packed[AT_N / 8];

@@ -30,7 +30,8 @@
 // Keys that a row does not see are selected away among the scores.  Their values take part with weight zero, so groups of values that
 // are NaN are set to zero, and the rows that do see them are marked: their outputs of that group are NaN.
 //
-// Warps merge in shared memory, spans by the last block to arrive, in the order of the spans.
+// Warps merge in shared memory.  Spans merge in their order: as a cluster every block joins a part of the rows out of the shared memory of
+// all (1.1 us of 8 spans), beyond a cluster's size the last block to arrive joins what the others left in memory (3.4).
 #include "kv4.h"
 
 QIL_ERROR_STORAGE
@@ -43,8 +44,9 @@ static_assert(D % KV4_GROUP == 0 && D >= 32 && D <= KV4_MAX_DIM, "head sizes 32,
 static constexpr int G = D / KV4_GROUP, RUN = 160 * G;
 static constexpr int WARPS = 4, TILE = 32, STAGES = 2;
 static constexpr int STAGE_BYTES = 8 * RUN;            // 4 runs of keys, 4 of values
-static constexpr int MOST_SPANS = 128;
+static constexpr int MOST_SPANS = 128, MOST_CLUSTER = 16;
 static constexpr int MOST_LIFT = 90;
+static constexpr float NOTHING = -3e38f;               // the largest score of none
 
 struct Kv4Few {
     const bf16* q;                  // [tokens, q_heads * D]
@@ -56,6 +58,7 @@ struct Kv4Few {
     int* tickets;                   // [few tokens][q_heads], zero between launches
     Kv4Table table;
     int n_spans, q_heads, kv_heads, window, most_tokens;
+    int clustered;                  // the spans of a tile of rows are a cluster
     int settled;                    // info and the table are older than the kernel before this one
     float scale_log2;
 };
@@ -100,6 +103,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+// What lies at an address of this block's shared memory in another block's of the cluster.
+__device__ __forceinline__ float cluster_load(unsigned shared_addr, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(map_to_rank(shared_addr, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 cluster_load2(unsigned shared_addr, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(shared_addr, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(unsigned shared_addr, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to_rank(shared_addr, rank)) : "memory");
+    return v;
+}
 // The pairs of a row's groups.
 __device__ __forceinline__ void load_pairs(const uint8_t* at, unsigned (&w)[G]) {
     if constexpr (G % 4 == 0) {
@@ -126,6 +145,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     __shared__ float q_unit[8 * NT];                       // what a row's scores are counted in
     __shared__ float row_ml[WARPS][8 * NT][2];
     __shared__ int last_block;
+    __shared__ float2 joint_ml[8 * NT];                    // of the block's rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int share = a.q_heads / a.kv_heads;
     if (!a.settled) qil_wait_for_producer();                 // 0.9 us of a launch's 4.7 when it is chained to the one before
@@ -139,7 +159,13 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     const int low = a.window > 0 ? max(0, pos_low + 1 - a.window) : 0;
     const int reach = a.window > 0 ? min(longest, a.window + info.z + TILE - 1) : longest;
     const Kv4Span span = kv4_span(my_span, a.n_spans, reach, low, pos_high + 1, TILE);
-    if (my_span >= span.count) return;
+    if (my_span >= span.count) {
+        if (a.clustered && span.count > 1) {                 // the others meet twice
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+        return;
+    }
 
     // ---- copies: this warp's tiles are first_tile, first_tile + WARPS, ...
     const int first_tile = span.first / TILE + warp, end_tile = (span.last + TILE - 1) / TILE;
@@ -184,56 +210,70 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) issue(s);
 
-    // ---- queries: a warp a row, a lane 4 neighbouring dimensions (twice beyond 128); times 2^up the row's largest lies in [2^99, 2^100)
-    for (int of = warp; of < 8 * NT; of += WARPS) {
-        constexpr int QUADS = (D + 127) / 128;
-        const int row = row0 + of;
-        if (row >= all_rows) {                              // nobody's: zeros
-            for (int i = lane; i < 4 * G; i += 32) q_frag[(i >> 2) * NT + of / 8][(of & 7) * 4 + (i & 3)] = make_uint4(0u, 0u, 0u, 0u);
-            for (int i = lane; i < 2 * G; i += 32) q_sums[of][i] = 0u;
-            if (lane == 0) q_unit[of] = 1.f;
-            continue;
-        }
-        float q[QUADS][4], most_q = 0.f;
-        const bf16* src = a.q + ((size_t)(first_token + row / share) * a.q_heads + kv * share + row % share) * D;
+    // ---- queries: a warp a row, a lane 4 neighbouring dimensions (twice beyond 128); times 2^up the row's largest lies in [2^115, 2^116).
+    // All of a warp's rows are on their way before the first is looked at: a row takes 0.9 us by itself.
+    {
+        constexpr int QUADS = (D + 127) / 128, MINE = 2 * NT;
+        uint2 word[MINE][QUADS];
 #pragma unroll
-        for (int n = 0; n < QUADS; ++n) {
-            const int d = 4 * (lane + 32 * n);
-            const uint2 w = d < D ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0u, 0u);
-            q[n][0] = kv4_step(w.x); q[n][1] = kv4_base(w.x); q[n][2] = kv4_step(w.y); q[n][3] = kv4_base(w.y);
+        for (int j = 0; j < MINE; ++j) {
+            const int row = row0 + warp + WARPS * j;
+            const bf16* src = a.q + ((size_t)(first_token + row / share) * a.q_heads + kv * share + row % share) * D;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) most_q = fmaxf(most_q, fabsf(q[n][i]));
-        }
-        most_q = warp_max(most_q);
-        const int up = most_q > 0.f && most_q < INFINITY ? 99 - ilogbf(most_q) : 0;
-        // 2^up in two factors: it may be beyond float32.  The sums are counted like the products of codes, 2^-133.
-        const float up1 = __uint_as_float((unsigned)(127 + up / 2) << 23), up2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
-#pragma unroll
-        for (int n = 0; n < QUADS; ++n) {
-            const int d = 4 * (lane + 32 * n), g = d / KV4_GROUP;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[n][i] = q[n][i] * up1 * up2;
-            float sum = (q[n][0] + q[n][1]) + (q[n][2] + q[n][3]);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sum = sum * 0x1p-100f * 0x1p-33f;
-            if (d < D) {
-                // dimension 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one; odd ones meet
-                // codes that lie four bits higher
-                bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 1 & 3)]) + (lane & 1);
-                to[0] = __float2bfloat16_rn(q[n][0]);
-                to[2] = __float2bfloat16_rn(q[n][1] * 0.0625f);
-                to[4] = __float2bfloat16_rn(q[n][2]);
-                to[6] = __float2bfloat16_rn(q[n][3] * 0.0625f);
-                if ((lane & 7) == 0) {
-                    const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
-                    q_sums[of][2 * g] = pack_bf16(first, second);
-                    q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
-                }
+            for (int n = 0; n < QUADS; ++n) {
+                const int d = 4 * (lane + 32 * n);
+                word[j][n] = d < D && row < all_rows ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0u, 0u);        // nobody's: zeros
             }
         }
-        if (lane == 0) q_unit[of] = scalbnf(a.scale_log2, 133 - up);
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            const int of = warp + WARPS * j;
+            if (j > 0 && row0 + WARPS * j >= all_rows) {        // nobody's, all four of them
+                for (int i = lane; i < 4 * G; i += 32) q_frag[(i >> 2) * NT + of / 8][(of & 7) * 4 + (i & 3)] = make_uint4(0u, 0u, 0u, 0u);
+                for (int i = lane; i < 2 * G; i += 32) q_sums[of][i] = 0u;
+                if (lane == 0) q_unit[of] = 1.f;
+                continue;
+            }
+            float q[QUADS][4], most_q = 0.f;
+#pragma unroll
+            for (int n = 0; n < QUADS; ++n) {
+                const uint2 w = word[j][n];
+                q[n][0] = kv4_step(w.x); q[n][1] = kv4_base(w.x); q[n][2] = kv4_step(w.y); q[n][3] = kv4_base(w.y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most_q = fmaxf(most_q, fabsf(q[n][i]));
+            }
+            most_q = warp_max(most_q);
+            const int up = most_q > 0.f && most_q < INFINITY ? 115 - ilogbf(most_q) : 100;
+            // 2^up in two factors: it may be beyond float32.  The sums are counted like the products of codes, 2^-133.
+            const float up1 = __uint_as_float((unsigned)(127 + up / 2) << 23), up2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
+#pragma unroll
+            for (int n = 0; n < QUADS; ++n) {
+                const int d = 4 * (lane + 32 * n), g = d / KV4_GROUP;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[n][i] = q[n][i] * up1 * up2;
+                float sum = (q[n][0] + q[n][1]) + (q[n][2] + q[n][3]);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum = sum * 0x1p-100f * 0x1p-33f;
+                if (d < D) {
+                    // dimension 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one; odd ones meet
+                    // codes that lie four bits higher
+                    bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 1 & 3)]) + (lane & 1);
+                    to[0] = __float2bfloat16_rn(q[n][0]);
+                    to[2] = __float2bfloat16_rn(q[n][1] * 0.0625f);
+                    to[4] = __float2bfloat16_rn(q[n][2]);
+                    to[6] = __float2bfloat16_rn(q[n][3] * 0.0625f);
+                    if ((lane & 7) == 0) {
+                        const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
+                        q_sums[of][2 * g] = pack_bf16(first, second);
+                        q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+                    }
+                }
+            }
+            // of queries beyond 2^108 a score's unit would be infinite, and infinity times a score of zero
+            if (lane == 0) q_unit[of] = fminf(scalbnf(a.scale_log2, 133 - up), 3e38f);
+        }
     }
     __syncthreads();
     constexpr int SUMS = (G + 3) / 4;               // MMAs for the bases: four groups each, lane c the parts of group 4 i + c
@@ -260,8 +300,10 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p (m + 8 s)), row 8 sum(p).
     // less: -8 sum(p s) times 2^(lift - 133) with p s as the first operand: query row r, of two groups the even one in columns 0 .. 3 and
     // the odd one in 4 .. 7, keys 0 .. 7 in row r and 8 .. 15 in row 8 + r
-    float most[NT][2];                          // of rows 2 c, 2 c + 1
-    int lift = MOST_LIFT;                       // p s stays below 2^108, so that it overflows nowhere, and far above 2^7
+    // largest scores of rows 2 c, 2 c + 1, in their units: what is taken off a score is one of them, and the largest minus itself is zero
+    // however large it is
+    float most[NT][2];
+    float lift = MOST_LIFT;                       // p s stays below 2^108, so that it overflows nowhere, and far above 2^7
     unsigned lift_limit = (100 - MOST_LIFT + 128) << 7;                       // a step of that many bits or more (NaN too) asks for another lift
     unsigned marked[NT][2];                     // groups whose values are NaN for them
 #pragma unroll
@@ -276,22 +318,20 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
             for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] = 0.f;
         }
-        most[nt][0] = most[nt][1] = -INFINITY;
+        most[nt][0] = most[nt][1] = NOTHING;
         marked[nt][0] = marked[nt][1] = 0u;
     }
     const int order = (r >> 1) + (r & 1) * 4;                     // the key of 8 that row r stands for
     const unsigned half = r & 1 ? 0x7632u : 0x5410u;              // my half of a word of values, of two keys
     auto row_pos = [&](int nt, int i) { return pos0 + min(row0 + nt * 8 + 2 * c + i, all_rows - 1) / share; };
 
-    float minus[NT][2];                                           // what is added to a scaled score before the exponential
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) minus[nt][0] = minus[nt][1] = (float)MOST_LIFT;
     unsigned sink = (127 - MOST_LIFT) << 7 | (127 - MOST_LIFT) << 23;         // 2^-lift, twice
     const unsigned one = r == 0 ? 0x3f803f80u : 0u;
     const unsigned eight0 = r < 4 ? 0x80088008u : 0u, eight1 = r < 4 ? 0u : 0x80088008u;      // codes of -8
     // tiles of keys that every row sees begin in [plain_low, plain_low + plain_more]
     const int plain_low = max(span.first, a.window > 0 ? pos_high - a.window + 1 : 0);
     const int plain_more = min(pos_low - TILE + 1, span.last - TILE) - plain_low;
+    bool far = false;                           // some score is beyond 2^20
     int stage = 0;
     for (int n = 0; n < tiles; ++n) {
         if ((n & 7) == 0 && n > 0) absent = __ballot_sync(0xffffffffu, runs_now < 0);
@@ -378,9 +418,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
             }
             // the lift: by the exponent of the tile's largest step
             const int exponent = (int)(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 7) - 127;
-            if (exponent + lift > 100) {
+            if (exponent + (int)lift > 100) {
                 const int lower = 92 - exponent;
-                const float by = scalbnf(1.f, lower - lift);
+                const float by = scalbnf(1.f, lower - (int)lift);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -394,12 +434,10 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= by;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) minus[nt][i] += (float)(lower - lift);
                 }
-                lift = lower;
-                lift_limit = (unsigned)min(max(228 - lift, 0), 255) << 7;
-                sink = (unsigned)(127 - lift) << 7 | (unsigned)(127 - lift) << 23;
+                lift = (float)lower;
+                lift_limit = (unsigned)min(max(228 - lower, 0), 255) << 7;
+                sink = (unsigned)(127 - lower) << 7 | (unsigned)(127 - lower) << 23;
             }
             __syncwarp();
 #pragma unroll
@@ -422,8 +460,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                peak[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i])) * unit[nt][i];
-                grew |= peak[nt][i] > most[nt][i] + 8.f;          // the first finite one too
+                peak[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i]));
+                grew |= (peak[nt][i] - most[nt][i]) * unit[nt][i] > 8.f;          // the first finite one too
             }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -435,11 +473,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                     p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 4));
                     p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 8));
                     p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 16));
-                    const bool grow = p > most[nt][i] + 8.f;
-                    keep[i] = grow ? fast_exp2(most[nt][i] - p) : 1.f;
+                    const bool grow = (p - most[nt][i]) * unit[nt][i] > 8.f;
+                    keep[i] = grow ? fast_exp2((most[nt][i] - p) * unit[nt][i]) : 1.f;
                     if (grow) {
                         most[nt][i] = p;
-                        minus[nt][i] = (float)lift - p;
+                        far = far || fabsf(p * unit[nt][i]) > 0x1p20f;
                     }
                 }
 #pragma unroll
@@ -457,20 +495,22 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
                     for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= r & 1 ? odd : even;
             }
+            far = __any_sync(0xffffffffu, far);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float minus[2] = {fminf(fmaf(-most[nt][0], unit[nt][0], lift), 3e38f), fminf(fmaf(-most[nt][1], unit[nt][1], lift), 3e38f)};      // finite, of NOTHING too
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 float e[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[i] = fast_exp2(fmaf(sc[u][nt][i], unit[nt][i & 1], minus[nt][i & 1]));
-                }
+                for (int i = 0; i < 4; ++i)
+                    e[i] = fast_exp2(far ? fmaf(sc[u][nt][i] - most[nt][i & 1], unit[nt][i & 1], lift) : fmaf(sc[u][nt][i], unit[nt][i & 1], minus[i & 1]));
                 p0[u][nt] = transposed(pack_bf16(e[0], e[1]));
                 p1[u][nt] = transposed(pack_bf16(e[2], e[3]));
             }
-        }        // ---- output
+        }
+        // ---- output
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const unsigned char* run0 = values + 2 * u * RUN;
@@ -517,13 +557,13 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     // ---- the block's rows: [WARPS][8 rows][D] floats at a time
     const bool alone = span.count == 1;
     float* rows_o = reinterpret_cast<float*>(shared);
-    const float down = scalbnf(1.f, 33 - lift);
+    const float down = scalbnf(1.f, 33 - (int)lift);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         if (r == 0) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                row_ml[warp][nt * 8 + 2 * c + i][0] = most[nt][i];
+                row_ml[warp][nt * 8 + 2 * c + i][0] = most[nt][i] == NOTHING ? -INFINITY : most[nt][i] * unit[nt][i];
                 row_ml[warp][nt * 8 + 2 * c + i][1] = side[nt][2 + i];
             }
         }
@@ -564,6 +604,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 *reinterpret_cast<uint2*>(a.out + ((size_t)(first_token + row / share) * a.q_heads + head) * D + d)
                     = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+            } else if (a.clustered) {
+                *reinterpret_cast<float4*>(rows_o + (WARPS * 8 + nt * 8 + of) * D + d) = sum;
+                if (d == 0) joint_ml[nt * 8 + of] = make_float2(peak, l);
             } else {
                 const size_t slot = ((size_t)(more.x + row / share) * a.q_heads + head) * a.n_spans + my_span;
                 *reinterpret_cast<float4*>(a.part_o + slot * D + d) = sum;
@@ -572,6 +615,32 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         }
     }
     if (alone) return;
+    if (a.clustered) {
+        // ---- every block joins a part of the rows, out of the shared memory of all
+        cluster_sync_all();
+        const unsigned mine_o = (unsigned)__cvta_generic_to_shared(rows_o + WARPS * 8 * D), mine_ml = (unsigned)__cvta_generic_to_shared(joint_ml);
+        for (int i = my_span * 32 * WARPS + threadIdx.x; i < rows * (D / 4); i += span.count * 32 * WARPS) {
+            const int of = i / (D / 4), d = i % (D / 4) * 4, row = row0 + of, head = kv * share + row % share;
+            float peak = -INFINITY, l = 0.f;
+            for (int s = 0; s < span.count; ++s) peak = fmaxf(peak, cluster_load(mine_ml + of * 8, s));
+            const float against = peak == -INFINITY ? 0.f : peak;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int s = 0; s < span.count; ++s) {
+                const float2 ml = cluster_load2(mine_ml + of * 8, s);
+                const float4 o = cluster_load4(mine_o + (of * D + d) * 4, s);
+                const float keep = fast_exp2(ml.x - against);
+                sum.x = fmaf(o.x, keep, sum.x); sum.y = fmaf(o.y, keep, sum.y);
+                sum.z = fmaf(o.z, keep, sum.z); sum.w = fmaf(o.w, keep, sum.w);
+                l = fmaf(ml.y, keep, l);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<uint2*>(a.out + ((size_t)(first_token + row / share) * a.q_heads + head) * D + d)
+                = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+        }
+        cluster_sync_all();                  // the others' reads are done
+        return;
+    }
     // ---- the last block of these rows joins the spans
     __threadfence();
     __syncthreads();
@@ -626,11 +695,14 @@ static int launch(const Kv4Few& a, int n, int most_rows, cudaStream_t stream) {
     if (!configured.here()) {
         const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory: %s", cudaGetErrorString(e));
+        if (cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            QIL_REFUSE("kv4: no clusters of %d blocks", MOST_CLUSTER);
         configured.done();
     }
     const dim3 grid(a.n_spans * ((most_rows + 8 * NT - 1) / (8 * NT)), a.kv_heads, n);
     if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments of %d kv heads", n, a.kv_heads);
-    const cudaError_t e = qil_launch_chained(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, stream, a);
+    const cudaError_t e = a.clustered ? qil_launch_clusters(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, a.n_spans, stream, a)
+                                      : qil_launch_chained(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, stream, a);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         snprintf(qil_error_text, sizeof(qil_error_text), "%s", cudaGetErrorString(e));
@@ -652,19 +724,20 @@ struct Kv4FewCall {
     const void* block_table;
     cudaStream_t stream;
     float scale;
-    int n, most_tokens, nt, n_spans, table_height, table_width, q_heads, kv_heads, page_size, num_pages, window, settled;
+    int n, most_tokens, nt, n_spans, table_height, table_width, q_heads, kv_heads, page_size, num_pages, window, clustered, settled;
 };
 extern "C" int qil_kv4_few_call_bytes() { return sizeof(Kv4FewCall); }
 extern "C" int qil_kv4_few(const void* packed) {
     const auto [q, pages, out, info, part_o, part_ml, tickets, block_table, stream, scale, n, most_tokens, nt, n_spans, table_height, table_width,
-                q_heads, kv_heads, page_size, num_pages, window, settled] = kv4_call<Kv4FewCall>(packed);
+                q_heads, kv_heads, page_size, num_pages, window, clustered, settled] = kv4_call<Kv4FewCall>(packed);
     if (n <= 0) return 0;
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
-    if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n_spans < 1 || n_spans > MOST_SPANS || most_tokens < 1 || window < 0)
+    if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n_spans < 1 || n_spans > (clustered ? MOST_CLUSTER : MOST_SPANS) || most_tokens < 1 || window < 0)
         QIL_REFUSE("%d query heads, %d kv heads, %d spans", q_heads, kv_heads, n_spans);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)pages | (uintptr_t)info | (uintptr_t)part_o) & 15) QIL_REFUSE("kv4: operands must be 16-byte aligned");
     const Kv4Few a = {(const bf16*)q, (const uint8_t*)pages, (bf16*)out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
-                      {(const int*)block_table, table_height, table_width, page_size, num_pages}, n_spans, q_heads, kv_heads, window, most_tokens, settled,
+                      {(const int*)block_table, table_height, table_width, page_size, num_pages}, n_spans, q_heads, kv_heads, window, most_tokens, clustered,
+                      settled,
                       scale * 1.4426950408889634f};
     const int rows = most_tokens * (q_heads / kv_heads);
     if (nt == 1) return launch<1>(a, n, rows, stream);

@@ -43,7 +43,7 @@ _few_libs: dict = {}
 
 
 # The C entries' arguments, packed: pointers, then 32-bit numbers (the structs beside the entries), padded to whole pointers.
-_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P10i", "9Pf11i", "9Pf12i"))
+_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P10i", "9Pf11i", "9Pf13i"))
 
 
 def _entry(lib, name, struct, size):
@@ -340,36 +340,48 @@ class StepPlan:
 STEP = 128
 #: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 by its tiles of rows (one B200, a
 #: recorded chain of the kernel; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
-STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 3.2, 4.0, 4.6)}
+STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 2.9, 4.0, 4.6)}
 SINGLES_STEP_US = (2.0, 2.4, 3.0)
-#: ... a launch and a block's start, what the join costs at all and what every span adds.  Measured against the model (us): one request
-#: behind 8191 and 8, 16, 22, 32, 64 spans 15.1, 10.7, 13.3, 10.9, 12.9 (16.6, 12.6, 13.1, 12.3, 12.9); 8 requests and 4, 6, 8, 12 spans
-#: 32.8, 35.7, 28.6, 37.1; 48 requests and 1, 2, 3, 4 spans 157, 131, 118, 124.
+#: ... a launch and a block's start, and what a join of spans costs at all and for every span: by tiles of rows through memory, the last
+#: block to arrive, and as a cluster of blocks.  Measured (us, memory / cluster): one request of 2 tokens behind 2043 and 2, 4, 8, 16 spans 17.5 /
+#: 14.6, 14.4 / 10.5, 10.9 / 8.6, 10.6 / 8.9, of 4 tokens 26.8 / 21.2, 21.9 / 14.8, 17.2 / 12.1, 16.8 / 12.3; 8 requests of one token behind 8191
+#: and 8 spans 28.2 / 26.8.
 START_US, JOIN_US, SPAN_US = tuning.KV4_START_US, tuning.KV4_JOIN_US, tuning.KV4_SPAN_US
+JOINS_US = {1: (JOIN_US, SPAN_US), 2: (5.0, 0.2)}
+CLUSTER_SPAN_US = 0.14
+#: Spans that are a cluster where all of them run at the same time, by tiles of rows.  Clusters of other sizes are placed badly (8 requests behind 8191,
+#: 9 spans: 27.4 through memory, 37.6 as clusters; one request and 16 spans 11.3 / 12.6), and so are clusters of a second wave (16
+#: requests behind 8191 and 8 spans 51.6 / 52.8).
+CLUSTERS = {1: (2, 4, 8), 2: (2, 4, 8, 16)}
 SMS = 148
 
 
+def _clustered(n, blocks_per_span, step_us, clusters) -> bool:
+    return n in clusters and blocks_per_span * n <= SMS * len(step_us)
+
+
 @functools.lru_cache(maxsize=4096)
-def _plan(blocks_per_span, step_us, size, lo, hi, most) -> int:
+def _plan(blocks_per_span, step_us, size, lo, hi, most, join, clusters) -> int:
     """The number of spans that costs least per step of keys at both ends of [lo, hi] steps of longest context."""
     full = SMS * len(step_us)
 
     def cost(steps, n):
+        clustered = _clustered(n, blocks_per_span, step_us, clusters)
         each = -(-steps // n)
         n = -(-steps // each)                           # spans that hold anything
         waves, rest = divmod(blocks_per_span * n, full)
         time = each * size * (waves * step_us[-1] + (step_us[-(-rest // SMS) - 1] if rest else 0.0)) + START_US * (waves + (rest > 0))
-        return (time + (JOIN_US + SPAN_US * n if n > 1 else 0.0)) / steps
+        return (time + (CLUSTER_SPAN_US * n if clustered else join[0] + join[1] * n if n > 1 else 0.0)) / steps
     return min(range(1, min(hi, most) + 1), key=lambda n: cost(hi, n) + (cost(lo, min(n, lo)) if lo != hi else 0.0))
 
 
-def _spans(blocks_per_span, step_us, size, plan, window, most) -> int:
+def _spans(blocks_per_span, step_us, size, plan, window, most, join=(JOIN_US, SPAN_US), clusters=()) -> int:
     """Parts to cut the contexts into."""
     hi, lo = plan.max_context, plan.min_context or plan.max_context
     if window:
         hi, lo = min(hi, window + STEP), min(lo, window + STEP)
     hi = max(1, -(-hi // STEP))
-    return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most))
+    return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most), join, clusters)
 
 
 def _capturing() -> bool:
@@ -431,13 +443,15 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
     blocks = n * n_kv_heads * -(-rows // (8 * nt))
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
-    n_spans = _spans(blocks, STEP_US[nt][:blocks_a_sm[nt]], 0.4 + 0.15 * (head_dim // GROUP), plan, window, most)
+    step_us = STEP_US[nt][:blocks_a_sm[nt]]
+    n_spans = _spans(blocks, step_us, 0.4 + 0.15 * (head_dim // GROUP), plan, window, most, JOINS_US[nt], CLUSTERS[nt])
+    clustered = _clustered(n_spans, blocks, step_us, CLUSTERS[nt])
     device = q.get_device()
-    part_o, part_ml, tickets = _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim)
+    part_o, part_ml, tickets = _scratch(extras, device, tokens, n_q_heads, 1 if clustered else n_spans, head_dim)
     _check(lib, lib.qil_kv4_few(_FEW.pack(
         q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr(), part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(),
         block_table.data_ptr(), _stream(device), scale, n, most_tokens, nt, n_spans, *block_table.shape, n_q_heads, n_kv_heads, page_size,
-        pages.shape[0], window, plan.settled)), "kv4.attend (few tokens)")
+        pages.shape[0], window, clustered, plan.settled)), "kv4.attend (few tokens)")
 
 
 def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):

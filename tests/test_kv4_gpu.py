@@ -411,3 +411,27 @@ def test_refusals():
     refused(module.StepPlan.of_segments, [0], [3], [0], "cuda")
     refused(module.StepPlan.of_segments, [0, 1], [3], [1], "cuda")
     refused(module.StepPlan.of_segments, [0], [-1], [1], "cuda")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attend_queries_of_any_size(dtype, dim):
+    """Zero and tiny queries weigh all they see alike; one that is 10^30 times a key sees that key only.  Single tokens, a few and a portion."""
+    case = attend_case(4, 2, dim, 16, [90, 70, 40], [1, 3, 60], dtype, seed=5)
+    q, first = case["q"].view(-1, 4, dim), 0
+    q[:, 0], q[:, 1] = 0.0, 1e-30 * q[:, 1]
+    for i, n in enumerate(case["lens"]):
+        q[first:first + n, 2:] = (1e30 * case["held"][i][0][7, 1].to(q.dtype)).to(dtype)
+        first += n
+    got, first = attend_run(case).cpu().double().view(-1, 4, dim), 0
+    for i, (start, n) in enumerate(zip(case["starts"], case["lens"])):
+        values = case["held"][i][1]
+        for t in range(n):
+            seen = values[:start + t + 1, 0]
+            # p rounded (2^-8), its product with a step once more: 2^-8 of what is weighed each; the result once; float32 sums
+            bar = (3 * 2.0 ** -8 if dtype == BF16 else 2.0 ** -18) * seen.abs().amax(0)
+            assert ((got[first + t, :2] - seen.mean(0)).abs() <= bar).all()
+            one = values[7, 1]
+            bar = (4 * 2.0 ** -8 if dtype == BF16 else 2.0 ** -18) * values[:start + t + 1, 1].abs().amax()
+            assert ((got[first + t, 2:] - one).abs() <= bar).all()
+        first += n
