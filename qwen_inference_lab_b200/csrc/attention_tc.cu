@@ -649,33 +649,50 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 }
 
 #if QIL_KEYS_F16
-// out = sum over splits of O 2^(m - M) over the sum of l 2^(m - M), M their largest maximum.  A warp a row.
+// out = sum over splits of O 2^(m - M) over the sum of l 2^(m - M), M the largest maximum so far.  A warp a row; the splits' loads do not
+// wait for one another.
 __global__ void __launch_bounds__(256) at_join_kernel(AtParams p, int splits) {
+    constexpr int PER = AT_E / 32;                       // neighbouring elements a lane
     const int row = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int4 info = at_tile(p, blockIdx.y, AT_M / p.pack);             // older than the kernel that makes the rows
     qil_wait_for_producer();
-    const int4 info = at_tile(p, blockIdx.y, AT_M / p.pack);
     if (row >= info.z * p.pack) return;
     // the splits that hold anything, as the blocks counted them
     const int hi = info.y + info.z - 1;
     const int whole = hi / AT_N + 1 - (p.window > 0 ? max(0, info.y - p.window + 1) : 0) / AT_N;
     const int each = (whole + splits - 1) / splits, used = (whole + each - 1) / each;
     const size_t part = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits) * AT_M + row;
-    float most = -INFINITY, l = 0.f, o[AT_E / 32];
-    for (int z = 0; z < used; ++z) most = fmaxf(most, p.part_ml[part + (size_t)z * AT_M].x);
-    const float against = most == -INFINITY ? 0.f : most;
+    float most = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
-    for (int i = 0; i < AT_E / 32; ++i) o[i] = 0.f;
+    for (int i = 0; i < PER; ++i) o[i] = 0.f;
+#pragma unroll 4
     for (int z = 0; z < used; ++z) {
         const float2 ml = p.part_ml[part + (size_t)z * AT_M];
-        const float keep = exp2f(ml.x - against);
-        l = fmaf(ml.y, keep, l);
+        const float* from = p.part_o + (part + (size_t)z * AT_M) * AT_E + lane * PER;
+        float v[PER];
+        if constexpr (PER == 4) {
+            const float4 w = *reinterpret_cast<const float4*>(from);
+            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < AT_E / 32; ++i) o[i] = fmaf(p.part_o[(part + (size_t)z * AT_M) * AT_E + i * 32 + lane], keep, o[i]);
+            for (int i = 0; i < PER; ++i) v[i] = from[i];
+        }
+        const float larger = fmaxf(most, ml.x), against = larger == -INFINITY ? 0.f : larger;
+        const float keep = exp2f(ml.x - against), old = exp2f(most - against);
+        most = larger;
+        l = fmaf(ml.y, keep, l * old);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] = fmaf(v[i], keep, o[i] * old);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    bf16* dst = p.out + ((size_t)(info.x + row / p.pack) * p.n_q_heads + blockIdx.x * p.pack + row % p.pack) * AT_E;
+    bf16* dst = p.out + ((size_t)(info.x + row / p.pack) * p.n_q_heads + blockIdx.x * p.pack + row % p.pack) * AT_E + lane * PER;
+    if constexpr (PER == 4) {
+        const __nv_bfloat162 low = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), high = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const unsigned*>(&low), *reinterpret_cast<const unsigned*>(&high));
+    } else {
 #pragma unroll
-    for (int i = 0; i < AT_E / 32; ++i) dst[i * 32 + lane] = __float2bfloat16_rn(o[i] * inv);
+        for (int i = 0; i < PER; ++i) dst[i] = __float2bfloat16_rn(o[i] * inv);
+    }
 }
 #endif
 

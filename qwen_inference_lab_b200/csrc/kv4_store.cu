@@ -526,6 +526,7 @@ struct Kv4Spread {
     int* value_marks;               // [page][kv head]
     unsigned char* marks;           // [page][kv head][64]
     int kv_heads, dim, window, least;
+    int beside;                     // the kernel before this one attends to the same step's short segments
 };
 // The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.
 __device__ __forceinline__ float bring_up(float largest, float& up) {
@@ -547,14 +548,20 @@ __device__ __forceinline__ void store8_half(__half* p, const float (&v)[8], floa
 template <int GROUPS>
 __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Spread a) {
     __shared__ float largest_of[READ_WARPS];
-    qil_wait_for_producer();
+    // The attention to short segments writes nothing that is read or written here, and all its blocks have seen the end of what came before
+    // it when the first of this kernel's starts: so the two run side by side, and the end of this one, which the next kernel waits for, waits
+    // for that one's (12 single tokens behind 2000 to 8000 and a portion behind 6000: 108.7 -> 106.6 us, the faster join of splits in it).
+    if (!a.beside) qil_wait_for_producer();
     qil_release_consumer();
     constexpr int dim = GROUPS * KV4_GROUP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int4 mine = reinterpret_cast<const int4*>(a.info)[blockIdx.z];
     const int plane = blockIdx.y / a.kv_heads, head = blockIdx.y % a.kv_heads;
     const int page0 = blockIdx.x * SPREAD_PAGE;
-    if (mine.z - mine.y < a.least || page0 >= mine.z || (a.window > 0 && page0 + SPREAD_PAGE <= mine.y + 1 - a.window)) return;       // nobody will look
+    if (mine.z - mine.y < a.least || page0 >= mine.z || (a.window > 0 && page0 + SPREAD_PAGE <= mine.y + 1 - a.window)) {       // nobody will look
+        qil_wait_for_producer();
+        return;
+    }
     const int slot_out = warp * 8 + (lane >> 2), pos = page0 + slot_out;
     const size_t at = (size_t)(mine.w + blockIdx.x) * a.kv_heads + head;
     __half* dst = a.rows + ((((size_t)(mine.w + blockIdx.x) * 2 + plane) * a.kv_heads + head) * SPREAD_PAGE + slot_out) * dim + (lane & 3) * 8;
@@ -593,6 +600,7 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
             eight_values(codes[g], pairs[g], v);
             store8_half(dst + g * KV4_GROUP, v, up);
         }
+        qil_wait_for_producer();
         return;
     }
     unsigned nan = 0u;
@@ -610,23 +618,24 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     const int any = __syncthreads_or(nan != 0u);
     if (threadIdx.x == 0) a.value_marks[at] = any;
     if (any && (lane & 3) == 0) a.marks[at * SPREAD_PAGE + slot_out] = (unsigned char)nan;
+    qil_wait_for_producer();
 }
 
 struct Kv4SpreadCall {
     const void *pages, *block_table, *info;
     void *rows, *key_factor, *value_marks, *marks;
     cudaStream_t stream;
-    int table_height, table_width, segments, width, kv_heads, dim, page_size, num_pages, window, least;
+    int table_height, table_width, segments, width, kv_heads, dim, page_size, num_pages, window, least, beside;
 };
 extern "C" int qil_kv4_spread(const void* packed) {
     const auto [pages, block_table, info, rows, key_factor, value_marks, marks, stream, table_height, table_width, segments, width, kv_heads, dim,
-                page_size, num_pages, window, least] = kv4_call<Kv4SpreadCall>(packed);
+                page_size, num_pages, window, least, beside] = kv4_call<Kv4SpreadCall>(packed);
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments >= 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
     const Kv4Spread a = {(const uint8_t*)pages, {(const int*)block_table, table_height, table_width, page_size, num_pages}, (const int*)info,
-                         (__half*)rows, (float*)key_factor, (int*)value_marks, (unsigned char*)marks, kv_heads, dim, window, least};
+                         (__half*)rows, (float*)key_factor, (int*)value_marks, (unsigned char*)marks, kv_heads, dim, window, least, beside};
     const dim3 grid(width, 2 * kv_heads, segments);
     void (*kernel)(Kv4Spread) = dim == 32 ? kv4_spread_kernel<1> : dim == 64 ? kv4_spread_kernel<2> : dim == 96 ? kv4_spread_kernel<3> : kv4_spread_kernel<4>;
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);

@@ -43,7 +43,7 @@ _few_libs: dict = {}
 
 
 # The C entries' arguments, packed: pointers, then 32-bit numbers (the structs beside the entries), padded to whole pointers.
-_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P10i", "9Pf11i", "9Pf13i"))
+_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P11i", "9Pf11i", "9Pf13i"))
 
 
 def _entry(lib, name, struct, size):
@@ -469,8 +469,9 @@ def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, h
             pages.shape[0], window, dtype_code(q.dtype))), "kv4.attend (single tokens)")
 
 
-def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
-    """A batch of portions of at least ``least`` tokens: their contexts' rows as pages of 64 positions, then the attention over those."""
+def _portions(plan, batch, least, beside, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
+    """A batch of portions of at least ``least`` tokens: their contexts' rows as pages of 64 positions, then the attention over those.
+    ``beside``: the launch before this is ``_few``'s of the same step."""
     array, count = plan.array, plan.count
     segments, n_pages = count[f"b{batch}.read"] // 4, count[f"b{batch}.table"]
     table = array[f"b{batch}.table"][:n_pages].view(segments, n_pages // segments)
@@ -501,7 +502,7 @@ def _portions(plan, batch, least, q, pages, out, block_table, n_q_heads, n_kv_he
     lib = library()
     _check(lib, lib.qil_kv4_spread(_SPREAD.pack(
         pages.data_ptr(), block_table.data_ptr(), array[f"b{batch}.spread"].data_ptr(), rows, key_factor, value_marks, marks, _stream(q.get_device()),
-        *block_table.shape, segments, most, n_kv_heads, head_dim, page_size, pages.shape[0], window, least)), "kv4.attend (rows of portions)")
+        *block_table.shape, segments, most, n_kv_heads, head_dim, page_size, pages.shape[0], window, least, beside)), "kv4.attend (rows of portions)")
     attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
                                 table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits)
 
@@ -536,7 +537,7 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
         if count["portion_tokens"]:
             if attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads):
                 for batch in range(len(plan.portion_lens)):
-                    _portions(plan, batch, FEW_TOKENS + 1, *shape)
+                    _portions(plan, batch, FEW_TOKENS + 1, False, *shape)
             else:       # heads of a size that the tile kernel does not take: token by token
                 _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan, *shape)
         return out
@@ -552,5 +553,5 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
             _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, *shape)
         if len(few) < len(plan.multi_lens):
             for batch in range(len(plan.portion_lens)):
-                _portions(plan, batch, max(most, 1) + 1, *shape)
+                _portions(plan, batch, max(most, 1) + 1, batch == 0 and bool(count["singles"] or len(few)), *shape)
     return out
