@@ -9,8 +9,10 @@
 // 10^5 elements would land on the other side of a border.  Queries have no borders and stay in 32 bits.
 //
 // 64-bit arithmetic is what such a kernel would take its time for, and hardly any element needs it: a row is computed in 32 bits first,
-// with a bound on what that may be off (12 roundings of the two products that a turn adds), and again in 64 bits only if a step, a
-// base or a code could come out otherwise within that bound (a few rows in a hundred).  The rest is instructions: a lane takes 8
+// with a bound on what that may be off (up to 15 roundings of the two products that a turn adds), and again in 64 bits only if a step, a
+// base or a code could come out otherwise within that bound (a row or two in a hundred).  Such a row keeps its warp waiting for 3.9 us, and
+// among 64 tokens there is one nearly always: 64 tokens of 32 + 2 x 8 heads of 128 take 7.5 us, 4.1 if none had to; 2048 take 35.8 and 33.0.
+// (The same in pairs of 32-bit numbers with an exact sum and product waits 2.9: not worth a third way.)  The rest is instructions: a lane takes 8
 // neighbouring elements, so that a head of 128 is half a warp and a group's codes are one word of each of four lanes, and a token's
 // cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
 //
@@ -223,37 +225,37 @@ __device__ __forceinline__ void angle_of(const Kv4Store& a, int pos, int pair, d
         s *= (double)a.gain;
     }
 }
-struct EightPairs { float x[8], partner[8]; };
-// A warp's keys in 64 bits, and their codes.  Out of line: few rows come here, and its registers are twice the others'.
+// A warp's keys in 64 bits, and their codes.  Out of line: few rows come here, and its registers are twice the others'.  All that it needs
+// comes by value, in registers: read through a pointer to the kernel's arguments it is in no cache.
 template <typename W, int LANES>
-__device__ __noinline__ uint2 keys_exact(const Kv4Store* p, const double2* angles, EightPairs e, int d0) {
-    const Kv4Store& a = *p;
-    const Turn turn = {a.rot_dims, a.rot_dims >> 1, a.interleaved};
-    const W* weight = reinterpret_cast<const W*>(a.k_weight);
+__device__ __noinline__ uint2 keys_exact(const W* weight, const double2* angles, float eps, int norm, int dim, int rot_dims, int interleaved, int d0,
+                                         float4 x0, float4 x1, float4 v0, float4 v1) {
+    const Turn turn = {rot_dims, rot_dims >> 1, interleaved};
+    const float own[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w}, partner[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     double exact[8], r = 1.0, sq = 0.0;
-    if (a.norm == 1) {
+    if (norm == 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq += (double)e.x[i] * (double)e.x[i];
-        r = rsqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+        for (int i = 0; i < 8; ++i) sq += (double)own[i] * (double)own[i];
+        r = rsqrt(head_sum<LANES>(sq) / (double)dim + (double)eps);
         sq = 0.0;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int d = d0 + i;
-        double u = (double)e.x[i], v = (double)e.partner[i];
-        if (a.norm == 1 && d < a.dim) {
+        double u = (double)own[i], v = (double)partner[i];
+        if (norm == 1 && d < dim) {
             u = u * r * (double)to_f32<W>(weight[d]);
             v = v * r * (double)to_f32<W>(weight[turn.other_of(d)]);
         }
-        if (d < a.rot_dims) {
+        if (d < rot_dims) {
             const double2 at = angles[turn.pair_at(d)];
             u = turn.second(d) ? u * at.x + v * at.y : u * at.x - v * at.y;
         }
         exact[i] = u;
         sq += u * u;
     }
-    if (a.norm == 2) {
-        r = rsqrt(head_sum<LANES>(sq) / (double)a.dim + (double)a.eps);
+    if (norm == 2) {
+        r = rsqrt(head_sum<LANES>(sq) / (double)dim + (double)eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) exact[i] *= r;
     }
@@ -261,10 +263,8 @@ __device__ __noinline__ uint2 keys_exact(const Kv4Store* p, const double2* angle
     code_exact(exact, found.x, found.y);
     return found;
 }
-__device__ __noinline__ uint2 values_exact(EightPairs e) {
-    double exact[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) exact[i] = (double)e.x[i];
+__device__ __noinline__ uint2 values_exact(float4 x0, float4 x1) {
+    const double exact[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
     uint2 found;
     code_exact(exact, found.x, found.y);
     return found;
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
             if (a.norm) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] *= r;
-                off *= r;
+                off *= r < 1e13f ? r : INFINITY;                                             // squares of less than 1e-26 lose bits
             }
         } else {
 #pragma unroll
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
             if (mine) store8(reinterpret_cast<T*>(a.q_out) + ((size_t)token * a.q_heads + head) * a.dim + d0, y);
             continue;
         }
-        // 12 roundings of the two products; where the norm is of the turned head their errors go into its sum of squares, and so from
+        // 15 roundings of the two products; where the norm is of the turned head their errors go into its sum of squares, and so from
         // any element into any other: up to 60 roundings of the largest (one large element among 255 equal ones)
 #pragma unroll
         for (int o = 1; o < LANES; o <<= 1)
@@ -386,13 +386,11 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
         unsigned codes, pair;
         const bool sure = code_within(y, off * (a.norm == 2 ? 0x1p-18f : 0x1p-20f), codes, pair);
         if (__any_sync(0xffffffffu, mine && !sure)) {
-            EightPairs e;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e.x[i] = x[i];
-                e.partner[i] = now == 1 ? xp[i] : 0.f;
-            }
-            const uint2 found = now == 1 ? keys_exact<W, LANES>(&a, angles, e, d0) : values_exact(e);
+            const float4 x0 = make_float4(x[0], x[1], x[2], x[3]), x1 = make_float4(x[4], x[5], x[6], x[7]);
+            const uint2 found = now == 1
+                ? keys_exact<W, LANES>(reinterpret_cast<const W*>(a.k_weight), angles, a.eps, a.norm, a.dim, a.rot_dims, a.interleaved, d0, x0, x1,
+                                       make_float4(xp[0], xp[1], xp[2], xp[3]), make_float4(xp[4], xp[5], xp[6], xp[7]))
+                : values_exact(x0, x1);
             codes = found.x;
             pair = found.y;
         }
