@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
     __shared__ float largest_of[READ_WARPS];
     // The attention to short segments writes nothing that is read or written here, and all its blocks have seen the end of what came before
     // it when the first of this kernel's starts: so the two run side by side, and the end of this one, which the next kernel waits for, waits
-    // for that one's (12 single tokens behind 2000 to 8000 and a portion behind 6000: 108.7 -> 106.6 us, the faster join of splits in it).
+    // for that one's (12 single tokens behind up to 3000 and a portion of 509 behind 6001: 108.7 -> 106.6 us, the faster join of splits in it).
     if (!a.beside) qil_wait_for_producer();
     qil_release_consumer();
     constexpr int dim = GROUPS * KV4_GROUP;

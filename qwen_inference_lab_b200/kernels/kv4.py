@@ -512,8 +512,8 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
 
     q and out [N, n_q_heads * head_dim], bfloat16 or float32, the plan's tokens' rows of the flat batch; rows of other tokens are left as they
     are.  A token at position p sees the positions up to p, with ``window`` > 0 the last ``window`` of them.  Segments of up to FEW_TOKENS
-    do not see positions whose page the block table does not have (a token that sees none gets zeros); longer ones need the pages of all
-    that they see.  A value that is NaN reaches the tokens that see it and no others.  ``extras``: a dict that the caller keeps from call
+    tokens (bfloat16: of up to FEW_ROWS tokens times heads on a kv head) do not see positions whose page the block table does not have, and a
+    token that sees none gets zeros; longer ones need the pages of all that they see.  A value that is NaN reaches the tokens that see it and no others.  ``extras``: a dict that the caller keeps from call
     to call for the scratch memory, and for as long as a graph that recorded the call; calls that may run at the same time (other
     streams, recorded graphs too) need one each."""
     device = _device_of(q, "q")
@@ -528,6 +528,8 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
         raise KernelError("kv4.attend: a window cannot be negative, and a scale is a positive number")
     if plan.array["singles"].get_device() != device or q.shape[0] < plan.tokens:
         raise KernelError(f"kv4.attend: a plan of {plan.tokens} tokens on {plan.array['singles'].device} for queries {tuple(q.shape)}")
+    if window >= plan.max_context:            # everybody sees all
+        window = 0
     shape = (q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, float(scale), int(window), extras)
     count, array = plan.count, plan.array
     if q.dtype == torch.float32:

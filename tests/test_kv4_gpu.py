@@ -435,3 +435,113 @@ def test_attend_queries_of_any_size(dtype, dim):
             bar = (4 * 2.0 ** -8 if dtype == BF16 else 2.0 ** -18) * values[:start + t + 1, 1].abs().amax()
             assert ((got[first + t, 2:] - one).abs() <= bar).all()
         first += n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("case", [
+    (40, 1, 64, 16, [70, 5, 0], [1, 2, 33]),                  # more heads on a key than few tokens have rows
+    (14, 2, 160, 8, [40, 3], [1, 6]),                         # a head size that no model here has
+    (2, 2, 224, 64, [0, 65], [70, 1]),
+    (33, 3, 32, 8, [300], [12]),
+], ids=["40_1x64", "14_2x160", "2_2x224", "33_3x32"])
+def test_attend_unusual_shapes(case, dtype):
+    built = attend_case(*case, dtype, seed=11)
+    attend_check(built, attend_run(built))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_attend_nothing_and_windows_that_hide_nothing(dtype):
+    module = kv4()
+    built = attend_case(8, 2, 64, 16, [100, 20], [1, 40], dtype, seed=3)
+    open_out = attend_run(built)
+    for window in (141, 1 << 31, 1 << 40):
+        assert torch.equal(attend_run(built, window), open_out)
+    out = torch.full((3, 512), 7.0, dtype=dtype, device="cuda")
+    empty = module.StepPlan.of_segments([], [], [], "cuda")
+    module.attend(empty, torch.zeros_like(out), built["pages"].cuda(), out, built["table"].cuda(), 8, 2, 64, 16, 0.125, extras={})
+    assert (out == 7.0).all()
+
+
+def test_rows_outside_the_table_are_rows_without_pages():
+    """A plan may name a row that the table does not have: nothing is seen there, nothing is written."""
+    module = kv4()
+    built = attend_case(4, 2, 64, 16, [20], [1], BF16, seed=4)
+    plan = module.StepPlan.of_segments([7], [20], [1], "cuda")
+    assert (attend_run(built, plan=plan) == 0).all()
+    case = dict(built, q=built["q"].float(), dtype=F32)
+    assert (attend_run(case, plan=plan) == 0).all()
+    info = torch.tensor([9, 0, 16, 0], dtype=torch.int32, device="cuda")
+    back = torch.full((1, 2, 2, 16, 64), 5.0, device="cuda")
+    module.read(built["pages"].cuda(), built["table"].cuda(), info, 1, 16, back, 2, 64, 16)
+    assert (back == 0).all()
+    pages, proj = built["pages"].cuda(), torch.randn(1, 512, device="cuda")
+    one = lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    for row, position in ((9, 0), (-1, 0), (0, -1), (0, 1 << 30)):
+        module.store(proj, (0, 256, 384), torch.empty(1, 256, device="cuda"), pages, one(position), one(row), built["table"].cuda(), 4, 2, 64, 16)
+    assert torch.equal(pages.cpu(), built["pages"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_a_table_written_right_before(dtype):
+    """The block table, the queries and the scratch are the previous kernel's: a plan of the caller's is read after it."""
+    module = kv4()
+    built = attend_case(8, 2, 128, 16, [600, 33, 1], [1, 1, 4], dtype, seed=8)
+    plan = module.StepPlan.of_segments(range(3), built["starts"], built["lens"], "cuda")
+    right, q, pages = built["table"].cuda(), built["q"].cuda(), built["pages"].cuda()
+    expected, extras = attend_run(built), {}
+    table, out = torch.empty_like(right), torch.empty_like(q)
+    for _ in range(20):
+        table.fill_(-1)
+        out.fill_(math.nan)
+        torch.add(right, 0, out=table)
+        module.attend(plan, q, pages, out, table, 8, 2, 128, 16, 128 ** -0.5, extras=extras)
+        assert torch.equal(out, expected)
+
+
+def test_another_stream():
+    """Work queued on a stream of the caller's: store, attend and read there, in order."""
+    module = kv4()
+    built = attend_case(8, 2, 64, 16, [50, 9], [1, 30], BF16, seed=6)
+    expected, stream = attend_run(built), torch.cuda.Stream()
+    plan = module.StepPlan.of_segments(range(2), built["starts"], built["lens"], "cuda")
+    q, pages, table, extras = built["q"].cuda(), built["pages"].cuda(), built["table"].cuda(), {}
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        outs = []
+        for _ in range(5):
+            outs.append(torch.empty_like(q))
+            module.attend(plan, q, pages, outs[-1], table, 8, 2, 64, 16, 0.125, extras=extras)
+    other = torch.empty_like(q)
+    module.attend(plan, q, pages, other, table, 8, 2, 64, 16, 0.125, extras={})            # beside it, scratch of its own
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, expected) for out in (*outs, other))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("clusters", [True, False], ids=["clusters", "memory"])
+def test_two_graphs_and_a_call_share_scratch(dtype, clusters, monkeypatch):
+    """Recorded before any other call with the dict, replayed one after another in any order, calls in between, after larger ones replaced
+    the scratch."""
+    module = kv4()
+    if not clusters:
+        monkeypatch.setattr(module, "CLUSTERS", {1: (), 2: ()})
+    built = attend_case(8, 2, 64, 16, [2000, 700], [1, 1], dtype, seed=9)
+    large = attend_case(8, 2, 64, 16, [900] * 9 + [10], [1] * 9 + [90], dtype, seed=10)
+    expected, expected_large = attend_run(built), attend_run(large)
+    plan = module.StepPlan.of_segments(range(2), built["starts"], built["lens"], "cuda")
+    q, pages, table, extras, graphs = built["q"].cuda(), built["pages"].cuda(), built["table"].cuda(), {}, []
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                module.attend(plan, q, pages, out, table, 8, 2, 64, 16, 0.125, extras=extras)
+            graphs.append((graph, out))
+        for turn, which in enumerate((1, 0, 1, 1, 0, 0)):
+            if turn in (1, 3):
+                assert torch.equal(attend_run(large, extras=extras), expected_large)
+            assert torch.equal(attend_run(built, extras=extras), expected)
+            graph, out = graphs[which]
+            out.fill_(math.nan)
+            graph.replay()
+            assert torch.equal(out, expected)
