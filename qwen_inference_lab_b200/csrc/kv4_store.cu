@@ -11,7 +11,7 @@
 // 64-bit arithmetic is what such a kernel would take its time for, and hardly any element needs it: a row is computed in 32 bits first,
 // with a bound on what that may be off (up to 15 roundings of the two products that a turn adds), and again in 64 bits only if a step, a
 // base or a code could come out otherwise within that bound (a row or two in a hundred).  Such a row keeps its warp waiting for 3.9 us, and
-// among 64 tokens there is one nearly always: 64 tokens of 32 + 2 x 8 heads of 128 take 7.5 us, 4.1 if none had to; 2048 take 35.8 and 33.0.
+// among 64 tokens there is one nearly always: 64 tokens of 32 + 2 x 8 heads of 128 take 7.0 us, 3.8 if none had to; 2048 take 30.4 and 26.9.
 // (The same in pairs of 32-bit numbers with an exact sum and product waits 2.9: not worth a third way.)  The rest is instructions: a lane takes 8
 // neighbouring elements, so that a head of 128 is half a warp and a group's codes are one word of each of four lanes, and a token's
 // cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
@@ -26,7 +26,9 @@
 
 QIL_ERROR_STORAGE
 
-static constexpr int STORE_WARPS = 8;
+// Warps a block, blocks an SM.  Measured (us, 64 / 256 / 2048 tokens): 8 x 4 7.5 / 10.2 / 34.0, 8 x 3 6.5 / 9.2 / 35.8, 4 x 6 6.5 / 8.5 / 33.8, 4 x 7 7.0 /
+// 9.1 / 30.5, 4 x 8 7.4 / 10.3 / 30.6, 2 x 14 7.4 / 9.8 / 29.7.
+static constexpr int STORE_WARPS = 4, STORE_BLOCKS = 7;
 
 struct Kv4Store {
     const void* proj;               // T [tokens, ld]; q, k, v from their columns on
@@ -270,10 +272,10 @@ __device__ __noinline__ uint2 values_exact(float4 x0, float4 x1) {
     return found;
 }
 
-// A block: a token and every (gridDim.y)th set of STORE_WARPS steps; a warp takes 32 / LANES heads of one kind a step, LANES lanes of 8
+// A block: a token and every (gridDim.y)th set of STORE_WARPS steps, from the last on; a warp takes 32 / LANES heads of one kind a step, LANES lanes of 8
 // elements each (the first dim / 8 of them; a power of two).
 template <typename T, typename W, int LANES>
-__global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __grid_constant__ Kv4Store a) {
+__global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kernel(const __grid_constant__ Kv4Store a) {
     constexpr int HEADS = 32 / LANES;
     // what an element and its partner are multiplied by: cosines times own weights, signed sines times partners', of queries and of keys
     __shared__ __align__(16) float factor[2][2][8 * LANES];
@@ -308,12 +310,12 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, 4) kv4_store_kernel(const __
     const int other_lane = lane + (d0 >= a.rot_dims ? 0 : d0 < half ? half / 8 : -(half / 8));
     float cw[8], sw[8];
     int kind = -1;
-    // neighbouring steps for a warp: they are mostly of one kind
-    const int steps = steps_q + 2 * steps_kv, each = (steps + gridDim.y * STORE_WARPS - 1) / (gridDim.y * STORE_WARPS);
-    const int begin = (blockIdx.y * STORE_WARPS + warp) * each;
-    for (int step = begin; step < min(begin + each, steps); ++step) {
+    // every warp takes values or keys, which take longest, and then queries (2048 tokens 34.0 us, a warp's steps side by side 35.8)
+    const int steps = steps_q + 2 * steps_kv;
+    for (int back = blockIdx.y * STORE_WARPS + warp; back < steps; back += gridDim.y * STORE_WARPS) {
+        const int step = steps - 1 - back;
         const int now = step < steps_q ? 0 : step < steps_q + steps_kv ? 1 : 2;              // queries, keys, values
-        if (now > 0 && page < 0) break;
+        if (now > 0 && page < 0) continue;
         const int head = (step - (now == 0 ? 0 : now == 1 ? steps_q : steps_q + steps_kv)) * HEADS + sub;
         const bool mine = head < (now == 0 ? a.q_heads : a.kv_heads) && d0 < a.dim;
         const T* src = reinterpret_cast<const T*>(a.proj) + (size_t)token * a.ld + (now == 0 ? a.q_col : now == 1 ? a.k_col : a.v_col) + (size_t)head * a.dim;
@@ -432,8 +434,9 @@ extern "C" int qil_kv4_store(const void* packed) {
     if ((uintptr_t)q_out % 16) QIL_REFUSE("queries out must start on a 16-byte boundary");
     const int lanes = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32, heads = 32 / lanes;
     const int steps = (q_heads + heads - 1) / heads + 2 * ((kv_heads + heads - 1) / heads), sets = (steps + STORE_WARPS - 1) / STORE_WARPS;
-    // a step a warp while that does not fill the GPU (148 SMs of 3 blocks), else all of a token's in one block: its angles are made once
-    const dim3 grid(tokens, tokens * sets <= 444 ? sets : 1);
+    // as many blocks a token as fill the GPU once, a step a warp at most
+    const int fit = 148 * STORE_BLOCKS / tokens;              // 148 SMs
+    const dim3 grid(tokens, fit < 1 ? 1 : fit < sets ? fit : sets);
 #define KV4_STORE(L)                                                                                                       \
     if (lanes == L) QIL_DISPATCH_2(act, weight, qil_launch_chained(kv4_store_kernel<T, W, L>, grid, dim3(32 * STORE_WARPS), 0, stream, a))
     KV4_STORE(4);
