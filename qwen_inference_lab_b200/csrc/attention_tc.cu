@@ -19,11 +19,12 @@
 //               and the rescale of O in tensor memory when the running maximum moved by more than
 //               2^8 (until then P is computed against the older maximum, which is exact algebra and
 //               safe in float32), in tiles of fewer tokens whenever it moved; finally O / l -> global memory.
-// With -DQIL_KEYS_F16=1 keys are float16, each page of them with a power of two taken out, which the softmax multiplies back (pages of 64:
-// a tile's scores have one factor); the softmax warps make float16 of the queries' rows where they lie, each with a power of two of its own;
-// values, P and the output are bfloat16 as ever.  Rows that were
+// With -DQIL_KEYS_F16=1 keys and values are float16, each page of them with a power of two taken out, which the softmax multiplies back (pages of
+// 64: a tile's scores have one factor, its weights another); the softmax warps make float16 of the queries' rows where they lie, each with a power
+// of two of its own; P is float16, the output bfloat16 as ever.  Rows that were
 // held in fewer bits and are read back for this kernel have more than bfloat16's 8: as bfloat16 keys they are off by 2^-9, which
-// scores of some size turn into a weight's error several times that of its own rounding.  Value groups that are NaN come as zeros and
+// scores of some size turn into a weight's error several times that of its own rounding, and with values and P as bfloat16 the
+// result was off by 2.6e-3 where its own rounding is 1.65e-3.  Value groups that are NaN come as zeros and
 // marks: a row that sees a mark gets NaN there, one that masks it does not.  In this form a block's 128 rows are `pack` query heads of one kv
 // head times 128 / pack tokens (a short portion fills a tile, and a tile of fewer tokens masks less), and where the blocks would not fill
 // the GPU a context is cut over several blocks (`splits`), whose unnormed outputs a second kernel joins.
@@ -60,6 +61,7 @@ static_assert(AT_D % 16 == 0 && AT_D >= 16 && AT_D <= 128 && AT_E % 16 == 0 && A
 #define AT_VTILE (AT_ES * AT_SLAB)    // a V tile
 #define AT_TMEM_COLS (AT_N == 64 ? 256 : 512)
 #define AT_STAGES 2
+#define AT_LIFT 5                       // float16 weights: 2^5 of what bfloat16 ones are (2^13 at most), so that small ones keep their bits
 #ifndef QIL_KEYS_F16
 #define QIL_KEYS_F16 0
 #endif
@@ -163,14 +165,14 @@ struct AtParams {
     int* error_word;
     long long* trace;           // only read when compiled with AT_TRACE
 #if QIL_KEYS_F16
-    const float* key_factor;            // [page][kv head]: what a page's float16 keys are
+    const float* factors;               // [page][2][kv head]: what a page's keys and values are to be multiplied by, powers of two
     const int* value_marks;             // [page][kv head]: does any value group of the page have a mark?
     const unsigned char* marks;         // [page][kv head][64]: bit g: group g of 32 columns of that position's value is NaN
     const int4* segments;               // (first token, its position, tokens, block-table row) each, the longest contexts first
     int n_segments, pack;
     int least;                          // segments of fewer tokens are left alone
-    float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum)
-    float2* part_ml;
+    float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum, largest power of their values)
+    float4* part_ml;
 #endif
 };
 
@@ -187,6 +189,17 @@ __device__ __forceinline__ int4 at_tile(const AtParams& p, int index, int tokens
         index -= tiles;
     }
     return make_int4(0, 0, 0, 0);       // never: the grid is as large as the tiles are many
+}
+__device__ __forceinline__ int at_exponent(float power) { return (__float_as_int(power) >> 23) - 127; }
+// The largest power of two taken out of the values of a head's pages [first, last] of a table row, in all lanes of a warp.
+__device__ __forceinline__ int at_value_top(const AtParams& p, const int* table, int first, int last, int kv_head) {
+    int top = -127;
+#pragma unroll 4
+    for (int i = first + (int)(threadIdx.x & 31); i <= min(last, p.table_stride - 1); i += 32) {
+        const int page = table[i];
+        if (page >= 0) top = max(top, at_exponent(p.factors[((size_t)page * 2 + 1) * p.n_kv_heads + kv_head]));
+    }
+    return __reduce_max_sync(0xffffffffu, top);
 }
 #endif
 
@@ -341,7 +354,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         // bfloat16 -> float32, M = 128; scores: N = keys; output: N = the value slabs' columns, B (V) read MN-major
         const bool leader = elect_one();
         const unsigned idesc_s = umma_idesc(AT_M, AT_N) & (QIL_KEYS_F16 ? ~((1u << 7) | (1u << 10)) : ~0u);      // float16 operands: zeros there
-        const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AT_ES * 64 >> 3) << 17) | ((unsigned)(AT_M >> 4) << 24);
+        const unsigned idesc_pv = (1u << 4) | (QIL_KEYS_F16 ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) | ((unsigned)(AT_ES * 64 >> 3) << 17) | ((unsigned)(AT_M >> 4) << 24);
 #if QIL_KEYS_F16
         bool ok = warp_mbar_wait(&sh->q_ready, 0);
 #else
@@ -400,6 +413,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const bool biased = p.slopes_log2 != nullptr;
         const float slope = biased ? p.slopes_log2[head] : 0.f;
 #if QIL_KEYS_F16
+        // The rows' weights carry their page's power of two, less the largest: what they weigh is float16 of one scale.  m_used counts it: the
+        // largest of score + power.  (Looked up while the queries are on their way.)
+        const int value_top = at_value_top(p, table, whole0, hi / AT_N, kv_head);
+        float my_shift = 0.f, m_score = 0.f, m_shift = 0.f;
         // this thread's row, 16 bytes at a time, neighbouring rows at different places of their 128 bytes (which element lies where
         // does not matter): its largest into [256, 512)
         if (!warp_mbar_wait(&sh->q_full, 0)) { if (lane == 0) atomicExch(p.error_word, 25); }
@@ -454,11 +471,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const int index = tile0 + j + lane;
                 const int page = (index <= hi / AT_N && index < p.table_stride) ? table[index] : -1;
                 my_page = page < 0 ? -1 : page * p.n_kv_heads + kv_head;
-                my_factor = my_page < 0 ? 1.f : p.key_factor[my_page];
+                my_factor = page < 0 ? 1.f : p.factors[(size_t)page * 2 * p.n_kv_heads + kv_head];
+                // beyond 2^90 below the largest a page's values weigh too much (2^-81 of the largest at most)
+                my_shift = page < 0 ? 0.f : (float)max(at_exponent(p.factors[((size_t)page * 2 + 1) * p.n_kv_heads + kv_head]) - value_top, -90);
                 if (my_page >= 0 && p.value_marks[my_page] == 0) my_page = -1;
             }
             float scale_later = row_scale * __shfl_sync(0xffffffffu, my_factor, j % 32);
             const int marks_at = __shfl_sync(0xffffffffu, my_page, j % 32);
+            const float shift = __shfl_sync(0xffffffffu, my_shift, j % 32);
             if (marks_at >= 0)
                 for (int i = 0; i < AT_N; ++i)
                     if ((tile0 + j) * AT_N + i <= pos && (tile0 + j) * AT_N + i >= lo) marked |= p.marks[(size_t)marks_at * AT_N + i];
@@ -514,17 +534,29 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_later;
             // Move the maximum only when it grew by more than 2^8 (`slack`): until then exp2(s - m_used) <= 256,
             // harmless in float32 and bfloat16, and O needs no rescale (which costs a TMEM round trip).
+#if QIL_KEYS_F16
+            const float t = tmax + shift;
+            const bool grow = t > m_used + slack;
+            const float factor = (grow && j > 0) ? at_exp2(m_used - t) : 1.0f;
+            if (grow) {
+                m_used = t;
+                m_score = tmax;
+                m_shift = shift;
+            }
+            float minus_m = (m_used == -INFINITY) ? 0.f : (shift + (float)AT_LIFT) - m_used;
+            // scores beyond 2^20: rounded together with the subtraction, the largest minus itself would be up to 2^-25 of it
+            if (__any_sync(0xffffffffu, fabsf(minus_m) > 0x1p20f)) {
+                const float less = (m_used == -INFINITY) ? 0.f : m_score;
+#pragma unroll
+                for (int i = 0; i < AT_N; ++i) s[i] = __fadd_rn(__fmul_rn(s[i], scale_later), -less);
+                scale_later = 1.f;
+                minus_m = shift - m_shift + (float)AT_LIFT;
+            }
+#else
             const bool grow = tmax > m_used + slack;           // also true at the first tile (m_used = -inf)
             const float factor = (grow && j > 0) ? at_exp2(m_used - tmax) : 1.0f;
             if (grow) m_used = tmax;
             const float minus_m = (m_used == -INFINITY) ? 0.f : -m_used;
-#if QIL_KEYS_F16
-            // scores beyond 2^20: rounded together with the subtraction, the largest minus itself would be up to 2^-25 of it
-            if (__any_sync(0xffffffffu, fabsf(minus_m) > 0x1p20f)) {
-#pragma unroll
-                for (int i = 0; i < AT_N; ++i) s[i] = __fmul_rn(s[i], scale_later);
-                scale_later = 1.f;
-            }
 #endif
             // P = exp2(s * scale - m) as bfloat16, kept in registers until it is stored
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
@@ -537,12 +569,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     e[i] = at_exp2(fmaf(s[c * 8 + i], scale_later, minus_m));
                     sums[i & 3] += e[i];
                 }
+#if QIL_KEYS_F16
+                __half2 b0 = __floats2half2_rn(e[0], e[1]), b1 = __floats2half2_rn(e[2], e[3]);
+                __half2 b2 = __floats2half2_rn(e[4], e[5]), b3 = __floats2half2_rn(e[6], e[7]);
+#else
                 __nv_bfloat162 b0 = __floats2bfloat162_rn(e[0], e[1]), b1 = __floats2bfloat162_rn(e[2], e[3]);
                 __nv_bfloat162 b2 = __floats2bfloat162_rn(e[4], e[5]), b3 = __floats2bfloat162_rn(e[6], e[7]);
+#endif
                 packed[c].x = *reinterpret_cast<unsigned*>(&b0); packed[c].y = *reinterpret_cast<unsigned*>(&b1);
                 packed[c].z = *reinterpret_cast<unsigned*>(&b2); packed[c].w = *reinterpret_cast<unsigned*>(&b3);
             }
+#if QIL_KEYS_F16
+            const float sum = ((sums[0] + sums[1]) + (sums[2] + sums[3])) * at_exp2(-shift);       // without the page's power
+#else
             const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+#endif
             if (warp == 2 && lane == 0) AT_STAMP(2, 6 * j + 3);
             const bool rescale = __any_sync(0xffffffffu, factor != 1.0f);
             if (rescale || (j > 0 && j == n_tiles - 1)) {
@@ -606,8 +647,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const float inv = l > 0.f ? 1.f / l : 0.f;
             bf16* dst = p.out + ((size_t)(n0 + row / pack) * p.n_q_heads + head + row % pack) * AT_E;
 #if QIL_KEYS_F16
+            const float value_scale = __int_as_float(max(value_top + 127, 1) << 23);
             const size_t part = ((((size_t)blockIdx.y * gridDim.x + blockIdx.x) * gridDim.z + blockIdx.z) * AT_M + row);
-            if (gridDim.z > 1) p.part_ml[part] = make_float2(m_used, l);
+            if (gridDim.z > 1) p.part_ml[part] = make_float4(m_used, l, value_scale, 0.f);
 #endif
 #pragma unroll 1
             for (int c = 0; c < (AT_E + 31) / 32; ++c) {
@@ -630,8 +672,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     if (AT_E % 32 != 0 && c * 32 + q * 8 >= AT_E) break;
                     uint4 packed;
                     bf16* o = reinterpret_cast<bf16*>(&packed);
+#if QIL_KEYS_F16
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(__uint_as_float(r[q * 8 + i]) * inv * value_scale);
+#else
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(__uint_as_float(r[q * 8 + i]) * inv);
+#endif
 #if QIL_KEYS_F16
                     if (marked >> c & 1u) packed = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
 #endif
@@ -662,12 +709,13 @@ __global__ void __launch_bounds__(256) at_join_kernel(AtParams p, int splits) {
     const int whole = hi / AT_N + 1 - (p.window > 0 ? max(0, info.y - p.window + 1) : 0) / AT_N;
     const int each = (whole + splits - 1) / splits, used = (whole + each - 1) / each;
     const size_t part = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits) * AT_M + row;
-    float most = -INFINITY, l = 0.f, o[PER];
+    float most = -INFINITY, l = 0.f, value_scale = 0.f, o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) o[i] = 0.f;
 #pragma unroll 4
     for (int z = 0; z < used; ++z) {
-        const float2 ml = p.part_ml[part + (size_t)z * AT_M];
+        const float4 ml = p.part_ml[part + (size_t)z * AT_M];
+        value_scale = ml.z;                              // the same of all splits
         const float* from = p.part_o + (part + (size_t)z * AT_M) * AT_E + lane * PER;
         float v[PER];
         if constexpr (PER == 4) {
@@ -687,11 +735,12 @@ __global__ void __launch_bounds__(256) at_join_kernel(AtParams p, int splits) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bf16* dst = p.out + ((size_t)(info.x + row / p.pack) * p.n_q_heads + blockIdx.x * p.pack + row % p.pack) * AT_E + lane * PER;
     if constexpr (PER == 4) {
-        const __nv_bfloat162 low = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), high = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
+        const __nv_bfloat162 low = __floats2bfloat162_rn(o[0] * inv * value_scale, o[1] * inv * value_scale),
+                             high = __floats2bfloat162_rn(o[2] * inv * value_scale, o[3] * inv * value_scale);
         *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const unsigned*>(&low), *reinterpret_cast<const unsigned*>(&high));
     } else {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) dst[i] = __float2bfloat16_rn(o[i] * inv);
+        for (int i = 0; i < PER; ++i) dst[i] = __float2bfloat16_rn(o[i] * inv * value_scale);
     }
 }
 #endif
@@ -817,16 +866,16 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
 // least `least` tokens, 128 / pack tokens each; splits > 1: part_o float32 [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml as many pairs of rows.
 extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* segments, int n_segments, int least, int n_tiles, int n_tokens,
                                           const int* block_table, int table_stride, int n_q_heads, int n_kv_heads, int num_pages, float scale,
-                                          int window, int pack, int splits, const float* key_factor, const int* value_marks,
+                                          int window, int pack, int splits, const float* factors, const int* value_marks,
                                           const unsigned char* marks, float* part_o, float* part_ml, int* error_word, cudaStream_t stream) {
-    if (key_factor == nullptr || value_marks == nullptr || marks == nullptr) QIL_REFUSE("attn_tc: float16 keys come with factors and marks");
+    if (factors == nullptr || value_marks == nullptr || marks == nullptr) QIL_REFUSE("attn_tc: float16 keys come with factors and marks");
     if (n_kv_heads <= 0 || pack <= 0 || AT_M % pack || (n_q_heads / n_kv_heads) % pack || splits < 1 || splits > 65535
         || (splits > 1 && (part_o == nullptr || part_ml == nullptr)))
         QIL_REFUSE("attn_tc: %d heads of %d over %d a tile, %d splits", pack, n_q_heads, n_kv_heads, splits);
     AtParams p = {};
-    p.key_factor = key_factor; p.value_marks = value_marks; p.marks = marks;
+    p.factors = factors; p.value_marks = value_marks; p.marks = marks;
     p.segments = (const int4*)segments; p.n_segments = n_segments; p.least = least; p.pack = pack;
-    p.part_o = part_o; p.part_ml = (float2*)part_ml;
+    p.part_o = part_o; p.part_ml = (float4*)part_ml;
     return at_launch(q, kv, out, segments, n_tiles, n_tokens, block_table, table_stride, n_q_heads, n_kv_heads, AT_N, num_pages, scale,
                      nullptr, 0, nullptr, 0.f, window, error_word, nullptr, p, splits, stream);
 }

@@ -17,8 +17,7 @@
 // cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
 //
 // kv4_spread: the rows of a prompt portion's context for the kernel that attends to 16-bit operands (attention_tc.cu with float16 keys):
-// keys as float16 with a power of two taken out per page of 64 and head, values as bfloat16; where a group of values is NaN, zeros and
-// a mark.
+// float16 keys and values with a power of two taken out of each per page of 64 and head; where a group of values is NaN, zeros and a mark.
 //
 // kv4_read: rows of requests as ordinary pages [page][2][kv head][slot][d] of float32 or bfloat16.
 #include "kv4.h"
@@ -522,8 +521,8 @@ struct Kv4Spread {
     const uint8_t* pages;
     Kv4Table table;
     const int* info;                // [segments][4]: table row, the segment's first position, its end, first page of rows
-    __half* rows;                   // [page][2][kv head][64][dim]: float16 keys, then bfloat16 values
-    float* key_factor;              // [page][kv head]
+    __half* rows;                   // [page][2][kv head][64][dim]: keys, then values
+    float* factors;                 // [page][2][kv head]: what the page's rows are to be multiplied by
     int* value_marks;               // [page][kv head]
     unsigned char* marks;           // [page][kv head][64]
     int kv_heads, dim, window, least;
@@ -579,64 +578,55 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
             pairs[g] = *reinterpret_cast<const unsigned*>(run + kv4_pair_at(g, slot, GROUPS));
         }
     }
-    if (plane == 0) {
-        float largest = 0.f;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            const float s = kv4_step(pairs[g]), m = kv4_base(pairs[g]);
-            largest = fmaxf(largest, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));            // NaN is left out
-        }
-        largest = warp_max(largest);
-        if (lane == 0) largest_of[warp] = largest;
-        __syncthreads();
-        largest = largest_of[0];
-#pragma unroll
-        for (int w = 1; w < READ_WARPS; ++w) largest = fmaxf(largest, largest_of[w]);
-        float up;
-        const float factor = bring_up(largest, up);
-        if (threadIdx.x == 0) a.key_factor[at] = factor;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            float v[8];
-            eight_values(codes[g], pairs[g], v);
-            store8_half(dst + g * KV4_GROUP, v, up);
-        }
-        qil_wait_for_producer();
-        return;
-    }
     unsigned nan = 0u;
+    float largest = 0.f;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-        const float s = kv4_step(pairs[g]);
-        if (!(s == s)) {
+        const float s = kv4_step(pairs[g]), m = kv4_base(pairs[g]);
+        if (plane == 1 && !(s == s)) {
             nan |= 1u << g;
             pairs[g] = 0u;
+        } else {
+            largest = fmaxf(largest, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));            // NaN is left out
         }
+    }
+    largest = warp_max(largest);
+    if (lane == 0) largest_of[warp] = largest;
+    const int any = __syncthreads_or(nan != 0u);
+    largest = largest_of[0];
+#pragma unroll
+    for (int w = 1; w < READ_WARPS; ++w) largest = fmaxf(largest, largest_of[w]);
+    float up;
+    const float factor = bring_up(largest, up);
+    if (threadIdx.x == 0) a.factors[((size_t)(mine.w + blockIdx.x) * 2 + plane) * a.kv_heads + head] = factor;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
         float v[8];
         eight_values(codes[g], pairs[g], v);
-        store8(reinterpret_cast<bf16*>(dst) + g * KV4_GROUP, v);
+        store8_half(dst + g * KV4_GROUP, v, up);
     }
-    const int any = __syncthreads_or(nan != 0u);
-    if (threadIdx.x == 0) a.value_marks[at] = any;
-    if (any && (lane & 3) == 0) a.marks[at * SPREAD_PAGE + slot_out] = (unsigned char)nan;
+    if (plane == 1) {
+        if (threadIdx.x == 0) a.value_marks[at] = any;
+        if (any && (lane & 3) == 0) a.marks[at * SPREAD_PAGE + slot_out] = (unsigned char)nan;
+    }
     qil_wait_for_producer();
 }
 
 struct Kv4SpreadCall {
     const void *pages, *block_table, *info;
-    void *rows, *key_factor, *value_marks, *marks;
+    void *rows, *factors, *value_marks, *marks;
     cudaStream_t stream;
     int table_height, table_width, segments, width, kv_heads, dim, page_size, num_pages, window, least, beside;
 };
 extern "C" int qil_kv4_spread(const void* packed) {
-    const auto [pages, block_table, info, rows, key_factor, value_marks, marks, stream, table_height, table_width, segments, width, kv_heads, dim,
+    const auto [pages, block_table, info, rows, factors, value_marks, marks, stream, table_height, table_width, segments, width, kv_heads, dim,
                 page_size, num_pages, window, least, beside] = kv4_call<Kv4SpreadCall>(packed);
     if (segments <= 0 || width <= 0) return 0;
     if (dim <= 0 || dim > 128 || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, 96, 128, not %d", dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || 2 * kv_heads > 65535 || segments >= 65535) QIL_REFUSE("%d kv heads, %d segments", kv_heads, segments);
     const Kv4Spread a = {(const uint8_t*)pages, {(const int*)block_table, table_height, table_width, page_size, num_pages}, (const int*)info,
-                         (__half*)rows, (float*)key_factor, (int*)value_marks, (unsigned char*)marks, kv_heads, dim, window, least, beside};
+                         (__half*)rows, (float*)factors, (int*)value_marks, (unsigned char*)marks, kv_heads, dim, window, least, beside};
     const dim3 grid(width, 2 * kv_heads, segments);
     void (*kernel)(Kv4Spread) = dim == 32 ? kv4_spread_kernel<1> : dim == 64 ? kv4_spread_kernel<2> : dim == 96 ? kv4_spread_kernel<3> : kv4_spread_kernel<4>;
     qil_launch_chained(kernel, grid, dim3(32 * READ_WARPS), 0, stream, a);

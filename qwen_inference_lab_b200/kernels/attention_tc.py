@@ -75,20 +75,20 @@ def keys16_splits(blocks, tiles) -> int:
     return max(1, min(2 * 148 // blocks, tiles // 8))
 
 
-def prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, segments, n_segments, least, n_tiles, table, n_pages,
+def prefill_keys16(q, rows, factors, value_marks, marks, part_o, part_ml, out, segments, n_segments, least, n_tiles, table, n_pages,
                    n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits):
-    """``prefill`` over ``rows``, pages [n_pages, 2, Hkv, 64, head_dim] of float16 keys and bfloat16 values: ``key_factor`` float32 [n_pages, Hkv]
-    multiplies the keys back; ``value_marks`` int32 [n_pages, Hkv] and ``marks`` uint8 [n_pages, Hkv, 64] say where a position's value groups of 32 are NaN (they hold zeros then).  ``segments`` int32 [n_segments * 4] =
+    """``prefill`` over ``rows``, pages [n_pages, 2, Hkv, 64, head_dim] of float16 keys and values: ``factors`` float32 [n_pages, 2, Hkv], powers of
+    two, multiply them back; ``value_marks`` int32 [n_pages, Hkv] and ``marks`` uint8 [n_pages, Hkv, 64] say where a position's value groups of 32 are NaN (they hold zeros then).  ``segments`` int32 [n_segments * 4] =
     (first token, its position, tokens, row of ``table``), the longest contexts first, of which those of fewer than ``least`` tokens are left alone;
     ``n_tiles``: of 128 / ``pack`` tokens over the others.
-    ``splits`` > 1: ``part_o`` and ``part_ml`` hold 128 rows of head_dim and of 2 floats for every tile, head group and split.
+    ``splits`` > 1: ``part_o`` and ``part_ml`` hold 128 rows of head_dim and of 4 floats for every tile, head group and split.
     From ``rows`` to ``part_ml`` they are addresses: ``kernels.kv4`` lays them out in one buffer and is what calls this."""
     lib = keys16_library(head_dim)
     word = _fault.tensor(out.device)
     _fault.mark()
     _check(lib, lib.qil_attn_tc_prefill_keys16(
         _p(q), c_void_p(rows), _p(out), _p(segments), c_int(n_segments), c_int(least), c_int(n_tiles), c_int(out.shape[0]), _p(table), c_int(table.shape[1]),
-        c_int(n_q_heads), c_int(n_kv_heads), c_int(n_pages), c_float(scale), c_int(window), c_int(pack), c_int(splits), c_void_p(key_factor),
+        c_int(n_q_heads), c_int(n_kv_heads), c_int(n_pages), c_float(scale), c_int(window), c_int(pack), c_int(splits), c_void_p(factors),
         c_void_p(value_marks), c_void_p(marks), c_void_p(part_o), c_void_p(part_ml), _p(word), _stream()),
         "attention (portions, float16 keys)", kernels=2 if splits > 1 else 1)
 

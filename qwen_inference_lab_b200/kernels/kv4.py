@@ -494,16 +494,16 @@ def _portions(plan, batch, least, beside, q, pages, out, block_table, n_q_heads,
     # rows, what goes with them and partial outputs, in one buffer: every part from a 128-byte boundary on
     heads, parts = n_pages * n_kv_heads, n_tiles * groups * splits * attention_tc.TILE if splits > 1 else 0
     at, total = [], 0
-    for nbytes in (2 * size, 4 * heads, 4 * heads, heads * READ_PAGE, 4 * parts * head_dim, 8 * parts):
+    for nbytes in (2 * size, 8 * heads, 4 * heads, heads * READ_PAGE, 4 * parts * head_dim, 16 * parts):
         at.append(total)
         total += -(-nbytes // 128) * 128
     base = _rows(extras, q.get_device(), total).data_ptr()
-    rows, key_factor, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
+    rows, factors, value_marks, marks, part_o, part_ml = (base + offset for offset in at)
     lib = library()
     _check(lib, lib.qil_kv4_spread(_SPREAD.pack(
-        pages.data_ptr(), block_table.data_ptr(), array[f"b{batch}.spread"].data_ptr(), rows, key_factor, value_marks, marks, _stream(q.get_device()),
+        pages.data_ptr(), block_table.data_ptr(), array[f"b{batch}.spread"].data_ptr(), rows, factors, value_marks, marks, _stream(q.get_device()),
         *block_table.shape, segments, most, n_kv_heads, head_dim, page_size, pages.shape[0], window, least, beside)), "kv4.attend (rows of portions)")
-    attention_tc.prefill_keys16(q, rows, key_factor, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
+    attention_tc.prefill_keys16(q, rows, factors, value_marks, marks, part_o, part_ml, out, array[f"b{batch}.segments"], segments, least, n_tiles,
                                 table, n_pages, n_q_heads, n_kv_heads, head_dim, scale, window, pack, splits)
 
 

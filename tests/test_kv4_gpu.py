@@ -545,3 +545,18 @@ def test_two_graphs_and_a_call_share_scratch(dtype, clusters, monkeypatch):
             out.fill_(math.nan)
             graph.replay()
             assert torch.equal(out, expected)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("lens", [[1, 4], [150, 40]], ids=["few", "portions"])
+def test_attend_values_of_all_sizes(lens, window, dtype):
+    """Pages whose values are 10^-20 beside pages of 10^6 and of zeros: rows that see the small ones only have them as exactly as others."""
+    starts = [700 - n for n in lens]
+    built = attend_case(8, 2, 64, 16, starts, lens, dtype, seed=12)
+    sizes = torch.tensor([1e-20, 1e3, 0.0, 1e-3, 1.0, 1e-12, 30.0, 1e6, 0.0, 1e-20, 1e-20, 5.0])[:, None, None]
+    keys = [held[0] for held in built["held"]]
+    values = [held[1].float() * sizes.repeat_interleave(64, dim=0)[:700] for held in built["held"]]
+    pages, table, held = plain.build(keys, values, [700, 700], 16, seed=1)
+    built.update(pages=pages, table=table, held=held)
+    attend_check(built, attend_run(built, window), window)
