@@ -16,6 +16,7 @@ from __future__ import annotations
 import functools
 from ctypes import c_char_p, c_int
 from struct import Struct
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -304,6 +305,18 @@ def refresh_single_tokens(arrays, starts) -> None:
         info[last:width * n:width] = longest
 
 
+class Reach(NamedTuple):
+    """Contexts that a launch walks: the longest of them, the shortest that the longest may be, their mean as a part of the longest."""
+    max_context: int
+    min_context: int
+    fill: float
+
+    @classmethod
+    def of(cls, ends, most=0, least=0):
+        longest = int(ends.max(initial=1))
+        return cls(most or longest, least, round(16 * float(ends.mean()) / longest) / 16 if len(ends) else 1.0)
+
+
 class StepPlan:
     """A step's segments on the device, as ``attend`` reads them.  ``max_context``: the longest context; of a recorded step the
     longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest.  ``settled``: no kernel right
@@ -316,6 +329,10 @@ class StepPlan:
         self.multi_lens = lens[lens > 1]
         self.tokens = int(lens.sum())
         self.max_context, self.min_context, self.settled = int(max_context), int(min_context), int(settled)
+        ends = starts + lens
+        # the contexts of single tokens and of longer segments; of recorded steps (single tokens) the longest is a bound
+        self.singles = Reach.of(ends[lens == 1], self.max_context if min_context else 0, self.min_context)
+        self.multi = Reach.of(ends[lens > 1])
 
     @classmethod
     def of_segments(cls, rows, starts, lens, device):
@@ -361,27 +378,28 @@ def _clustered(n, blocks_per_span, step_us, clusters) -> bool:
 
 
 @functools.lru_cache(maxsize=4096)
-def _plan(blocks_per_span, step_us, size, lo, hi, most, join, clusters) -> int:
-    """The number of spans that costs least per step of keys at both ends of [lo, hi] steps of longest context."""
+def _plan(blocks_per_span, step_us, size, lo, hi, most, join, clusters, fill) -> int:
+    """The number of spans that costs least per step of keys at both ends of [lo, hi] steps of longest context, of which the contexts have
+    ``fill`` on the average: half a span more than that share of the spans holds something (48 requests of up to 16384: 3 spans 169 us, 9 145)."""
     full = SMS * len(step_us)
 
     def cost(steps, n):
         clustered = _clustered(n, blocks_per_span, step_us, clusters)
         each = -(-steps // n)
         n = -(-steps // each)                           # spans that hold anything
-        waves, rest = divmod(blocks_per_span * n, full)
+        waves, rest = divmod(int(blocks_per_span * min(n, fill * n + 0.5)), full)
         time = each * size * (waves * step_us[-1] + (step_us[-(-rest // SMS) - 1] if rest else 0.0)) + START_US * (waves + (rest > 0))
         return (time + (CLUSTER_SPAN_US * n if clustered else join[0] + join[1] * n if n > 1 else 0.0)) / steps
     return min(range(1, min(hi, most) + 1), key=lambda n: cost(hi, n) + (cost(lo, min(n, lo)) if lo != hi else 0.0))
 
 
-def _spans(blocks_per_span, step_us, size, plan, window, most, join=(JOIN_US, SPAN_US), clusters=()) -> int:
+def _spans(blocks_per_span, step_us, size, reach, window, most, join=(JOIN_US, SPAN_US), clusters=()) -> int:
     """Parts to cut the contexts into."""
-    hi, lo = plan.max_context, plan.min_context or plan.max_context
+    hi, lo = reach.max_context, reach.min_context or reach.max_context
     if window:
         hi, lo = min(hi, window + STEP), min(lo, window + STEP)
     hi = max(1, -(-hi // STEP))
-    return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most), join, clusters)
+    return _plan(blocks_per_span, step_us, size, max(1, min(hi, -(-lo // STEP))), hi, max(1, most), join, clusters, 1.0 if window else reach.fill)
 
 
 def _capturing() -> bool:
@@ -436,7 +454,7 @@ def _rows(extras, device, nbytes):
     return held[0]
 
 
-def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
+def _few(info, n, tokens, most_tokens, plan, reach, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib, most, blocks_a_sm = few_library(head_dim)
     rows = most_tokens * (n_q_heads // n_kv_heads)
     nt = 1 if rows <= 8 else 2
@@ -444,7 +462,7 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
     # the partial sums of all spans: fewer spans where they would outgrow their limit
     most = min(most, attention_f32.MOST_SCRATCH // (4 * tokens * n_q_heads * head_dim))
     step_us = STEP_US[nt][:blocks_a_sm[nt]]
-    n_spans = _spans(blocks, step_us, 0.4 + 0.15 * (head_dim // GROUP), plan, window, most, JOINS_US[nt], CLUSTERS[nt])
+    n_spans = _spans(blocks, step_us, 0.4 + 0.15 * (head_dim // GROUP), reach, window, most, JOINS_US[nt], CLUSTERS[nt])
     clustered = _clustered(n_spans, blocks, step_us, CLUSTERS[nt])
     device = q.get_device()
     part_o, part_ml, tickets = _scratch(extras, device, tokens, n_q_heads, 1 if clustered else n_spans, head_dim)
@@ -454,13 +472,13 @@ def _few(info, n, tokens, most_tokens, plan, q, pages, out, block_table, n_q_hea
         pages.shape[0], window, clustered, plan.settled)), "kv4.attend (few tokens)")
 
 
-def _singles(info, n, plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
+def _singles(info, n, reach, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
     lib = library()
     chunks = -(-(n_q_heads // n_kv_heads) // lib.qil_kv4_singles_heads(n_q_heads // n_kv_heads))
     for begin in range(0, n, 65535):                       # a grid's third size
         some = min(65535, n - begin)
         most = attention_f32.MOST_SCRATCH // (4 * some * n_q_heads * head_dim)
-        n_spans = _spans(some * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, plan, window, most)
+        n_spans = _spans(some * n_kv_heads * chunks, SINGLES_STEP_US, 1.0, reach, window, most)
         device = q.get_device()
         part_o, part_ml, tickets = _scratch(extras, device, some, n_q_heads, n_spans, head_dim)
         _check(lib, lib.qil_kv4_singles(_SINGLES.pack(
@@ -533,26 +551,26 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
     shape = (q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, float(scale), int(window), extras)
     count, array = plan.count, plan.array
     if q.dtype == torch.float32:
-        for name in ("single_tokens", "few_tokens"):
+        for name, reach in (("single_tokens", plan.singles), ("few_tokens", plan.multi)):
             if count[name]:
-                _singles(array[name], count[name] // 4, plan, *shape)
+                _singles(array[name], count[name] // 4, reach, *shape)
         if count["portion_tokens"]:
             if attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads):
                 for batch in range(len(plan.portion_lens)):
                     _portions(plan, batch, FEW_TOKENS + 1, False, *shape)
             else:       # heads of a size that the tile kernel does not take: token by token
-                _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan, *shape)
+                _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan.multi, *shape)
         return out
     if count["singles"]:
-        _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, *shape)
+        _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, plan.singles, *shape)
     if len(plan.multi_lens):
         if not attention_tc.supports(head_dim, READ_PAGE, window):          # heads beyond 128
-            _few(array["multi"], len(plan.multi_lens), int(plan.multi_lens.sum()), int(plan.multi_lens.max()), plan, *shape)
+            _few(array["multi"], len(plan.multi_lens), int(plan.multi_lens.sum()), int(plan.multi_lens.max()), plan, plan.multi, *shape)
             return out
         most = FEW_ROWS // (n_q_heads // n_kv_heads)           # tokens
         few = plan.multi_lens[plan.multi_lens <= most]
         if len(few):
-            _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, *shape)
+            _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, plan.multi, *shape)
         if len(few) < len(plan.multi_lens):
             for batch in range(len(plan.portion_lens)):
                 _portions(plan, batch, max(most, 1) + 1, batch == 0 and bool(count["singles"] or len(few)), *shape)

@@ -126,12 +126,17 @@ def test_long_contexts_are_read_in_batches():
 
 def test_spans_fill_the_gpu():
     """More requests, fewer spans; a context of one step is not cut; never more spans than there is room for."""
-    plan = lambda context: kv4.StepPlan.of_segments([0], [context - 1], [1], "cpu")
+    plan = lambda context: kv4.StepPlan.of_segments([0], [context - 1], [1], "cpu").singles
     spans = lambda blocks, context, window=0, most=128: kv4._spans(blocks, kv4.STEP_US[1], 1.0, plan(context), window, most)
     assert spans(8, 100) == 1 and spans(8, 8192) >= 16 and spans(64, 8192) == 8 and spans(2000, 8192) <= 2
     assert spans(8, 8192, most=3) == 3 and spans(8, 100000, window=100) == spans(8, 228)
     counts = [spans(blocks, 16384) for blocks in (8, 32, 128, 600)]
     assert counts == sorted(counts, reverse=True)
+    # ragged contexts are cut more finely than as many of the longest; segments of several tokens do not count among single ones
+    ragged = kv4.StepPlan.of_segments(range(49), [*range(0, 16320, 340), 30000], [1] * 48 + [20], "cpu")
+    assert ragged.singles.max_context == 15981 and ragged.singles.fill == 0.5 and ragged.multi == (30020, 0, 1.0)
+    even = kv4.StepPlan.of_segments(range(48), [15980] * 48, [1] * 48, "cpu")
+    assert kv4._spans(384, kv4.STEP_US[1], 1.0, ragged.singles, 0, 128) > kv4._spans(384, kv4.STEP_US[1], 1.0, even.singles, 0, 128)
 
 
 def test_scratch_that_a_recorded_graph_points_to(monkeypatch):
