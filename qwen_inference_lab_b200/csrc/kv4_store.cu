@@ -11,7 +11,7 @@
 // 64-bit arithmetic is what such a kernel would take its time for, and hardly any element needs it: a row is computed in 32 bits first,
 // with a bound on what that may be off (up to 15 roundings of the two products that a turn adds), and again in 64 bits only if a step, a
 // base or a code could come out otherwise within that bound (a row or two in a hundred).  Such a row keeps its warp waiting for 3.9 us, and
-// among 64 tokens there is one nearly always: 64 tokens of 32 + 2 x 8 heads of 128 take 7.0 us, 3.8 if none had to; 2048 take 30.4 and 26.9.
+// among 64 tokens there is one nearly always: 64 tokens of 32 + 2 x 8 heads of 128 take 6.8 us, 3.6 if none had to; 2048 take 26.5 and 22.9.
 // (The same in pairs of 32-bit numbers with an exact sum and product waits 2.9: not worth a third way.)  The rest is instructions: a lane takes 8
 // neighbouring elements, so that a head of 128 is half a warp and a group's codes are one word of each of four lanes, and a token's
 // cosines and sines times the weights stay in registers from head to head: (x r w) c -+ (x' r w') s is r (x (w c) -+ x' (w' s)).
@@ -25,8 +25,8 @@
 
 QIL_ERROR_STORAGE
 
-// Warps a block, blocks an SM.  Measured (us, 64 / 256 / 2048 tokens): 8 x 4 7.5 / 10.2 / 34.0, 8 x 3 6.5 / 9.2 / 35.8, 4 x 6 6.5 / 8.5 / 33.8, 4 x 7 7.0 /
-// 9.1 / 30.5, 4 x 8 7.4 / 10.3 / 30.6, 2 x 14 7.4 / 9.8 / 29.7.
+// Warps a block, blocks an SM.  Measured (us, 64 / 256 / 2048 tokens): 8 x 4 7.2 / 9.3 / 31.5, 4 x 6 6.5 / 8.2 / 31.0, 4 x 7 6.7 / 8.8 / 26.9, 4 x 8 7.0 /
+// 9.5 / 26.7, 2 x 14 7.2 / 9.8 / 26.1.
 static constexpr int STORE_WARPS = 4, STORE_BLOCKS = 7;
 
 struct Kv4Store {
@@ -101,9 +101,9 @@ __device__ __forceinline__ void code_exact(const double (&y)[8], unsigned& codes
     pair = good ? pair_of(step, base) : NAN_PAIR;
 }
 // The same from elements of which those of this lane's group are off by `off` at most; false where that could make a difference.
-// Elements that are exact (off = 0) as their distances from the base are, as bfloat16 values are, lie between two codes often
+// Elements that are exact (EXACT, off = 0) as their distances from the base are, as bfloat16 values are, lie between two codes often
 // (s times a half is a number like they are): the sign of (y - m) - (n + 1/2) s, one rounding, decides them, and 0 is a tie.
-__device__ __forceinline__ bool code_within(const float (&y)[8], float off, unsigned& codes, unsigned& pair) {
+template <bool EXACT> __device__ __forceinline__ bool code_within(const float (&y)[8], float off, unsigned& codes, unsigned& pair) {
     float lo, hi;
     range_of(y, lo, hi);
     const float range = hi - lo, wide = fmaf(range, 2.4e-7f, 2.f * off) * 1.001f;      // what the range may be off, its own rounding included
@@ -124,7 +124,7 @@ __device__ __forceinline__ bool code_within(const float (&y)[8], float off, unsi
     }
     pair = pair_of(step, base);
     sure = sure && sum == sum;
-    if (sure && off == 0.f && !(furthest < most)) {
+    if (EXACT && sure && !(furthest < most)) {
         codes = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -199,6 +199,8 @@ __device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
 }
 
+// 1 / sqrt(v): queries have no borders and can do with 2^-22.
+__device__ __forceinline__ float root_of(float v, bool near) { return near ? rsqrtf(v) : 1.f / sqrtf(v); }
 // Sum over the lanes of a head.
 template <int LANES, typename R> __device__ __forceinline__ R head_sum(R v) {
 #pragma unroll
@@ -273,6 +275,7 @@ __device__ __noinline__ uint2 values_exact(float4 x0, float4 x1) {
 
 // A block: a token and every (gridDim.y)th set of STORE_WARPS steps, from the last on; a warp takes 32 / LANES heads of one kind a step, LANES lanes of 8
 // elements each (the first dim / 8 of them; a power of two).
+template <int KIND> struct Kind { static constexpr int kind = KIND; };
 template <typename T, typename W, int LANES>
 __global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kernel(const __grid_constant__ Kv4Store a) {
     constexpr int HEADS = 32 / LANES;
@@ -307,36 +310,34 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kern
     // where a halves layout's other elements lie: whole lanes away, or anywhere
     const bool by_lanes = half % 8 == 0;
     const int other_lane = lane + (d0 >= a.rot_dims ? 0 : d0 < half ? half / 8 : -(half / 8));
+    const int slot = pos % a.table_of.page_size;
+    const int head_bytes = (a.table_of.page_size >> 3) * kv4_run_bytes(groups);
+    uint8_t* const to = page < 0 ? nullptr : a.pages + kv4_run_at(page, 0, 0, slot, a.kv_heads, a.table_of.page_size, groups);
+    const int code_at = kv4_code_at(l >> 2, slot) + (l & 3) * 4, pair_at = kv4_pair_at(l >> 2, slot, groups);
     float cw[8], sw[8];
-    int kind = -1;
-    // every warp takes values or keys, which take longest, and then queries (2048 tokens 34.0 us, a warp's steps side by side 35.8)
-    const int steps = steps_q + 2 * steps_kv;
-    for (int back = blockIdx.y * STORE_WARPS + warp; back < steps; back += gridDim.y * STORE_WARPS) {
-        const int step = steps - 1 - back;
-        const int now = step < steps_q ? 0 : step < steps_q + steps_kv ? 1 : 2;              // queries, keys, values
-        if (now > 0 && page < 0) continue;
-        const int head = (step - (now == 0 ? 0 : now == 1 ? steps_q : steps_q + steps_kv)) * HEADS + sub;
+    auto load_factors = [&](int kind) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(&factor[kind][0][d0 + i]), s = *reinterpret_cast<const float4*>(&factor[kind][1][d0 + i]);
+            cw[i] = c.x; cw[i + 1] = c.y; cw[i + 2] = c.z; cw[i + 3] = c.w;
+            sw[i] = s.x; sw[i + 1] = s.y; sw[i + 2] = s.z; sw[i + 3] = s.w;
+        }
+    };
+    // the `index`th set of heads of a kind: queries, keys, values
+    auto step = [&](auto of, int index) {
+        constexpr int now = decltype(of)::kind;
+        const int head = index * HEADS + sub;
         const bool mine = head < (now == 0 ? a.q_heads : a.kv_heads) && d0 < a.dim;
-        const T* src = reinterpret_cast<const T*>(a.proj) + (size_t)token * a.ld + (now == 0 ? a.q_col : now == 1 ? a.k_col : a.v_col) + (size_t)head * a.dim;
+        const T* src = reinterpret_cast<const T*>(a.proj) + (size_t)token * a.ld + (now == 0 ? a.q_col : now == 1 ? a.k_col : a.v_col) + head * a.dim;
         typename Eight<T>::type own, partner;
         own.zero();
         if (mine) {
             if (a.vectors) own.load(src + d0);
             else own.one_by_one(src + d0);
         }
-        if (now != kind && now < 2) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const float4 c = *reinterpret_cast<const float4*>(&factor[now][0][d0 + i]), s = *reinterpret_cast<const float4*>(&factor[now][1][d0 + i]);
-                cw[i] = c.x; cw[i + 1] = c.y; cw[i + 2] = c.z; cw[i + 3] = c.w;
-                sw[i] = s.x; sw[i + 1] = s.y; sw[i + 2] = s.z; sw[i + 3] = s.w;
-            }
-            kind = now;
-        }
-        float x[8], y[8], off = 0.f;
+        float x[8], y[8], xp[8], off = 0.f;
         own.floats(x);
-        float xp[8];
-        if (now < 2) {
+        if constexpr (now < 2) {
             if (a.interleaved) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) xp[i] = x[i ^ 1];
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kern
                 float sq = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
-                r = 1.f / sqrtf(head_sum<LANES>(sq) / (float)a.dim + a.eps);
+                r = root_of(head_sum<LANES>(sq) / (float)a.dim + a.eps, now == 0);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -364,44 +365,59 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kern
                 float sq = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sq = fmaf(y[i], y[i], sq);
-                r = 1.f / sqrtf(head_sum<LANES>(sq) / (float)a.dim + a.eps);
+                r = root_of(head_sum<LANES>(sq) / (float)a.dim + a.eps, now == 0);
             }
             if (a.norm) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] *= r;
                 off *= r < 1e13f ? r : INFINITY;                                             // squares of less than 1e-26 lose bits
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i];
         }
-        if (now == 0) {
+        if constexpr (now == 0) {
             if (mine) store8(reinterpret_cast<T*>(a.q_out) + ((size_t)token * a.q_heads + head) * a.dim + d0, y);
-            continue;
-        }
-        // 15 roundings of the two products; where the norm is of the turned head their errors go into its sum of squares, and so from
-        // any element into any other: up to 60 roundings of the largest (one large element among 255 equal ones)
+        } else {
+            unsigned codes, pair;
+            bool sure;
+            if constexpr (now == 1) {
+                // 15 roundings of the two products; where the norm is of the turned head their errors go into its sum of squares, and so
+                // from any element into any other: up to 60 roundings of the largest (one large element among 255 equal ones)
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1)
-            if (o < 4 || a.norm == 2) off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, o));
-        unsigned codes, pair;
-        const bool sure = code_within(y, off * (a.norm == 2 ? 0x1p-18f : 0x1p-20f), codes, pair);
-        if (__any_sync(0xffffffffu, mine && !sure)) {
-            const float4 x0 = make_float4(x[0], x[1], x[2], x[3]), x1 = make_float4(x[4], x[5], x[6], x[7]);
-            const uint2 found = now == 1
-                ? keys_exact<W, LANES>(reinterpret_cast<const W*>(a.k_weight), angles, a.eps, a.norm, a.dim, a.rot_dims, a.interleaved, d0, x0, x1,
-                                       make_float4(xp[0], xp[1], xp[2], xp[3]), make_float4(xp[4], xp[5], xp[6], xp[7]))
-                : values_exact(x0, x1);
-            codes = found.x;
-            pair = found.y;
+                for (int o = 1; o < LANES; o <<= 1)
+                    if (o < 4 || a.norm == 2) off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, o));
+                sure = code_within<false>(y, off * (a.norm == 2 ? 0x1p-18f : 0x1p-20f), codes, pair);
+            } else {
+                sure = code_within<true>(x, 0.f, codes, pair);
+            }
+            if (__any_sync(0xffffffffu, mine && !sure)) {
+                const float4 x0 = make_float4(x[0], x[1], x[2], x[3]), x1 = make_float4(x[4], x[5], x[6], x[7]);
+                uint2 found;
+                if constexpr (now == 1)
+                    found = keys_exact<W, LANES>(reinterpret_cast<const W*>(a.k_weight), angles, a.eps, a.norm, a.dim, a.rot_dims, a.interleaved, d0, x0, x1,
+                                                 make_float4(xp[0], xp[1], xp[2], xp[3]), make_float4(xp[4], xp[5], xp[6], xp[7]));
+                else found = values_exact(x0, x1);
+                codes = found.x;
+                pair = found.y;
+            }
+            if (mine) {
+                uint8_t* run = to + (size_t)((now - 1) * a.kv_heads + head) * head_bytes;
+                *reinterpret_cast<unsigned*>(run + code_at) = codes;
+                if ((l & 3) == 0) *reinterpret_cast<unsigned*>(run + pair_at) = pair;
+            }
         }
-        if (mine) {
-            const int slot = pos % a.table_of.page_size;
-            uint8_t* run = a.pages + kv4_run_at(page, now - 1, head, slot, a.kv_heads, a.table_of.page_size, groups);
-            *reinterpret_cast<unsigned*>(run + kv4_code_at(l >> 2, slot) + (l & 3) * 4) = codes;
-            if ((l & 3) == 0) *reinterpret_cast<unsigned*>(run + kv4_pair_at(l >> 2, slot, groups)) = pair;
-        }
-    }
+    };
+    // Every warp takes values or keys, which take longest, and then queries; a loop of its own a kind (one for all of them, with branches inside,
+    // took 30.7 us of 2048 tokens instead of 26.9).
+    const int stride = gridDim.y * STORE_WARPS;
+    int at = blockIdx.y * STORE_WARPS + warp;
+    for (; at < steps_kv; at += stride)
+        if (page >= 0) step(Kind<2>(), at);
+    at -= steps_kv;
+    if (at < steps_kv) load_factors(1);
+    for (; at < steps_kv; at += stride)
+        if (page >= 0) step(Kind<1>(), at);
+    at -= steps_kv;
+    load_factors(0);
+    for (; at < steps_q; at += stride) step(Kind<0>(), at);
 }
 
 struct Kv4StoreCall {
