@@ -28,10 +28,10 @@ GROUP = 32
 MOST_DIM = 256
 PLAN_KEY = "kv4_attention"        # the step planner whose arrays ``attend`` reads (``describe_segments`` makes them)
 #: Rows (tokens of a segment times query heads of a kv head) up to which the kernel that walks the codes takes more than one token; of
-#: more the rows are read back once and attended to as 16-bit pages.  Measured (us, this kernel / the other one; 4 heads of 128 a kv head):
-#: 8 segments behind 4000 of 2, 4, 8, 16 tokens 21 / 72, 40 / 72, 59 / 72, 94 / 74; one segment 11 / 25, 18 / 25, 23 / 25, 27 / 26; 8
-#: segments behind 500 8.7 / 19, 13 / 19, 14 / 19, 22 / 22.
-FEW_ROWS = 32
+#: more the rows are read back once and attended to as 16-bit pages.  Measured (us, this kernel / the other one; 4 heads of 128 a kv head; of
+#: 2, 4, 8, 12, 16 tokens): 8 segments behind 4000 18 / 75, 33 / 77, 55 / 77, 56 / 78, 96 / 79; one 11 / 26, 14 / 26, 18 / 26, 29 / 26, 23 / 26; 8
+#: behind 500 9 / 21, 14 / 21, 18 / 21, 18 / 21, 23 / 24; 4 behind 16000 31 / 138, 58 / 138, 91 / 138, 111 / 138, 149 / 139.
+FEW_ROWS = 48
 #: Tokens of a segment up to which the 32-bit path takes them one by one.
 FEW_TOKENS = 8
 #: Positions per page of rows that are read back for a portion, and the most of them at a time (of several portions; a single
