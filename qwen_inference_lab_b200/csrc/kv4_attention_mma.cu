@@ -46,6 +46,7 @@ static constexpr int WARPS = 4, TILE = 32, STAGES = 2;
 static constexpr int STAGE_BYTES = 8 * RUN;            // 4 runs of keys, 4 of values
 static constexpr int MOST_SPANS = 128, MOST_CLUSTER = 16;
 static constexpr int MOST_LIFT = 90;
+static constexpr unsigned TINY_STEP = (127 - 60) << 7; // bits of 2^-60: times 2^MOST_LIFT and a small weight it would leave the products' range
 static constexpr float NOTHING = -3e38f;               // the largest score of none
 
 struct Kv4Few {
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
         for (int g = 1; g < G; ++g) largest = max_pairs(largest, pairs[g]);
         const bool partly = (unsigned)(k0 - plain_low) > (unsigned)plain_more || plain_more < 0 || gone;
-        if (partly || __any_sync(0xffffffffu, (largest & 0xffffu) >= lift_limit)) {
+        if (partly || __any_sync(0xffffffffu, (largest & 0xffffu) >= lift_limit) || (n == 0 && __all_sync(0xffffffffu, (largest & 0xffffu) < TINY_STEP))) {
             const int key = k0 + lane;
             const bool inside = key >= span.first && key < span.last && !(gone >> (lane >> 3) & 1);
             unsigned nan = 0;
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                         if (k0 + j <= pos && (a.window == 0 || k0 + j > pos - a.window)) marked[nt][i] |= groups;
                     }
             }
-            // the lift: by the exponent of the tile's largest step
+            // the lift: by the exponent of the tile's largest step; higher than the usual one only where the first tile's steps are tiny
             const int exponent = (int)(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 7) - 127;
             if (exponent + (int)lift > 100) {
                 const int lower = 92 - exponent;
@@ -438,6 +439,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 lift = (float)lower;
                 lift_limit = (unsigned)min(max(228 - lower, 0), 255) << 7;
                 sink = (unsigned)(127 - lower) << 7 | (unsigned)(127 - lower) << 23;
+            } else if (n == 0 && exponent > -127 && exponent < (int)(TINY_STEP >> 7) - 127) {
+                const int higher = min(92 - exponent, 118);           // p 2^lift stays below 2^127
+                lift = (float)higher;
+                lift_limit = (unsigned)max(228 - higher, 0) << 7;
+                sink = (unsigned)(127 - higher) << 7 | (unsigned)(127 - higher) << 23;
             }
             __syncwarp();
 #pragma unroll

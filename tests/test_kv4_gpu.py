@@ -560,3 +560,26 @@ def test_attend_values_of_all_sizes(lens, window, dtype):
     pages, table, held = plain.build(keys, values, [700, 700], 16, seed=1)
     built.update(pages=pages, table=table, held=held)
     attend_check(built, attend_run(built, window), window)
+
+
+@pytest.mark.parametrize("lens", [[1, 4], [150, 40]], ids=["few", "portions"])
+def test_attend_groups_of_other_sizes(lens):
+    """A head whose groups of values are up to 2^10 apart, and one of zeros: every group as exact as if it were alone."""
+    starts = [300 - n for n in lens]
+    built = attend_case(8, 2, 128, 16, starts, lens, BF16, seed=14)
+    sizes = torch.tensor([1.0, 2.0 ** -10, 0.0, 2.0 ** -5]).repeat_interleave(32)
+    keys, values = [held[0].float() for held in built["held"]], [held[1].float() * sizes for held in built["held"]]
+    pages, table, held = plain.build(keys, values, [300, 300], 16, seed=2)
+    built.update(pages=pages, table=table, held=held)
+    attend_check(built, attend_run(built))
+
+
+@pytest.mark.parametrize("size", [1e-30, 3e-5, 1e25])
+@pytest.mark.parametrize("lens", [[1, 4], [150, 40]], ids=["few", "portions"])
+def test_attend_values_all_of_one_size(lens, size):
+    starts = [300 - n for n in lens]
+    built = attend_case(8, 2, 64, 16, starts, lens, BF16, seed=13)
+    keys, values = ([held[i].float() * (size if i else 1.0) for held in built["held"]] for i in (0, 1))
+    pages, table, held = plain.build(keys, values, [300, 300], 16, seed=2)
+    built.update(pages=pages, table=table, held=held)
+    attend_check(built, attend_run(built))
