@@ -37,6 +37,8 @@ FEW_TOKENS = 8
 #: Positions per page of rows that are read back for a portion, and the most of them at a time (of several portions; a single
 #: one may be longer): 8 heads of 128 in bfloat16 take 4 KB a position.
 READ_PAGE, MOST_READ = 64, 1 << 16
+#: Bytes that the memory for those rows grows by at most beyond what is asked for.
+MOST_GROWTH = 256 << 20
 
 SOURCES, DEPENDS = ["kv4_store.cu", "kv4_attention.cu"], ["kv4.h"]
 _lib = None
@@ -443,12 +445,17 @@ def _scratch(extras, device, tokens, n_q_heads, n_spans, head_dim):
 
 
 def _rows(extras, device, nbytes):
-    """Memory for the rows of portions."""
+    """Memory for the rows of portions.  It grows to twice what it was, by MOST_GROWTH at most: a prompt that comes in chunks asks for a page
+    more every 64 positions, and as much as it asks for would leave the allocator a block that is too small behind every time (chunks of 64
+    behind up to 32768: 10 allocations instead of 512)."""
     key = ("kv4_rows", device)
     held = extras.get(key)
     if held is None or held[0].numel() < nbytes:
+        had = held[0].numel() if held else 0
         _replaced(held)
-        held = extras[key] = (torch.empty(nbytes, dtype=torch.uint8, device=device),)
+        held = None
+        extras.pop(key, None)           # given back before the larger one is asked for, unless a recorded graph points to it
+        held = extras[key] = (torch.empty(max(nbytes, min(2 * had, had + MOST_GROWTH)), dtype=torch.uint8, device=device),)
     if _capturing():
         _keep(extras, held)
     return held[0]
