@@ -70,7 +70,9 @@ class StepRunner:
         self._graph_pool = None
         self._extras: dict = {}      # what parts keep from step to step (scratch buffers), by their own keys
         self._single_token_template = None
-        self._reserve(8 * max_step_tokens + 16 * cache.max_requests + 64)
+        longest = min(model.max_positions, cache.table_width * cache.page_size)
+        self._reserve(8 * max_step_tokens + 16 * cache.max_requests + 64
+                      + sum(planner.most_ints(max_step_tokens, cache.max_requests, longest) for planner in self.planners))
         self.steps_run = 0
         self.kernel_launches = 0          # this engine's own kernels (library products are not counted)
         self.launches_per_graph: dict = {}
@@ -82,7 +84,7 @@ class StepRunner:
     def _reserve(self, ints):
         if ints <= self._capacity:
             return
-        self._capacity = int(ints)
+        self._capacity = max(int(ints), 2 * self._capacity)     # a larger step is seldom the only one
         self._meta_dev = torch.zeros(self._capacity, dtype=torch.int32, device=self.device)
         self._graphs.clear()     # recorded graphs point into the old buffer
         self._graph_pool = None  # their memory pool goes with the last of them: the next recording starts a new one

@@ -234,14 +234,24 @@ def read(pages, block_table, info, segments, longest, out, n_kv_heads, head_dim,
 
 
 # ------------------------------------------------------------------ the plan of a step
-def describe_segments(first, starts, lens, rows) -> dict:
+def _one_by_one(first, starts, lens, rows, indices):
+    """The tokens of the segments ``indices``, four ints each: (token, its position, block-table row, the longest context among these)."""
+    if not len(indices):
+        return np.zeros(0, dtype=np.int64)
+    of = np.repeat(indices, lens[indices])
+    offset = np.arange(len(of)) - np.repeat(np.cumsum(lens[indices]) - lens[indices], lens[indices])
+    return np.stack([first[of] + offset, starts[of] + offset, rows[of], np.full_like(of, (starts + lens)[indices].max())], axis=1).reshape(-1)
+
+
+def describe_segments(first, starts, lens, rows, portion_tokens=True) -> dict:
     """A step's segments as ``attend`` wants them (numpy int64 arrays in, one entry per segment: first token in the flat batch,
     its absolute position, tokens, block-table row).
 
     ``singles``, ``few``, ``multi``  the segments of one token, of 2 to FEW_ROWS and of any more than one: eight ints each, (first token, its
                         position, tokens, block-table row, tokens of the segments before in this array, the longest context among these, 0, 0)
-    ``single_tokens``, ``few_tokens``, ``portion_tokens``  the segments of one token, of 2 to FEW_TOKENS and the others token by token, four
-                        ints each, (token, its position, block-table row, the longest context among these)
+    ``single_tokens``, ``few_tokens``, ``portion_tokens``  the segments of one token, of 2 to FEW_TOKENS and the others token by token
+                        (``_one_by_one``); the last are read by float32 attention with heads that the tile kernel does not take only, and are
+                        left out where ``portion_tokens`` is False
     ``b0.spread`` ...   the segments of more than one token in batches whose contexts are read back together: (block-table row, first position,
                         end, first page); ``kv4.read``'s info of those beyond FEW_TOKENS; the block table of the pages they are read to; the
                         segments, and tiles of 64 of their tokens beyond FEW_TOKENS, over that table: (first token, its position, tokens, row of it)
@@ -257,18 +267,12 @@ def describe_segments(first, starts, lens, rows) -> dict:
         none = np.zeros_like(before)
         return np.stack([first[indices], starts[indices], lens[indices], rows[indices], before, none + ends[indices].max(), none, none], axis=1).reshape(-1)
 
-    def one_by_one(indices):
-        if not len(indices):
-            return np.zeros(0, dtype=np.int64)
-        of = np.repeat(indices, lens[indices])
-        offset = np.arange(len(of)) - np.repeat(np.cumsum(lens[indices]) - lens[indices], lens[indices])
-        return np.stack([first[of] + offset, starts[of] + offset, rows[of], np.full_like(of, ends[indices].max())], axis=1).reshape(-1)
-
     arrays = {}
     for name, some in (("singles", lens == 1), ("few", (lens > 1) & (lens <= FEW_ROWS)), ("multi", lens > 1)):
         arrays[name] = segments(np.nonzero(some)[0])
     for name, some in (("single_tokens", lens == 1), ("few_tokens", (lens > 1) & (lens <= FEW_TOKENS)), ("portion_tokens", lens > FEW_TOKENS)):
-        arrays[name] = one_by_one(np.nonzero(some)[0])
+        if portion_tokens or name != "portion_tokens":
+            arrays[name] = _one_by_one(first, starts, lens, rows, np.nonzero(some)[0])
     for batch, taken in enumerate(portion_batches(starts, lens)):
         width = -(-int(ends[taken[0]]) // READ_PAGE)               # pages a segment: of the longest, so that segment i's begin at i * width
         local = np.arange(len(taken), dtype=np.int64)
@@ -283,6 +287,15 @@ def describe_segments(first, starts, lens, rows) -> dict:
         found.sort(key=lambda t: -(t[1] + t[2]))                    # the longest contexts first: the short ones fill the gaps
         arrays[f"b{batch}.tiles"] = np.array(found, dtype=np.int64).reshape(-1)
     return arrays
+
+
+def most_ints(tokens, requests, context) -> int:
+    """A bound on the ints of ``describe_segments`` without ``portion_tokens``, every array rounded up to a multiple of 4 and at least 4, for
+    up to so many tokens of so many requests with contexts of up to ``context``: 12 a single token; of a longer segment 16 in ``few`` and ``multi``, 12 in
+    its batch, 8 for tiles that are not full, 20 where the batch is its own, and its pages; 4 a token one by one."""
+    requests = min(requests, tokens)
+    longer = min(requests, tokens // 2)
+    return 12 * requests + longer * (56 + -(-context // READ_PAGE)) + 4 * tokens + 4 * -(-tokens // attention_mma.QUERY_TILE) + 64
 
 
 def portion_batches(starts, lens) -> list:
@@ -324,9 +337,10 @@ class StepPlan:
     longest of the steps it is replayed for, ``min_context`` then the shortest of these steps' longest.  ``settled``: no kernel right
     before an ``attend`` writes these arrays or the block table, so that it may read them while that one finishes."""
 
-    def __init__(self, array, count, starts, lens, max_context, min_context=0, settled=False):
-        """``starts`` and ``lens``: the segments' on the host (numpy)."""
+    def __init__(self, array, count, first, starts, lens, rows, max_context, min_context=0, settled=False):
+        """``first``, ``starts``, ``lens`` and ``rows``: the segments' on the host (numpy)."""
         self.array, self.count = array, count
+        self._segments = first, starts, lens, rows
         self.portion_lens = [lens[taken] for taken in portion_batches(starts, lens)]          # of the batches' segments
         self.multi_lens = lens[lens > 1]
         self.tokens = int(lens.sum())
@@ -345,13 +359,23 @@ class StepPlan:
             raise KernelError("kv4.StepPlan: a row, a start and at least one token a segment")
         arrays = describe_segments(np.cumsum(lens) - lens, starts, lens, rows)
         array = {name: torch.from_numpy(values.astype(np.int32)).to(device) for name, values in arrays.items()}
-        return cls(array, {name: len(values) for name, values in arrays.items()}, starts, lens, int((starts + lens).max(initial=0)))
+        return cls(array, {name: len(values) for name, values in arrays.items()}, np.cumsum(lens) - lens, starts, lens, rows,
+                   int((starts + lens).max(initial=0)))
 
     @classmethod
     def of_step(cls, ctx):
         """Of the step in flight, from the arrays that the planner made for it: the step's ``store`` comes after they are there."""
         view = ctx.plans[PLAN_KEY]
-        return cls(view.array, view.count, ctx.h_seg_pos0, ctx.h_seg_len, ctx.max_context, ctx.min_context, settled=True)
+        return cls(view.array, view.count, ctx.h_seg_start, ctx.h_seg_pos0, ctx.h_seg_len, ctx.h_seg_row, ctx.max_context, ctx.min_context,
+                   settled=True)
+
+    def portion_tokens(self):
+        """(array, tokens) of the portions' tokens one by one.  A step's description leaves them out: few steps need them."""
+        if "portion_tokens" not in self.array:
+            tokens = _one_by_one(*self._segments, np.nonzero(self._segments[2] > FEW_TOKENS)[0]).astype(np.int32)
+            self.array["portion_tokens"] = torch.from_numpy(tokens).pin_memory().to(self.array["singles"].device, non_blocking=True)
+        array = self.array["portion_tokens"]
+        return array, array.shape[0] // 4
 
 
 # ------------------------------------------------------------------ attention
@@ -561,12 +585,12 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
         for name, reach in (("single_tokens", plan.singles), ("few_tokens", plan.multi)):
             if count[name]:
                 _singles(array[name], count[name] // 4, reach, *shape)
-        if count["portion_tokens"]:
+        if (plan.multi_lens > FEW_TOKENS).any():
             if attention_f32.supports(q, q, head_dim, head_dim, n_q_heads, n_kv_heads):
                 for batch in range(len(plan.portion_lens)):
                     _portions(plan, batch, FEW_TOKENS + 1, False, *shape)
             else:       # heads of a size that the tile kernel does not take: token by token
-                _singles(array["portion_tokens"], count["portion_tokens"] // 4, plan.multi, *shape)
+                _singles(*plan.portion_tokens(), plan.multi, *shape)
         return out
     if count["singles"]:
         _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, plan.singles, *shape)

@@ -75,7 +75,10 @@ class NarrowCachePlanner(StepPlanner):
     key = kv4.PLAN_KEY
 
     def plan(self, segments):
-        return kv4.describe_segments(segments.first, segments.starts, segments.lens, segments.rows)
+        return kv4.describe_segments(segments.first, segments.starts, segments.lens, segments.rows, portion_tokens=False)
+
+    def most_ints(self, tokens, requests, context):
+        return kv4.most_ints(tokens, requests, context)
 
     def refresh_single_tokens(self, arrays, segments):
         kv4.refresh_single_tokens(arrays, segments.starts)

@@ -208,11 +208,19 @@ class StepPlanner:
     requests in the same rows, only positions change, and a planner that can overwrite just those
     in its arrays of the previous step (numpy views, edited in place) returns True; returning
     False makes the step function call ``plan`` again.
+
+    ``most_ints`` is for planners whose arrays do not go by tokens and requests alone: a bound on the ints of their arrays, each
+    rounded up to a multiple of 4, for a step of that many tokens of that many requests with contexts of up to ``context``
+    positions.  The step function keeps room for as much beside a few ints a token and a request: a description that needs
+    more memory than there is moves to another buffer, and the recorded steps, which point into this one, are lost.
     """
     key = ""
 
     def plan(self, segments: Segments) -> dict:
         raise NotImplementedError
+
+    def most_ints(self, tokens, requests, context) -> int:
+        return 0
 
     def refresh_single_tokens(self, arrays: dict, segments: Segments) -> bool:
         return False

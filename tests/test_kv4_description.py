@@ -1,0 +1,87 @@
+"""The description of a step over 4-bit pages: how much memory it takes, what it leaves out (no GPU)."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from qwen_inference_lab_b200.cache import CacheManager
+from qwen_inference_lab_b200.engine import StepEntry, StepRunner
+from qwen_inference_lab_b200.kernels import kv4
+from qwen_inference_lab_b200.parts import KVCacheSpec, LayerCall
+from qwen_inference_lab_b200.parts.attention import PagedAttentionPlanner
+
+
+class FakeModel:
+    device, dtype = torch.device("cpu"), torch.bfloat16
+    vocab_size, max_positions = 1000, 40000
+    order = [LayerCall(0)]
+
+    def is_graph_safe(self):
+        return False
+
+    def step_planners(self):
+        return {PagedAttentionPlanner.key: PagedAttentionPlanner()}
+
+
+def make(budget, rows, pages=6000, page_size=16):
+    model = FakeModel()
+    cache = CacheManager([KVCacheSpec(1, 32, bits=4)], num_pages=pages, page_size=page_size, max_requests=rows,
+                         max_context=model.max_positions, dtype=model.dtype, device="cpu")
+    return cache, StepRunner(model, cache, max_step_tokens=budget, use_graphs=False)
+
+
+def test_recorded_steps_outlive_a_prompt_in_chunks():
+    """Two prompts that come in chunks of 64 behind longer and longer contexts: their descriptions fit the memory that recorded steps point to."""
+    cache, runner = make(128, 4)
+    cache.admit("a")
+    cache.admit("b")
+    buffer, runner._graphs["recorded"] = runner._meta_dev, object()
+    for start in range(0, 32000, 64):
+        entries = [StepEntry(name, [1] * 64) for name in "ab"]
+        for entry in entries:
+            cache.ensure(entry.request_id, start + 64)
+        runner._upload(runner._describe(entries).packed)
+        for entry in entries:
+            cache.advance(entry.request_id, start + 64)
+    assert runner._meta_dev is buffer and "recorded" in runner._graphs
+
+
+def test_memory_that_is_too_small_doubles():
+    cache, runner = make(16, 2, pages=40)
+    sizes = []
+    for ints in range(runner._capacity + 1, 20 * runner._capacity, 7):
+        runner._reserve(ints)
+        sizes.append(runner._capacity)
+    assert len(set(sizes)) <= 6
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_no_description_is_beyond_its_bound(seed, monkeypatch):
+    monkeypatch.setattr(kv4, "MOST_READ", 1 << random.Random(seed).choice([6, 9, 16]))
+    rng = random.Random(seed)
+    for _ in range(60):
+        requests, context = rng.randint(1, 40), int(2 ** rng.uniform(0, 15))
+        lens = np.array([min(context, rng.choice([1, 1, 2, 3, 8, 9, 33, 64, 65, 300])) for _ in range(rng.randint(1, requests))])
+        starts = np.array([rng.choice([0, context - n, rng.randint(0, context - n)]) for n in lens])
+        arrays = kv4.describe_segments(np.cumsum(lens) - lens, starts, lens, np.arange(len(lens)), portion_tokens=False)
+        ints = sum(max(4, -(-len(values) // 4) * 4) for values in arrays.values())
+        assert ints <= kv4.most_ints(int(lens.sum()), requests, context)
+
+
+def test_tokens_of_portions_are_described_where_they_are_asked_for():
+    whole = kv4.describe_segments([0, 1, 10], [5, 7, 100], [1, 9, 20], [2, 0, 1])
+    lean = kv4.describe_segments([0, 1, 10], [5, 7, 100], [1, 9, 20], [2, 0, 1], portion_tokens=False)
+    assert set(whole) - set(lean) == {"portion_tokens"} and all((whole[name] == lean[name]).all() for name in lean)
+    expected = [[1 + i, 7 + i, 0, 120] for i in range(9)] + [[10 + i, 100 + i, 1, 120] for i in range(20)]
+    assert whole["portion_tokens"].reshape(-1, 4).tolist() == expected
+    plan = kv4.StepPlan.of_segments([2, 0, 1], [5, 7, 100], [1, 9, 20], "cpu")
+    array, tokens = plan.portion_tokens()
+    assert tokens == 29 and array.view(-1, 4).tolist() == expected
+
+
+def test_steps_do_not_upload_the_tokens_of_portions():
+    cache, runner = make(128, 4, pages=40)
+    cache.admit("a")
+    cache.ensure("a", 64)
+    assert not any(name.endswith("portion_tokens") for name in runner._describe([StepEntry("a", [1] * 64)]).offsets)
