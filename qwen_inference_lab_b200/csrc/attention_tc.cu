@@ -846,12 +846,9 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
     p.error_word = error_word;
     p.trace = trace;
     const int smem = AT_QTILE + AT_STAGES * (AT_KTILE + AT_VTILE) + (int)sizeof(AtShared);
-    static bool configured = false;
-    if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) QIL_REFUSE("attn_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-        configured = true;
-    }
+    static QilPerDevice configured;
+    const cudaError_t e = configured.once(qil_device(), [&] { return cudaFuncSetAttribute(attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (e != cudaSuccess) QIL_REFUSE("attn_tc: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
 #if QIL_KEYS_F16
     qil_launch_chained(attn_tc_kernel, dim3(n_q_heads / p.pack, n_tiles, splits), dim3(AT_THREADS), smem, stream, map_q, map_k, map_v, p, (const int4*)nullptr);
     if (splits > 1) qil_launch_chained(at_join_kernel, dim3(n_q_heads / p.pack, n_tiles, AT_M / 8), dim3(256), 0, stream, p, splits);

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <stdio.h>
+#include "per_device.cuh"
 
 #define QIL_F32 0
 #define QIL_BF16 1
@@ -47,6 +48,11 @@ extern thread_local char qil_error_text[512];
 // soon as every block of this one is past it.  Launched the ordinary way both are no-ops.
 __device__ __forceinline__ void qil_wait_for_producer() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void qil_release_consumer() { asm volatile("griddepcontrol.launch_dependents;\n" ::); }
+
+static inline int qil_device() {
+    int device = -1;
+    return cudaGetDevice(&device) == cudaSuccess ? device : -1;
+}
 
 #include <stdlib.h>
 static inline bool qil_chaining_enabled() {

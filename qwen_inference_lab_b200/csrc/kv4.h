@@ -69,11 +69,3 @@ template <typename Call> static inline Call kv4_call(const void* packed) {
     memcpy(&call, packed, sizeof(Call));
     return call;
 }
-
-// What has to be done once on every device: a flag for each.
-struct Kv4PerDevice {
-    bool flags[64] = {};
-    int device = 0;
-    bool here() { return cudaGetDevice(&device) == cudaSuccess && device < 64 && flags[device]; }
-    void done() { if (device < 64) flags[device] = true; }
-};

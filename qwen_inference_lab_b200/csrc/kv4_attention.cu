@@ -208,12 +208,11 @@ template <typename T, int HEADS, int QUADS>
 static cudaError_t launch_singles(const Kv4Singles& a, int n, cudaStream_t stream) {
     const int share = a.q_heads / a.kv_heads, chunks = (share + HEADS - 1) / HEADS;
     const size_t smem = sizeof(float) * (HEADS * a.dim + WARPS * TILE * HEADS + WARPS * HEADS * a.dim + WARPS * HEADS * 2);
-    static Kv4PerDevice ready;
-    if (!ready.here()) {
-        const cudaError_t e = cudaFuncSetAttribute(kv4_singles_kernel<T, HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-        if (e != cudaSuccess) return e;
-        ready.done();
-    }
+    static QilPerDevice ready;
+    const cudaError_t e = ready.once(qil_device(), [] {
+        return cudaFuncSetAttribute(kv4_singles_kernel<T, HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    });
+    if (e != cudaSuccess) return e;
     return qil_launch_chained(kv4_singles_kernel<T, HEADS, QUADS>, dim3(a.n_spans, a.kv_heads * chunks, n), dim3(32 * WARPS), smem, stream, a);
 }
 

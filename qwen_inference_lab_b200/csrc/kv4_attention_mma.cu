@@ -697,14 +697,12 @@ template <int NT>
 static int launch(const Kv4Few& a, int n, int most_rows, cudaStream_t stream) {
     const int ring = WARPS * STAGES * STAGE_BYTES, rows = WARPS * 8 * D * 4, weights = 8 * NT * a.n_spans * 4;
     const int smem = ring > rows ? (ring > weights ? ring : weights) : (rows > weights ? rows : weights);
-    static Kv4PerDevice configured;
-    if (!configured.here()) {
+    static QilPerDevice configured;
+    const cudaError_t reserved = configured.once(qil_device(), [] {
         const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        if (e != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory: %s", cudaGetErrorString(e));
-        if (cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            QIL_REFUSE("kv4: no clusters of %d blocks", MOST_CLUSTER);
-        configured.done();
-    }
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
+    if (reserved != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory or clusters of %d blocks: %s", MOST_CLUSTER, cudaGetErrorString(reserved));
     const dim3 grid(a.n_spans * ((most_rows + 8 * NT - 1) / (8 * NT)), a.kv_heads, n);
     if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments of %d kv heads", n, a.kv_heads);
     const cudaError_t e = a.clustered ? qil_launch_clusters(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, a.n_spans, stream, a)
