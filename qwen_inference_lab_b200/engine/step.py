@@ -10,7 +10,8 @@ step (qil/engine.py:63-86); here every step is one pass over the layers.
 The batch is described to the kernels by int32 arrays in one device buffer,
 uploaded with a single copy per step (see :class:`StepContext` for the fields).
 Steps made only of single tokens are recorded into CUDA graphs, one per batch
-size and context bucket, and replayed after the metadata upload.
+size, context bucket and what a planner adds (``StepPlanner.recording``), and
+replayed after the metadata upload.
 """
 from __future__ import annotations
 
@@ -292,7 +293,8 @@ class StepRunner:
         bucket = 512
         while bucket < description.max_context:
             bucket *= 2
-        key = (n, bucket)
+        of_planners = (planner.recording(description.segments) for planner in self.planners)
+        key = (n, bucket, *(value for value in of_planners if value is not None))
         record = self._graphs.get(key)
         if record is None:
             ctx = self._context(description, bucket, min_context=bucket // 2 + 1 if bucket > 512 else 1)

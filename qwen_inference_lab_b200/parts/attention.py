@@ -80,6 +80,9 @@ class NarrowCachePlanner(StepPlanner):
     def most_ints(self, tokens, requests, context):
         return kv4.most_ints(tokens, requests, context)
 
+    def recording(self, segments):
+        return kv4.recorded_fill(segments.starts + segments.lens)
+
     def refresh_single_tokens(self, arrays, segments):
         kv4.refresh_single_tokens(arrays, segments.starts)
         return True

@@ -222,6 +222,12 @@ class StepPlanner:
     def most_ints(self, tokens, requests, context) -> int:
         return 0
 
+    def recording(self, segments: Segments):
+        """What a recorded step of single tokens depends on beside their number and the bucket of the longest context (a part that
+        chooses by anything else of the step that is recorded would give a step other bits by what ran before it): steps of
+        another value have a recording of their own.  None: nothing."""
+        return None
+
     def refresh_single_tokens(self, arrays: dict, segments: Segments) -> bool:
         return False
 

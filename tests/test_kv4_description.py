@@ -85,3 +85,22 @@ def test_steps_do_not_upload_the_tokens_of_portions():
     cache.admit("a")
     cache.ensure("a", 64)
     assert not any(name.endswith("portion_tokens") for name in runner._describe([StepEntry("a", [1] * 64)]).offsets)
+
+
+def test_a_recorded_step_goes_by_what_it_is_found_by():
+    """Steps that share a recording (the number of requests, the bucket of the longest context and what the planner says) are planned alike,
+    whichever of them came first."""
+    from types import SimpleNamespace
+    from qwen_inference_lab_b200.parts.attention import NarrowCachePlanner
+    rng, found, planner = random.Random(3), {}, NarrowCachePlanner()
+    for _ in range(400):
+        n, longest = rng.choice([1, 2, 48]), rng.randint(513, 1024)
+        starts = np.array([longest - 1] + [rng.randint(0, int((longest - 1) * rng.random())) for _ in range(n - 1)])
+        lens, rows = np.ones(n, dtype=np.int64), np.arange(n)
+        arrays = kv4.describe_segments(rows, starts, lens, rows)
+        view = SimpleNamespace(array=arrays, count={name: len(values) for name, values in arrays.items()})
+        ctx = SimpleNamespace(plans={kv4.PLAN_KEY: view}, h_seg_start=rows, h_seg_pos0=starts, h_seg_len=lens, h_seg_row=rows, max_context=1024, min_context=513)
+        key = n, planner.recording(SimpleNamespace(starts=starts, lens=lens))
+        found.setdefault(key, set()).add(kv4.StepPlan.of_step(ctx).singles)
+    # one request fills its longest context, 48 drawn so do not
+    assert {(1, 1.0), (2, 1.0), (2, 0.5), (48, 0.5)} <= set(found) and all(len(plans) == 1 for plans in found.values())

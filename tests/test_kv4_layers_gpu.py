@@ -2,9 +2,11 @@
 import pytest
 import torch
 
+from tests import harness
 from tests.plain import kv4_plain
 from tests.test_kv4_engine_gpu import NarrowPart, held
 from tests.test_parts_gpu import fill
+from tests.tiny_configs import TINY_D
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +51,40 @@ def test_float32_portions_of_any_head_size(heads, kv_heads, dim):
         got = torch.cat(rows[name]).double()
         # float32 projections: a code tips now and then and moves an output by a step of one key's share at most
         assert (got - expected).norm() <= 2e-3 * expected.norm(), float((got - expected).norm() / expected.norm())
+
+
+def test_recorded_steps_do_not_remember_who_recorded_them(tmp_path, monkeypatch):
+    """A step whose contexts are nearly as long as each other after one with a single long context, the same bits as without any recording.
+    The rule is replaced by one that shows the difference at these sizes."""
+    from qwen_inference_lab_b200.cache import CacheManager
+    from qwen_inference_lab_b200.engine import StepEntry, StepRunner
+    from qwen_inference_lab_b200.kernels import kv4
+    from qwen_inference_lab_b200.loading import load_model
+    asked = []
+    monkeypatch.setattr(kv4, "_spans", lambda blocks, step_us, size, reach, *rest: asked.append(reach.fill) or (2 if reach.fill > 0.7 else 4))
+    harness.write_folder(TINY_D, 3, tmp_path)
+    model, rows = load_model(tmp_path, device="cuda", dtype=F32), {}
+    tokens = [harness.random_tokens(TINY_D, 520, 90 + i) for i in range(3)]
+    for graphs in (True, False):
+        cache = CacheManager(model.cache_specs(kv_bits=4), num_pages=120, page_size=16, max_requests=3, max_context=model.max_positions, dtype=F32,
+                             device=model.device)
+        runner, done = StepRunner(model, cache, max_step_tokens=1024, use_graphs=graphs), [0, 0, 0]
+        for i in range(3):
+            cache.admit(i)
+
+        def step(sizes, want):
+            entries = []
+            for i, size in enumerate(sizes):
+                if size:
+                    entries.append(StepEntry(i, tokens[i][done[i]:done[i] + size], [size - 1] if want else []))
+                    done[i] += size
+            return runner.run(entries)
+
+        step((500, 20, 20), False)
+        ragged = step((1, 1, 1), True).clone()
+        step((0, 460, 470), False)
+        even = [step((1, 1, 1), True).clone() for _ in range(2)]
+        runner.check()
+        rows[graphs] = torch.stack([ragged, *even])
+        assert len(runner._graphs) == (2 if graphs else 0)
+    assert torch.equal(rows[True], rows[False]) and {1.0, 0.5} <= set(asked)
