@@ -1,4 +1,4 @@
-// Attention of single tokens over pages of 4 bits (layout: kv4.h) on the CUDA cores, float32 or bfloat16 queries, float32 arithmetic.
+// Attention of single tokens over pages of 4 bits (layout: kv4.h) on the CUDA cores, float32 queries and arithmetic.
 //
 //   out = sum_t p_t (m_t + s_t c_t),  p = softmax over the keys t in (pos - window, pos] of scale q . (m_t + s_t c_t)
 //
@@ -14,9 +14,9 @@ static constexpr int WARPS = 4;
 static constexpr int TILE = 32;                // keys a warp takes at a time
 
 struct Kv4Singles {
-    const void* q;                  // T [tokens, q_heads * dim]
+    const float* q;                 // [tokens, q_heads * dim]
     const uint8_t* pages;
-    void* out;
+    float* out;
     const int* info;                // [n][4]: token, position, table row, longest context of the step
     float* part_o;                  // [n][q_heads][n_spans][dim]
     float* part_ml;                 // [n][q_heads][n_spans][2]
@@ -27,7 +27,7 @@ struct Kv4Singles {
 };
 
 // Quads of 4 dimensions a lane owns: QUADS (2 where dim > 128).
-template <typename T, int HEADS, int QUADS>
+template <int HEADS, int QUADS>
 __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Singles a) {
     extern __shared__ float shared[];
     const int dim = a.dim, groups = dim / KV4_GROUP;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
     const int page_size = a.table.page_size;
     for (int i = threadIdx.x; i < HEADS * dim; i += 32 * WARPS) {
         const int h = i / dim;
-        qs[i] = h < heads ? to_f32<T>(reinterpret_cast<const T*>(a.q)[((size_t)token * a.q_heads + head0 + h) * dim + i % dim]) * a.scale_log2 : 0.f;
+        qs[i] = h < heads ? a.q[((size_t)token * a.q_heads + head0 + h) * dim + i % dim] * a.scale_log2 : 0.f;
     }
     __syncthreads();
 
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
             l += ml[(w * HEADS + h) * 2 + 1] * keep;
         }
         if (alone) {
-            reinterpret_cast<T*>(a.out)[((size_t)token * a.q_heads + head0 + h) * dim + d] = from_f32<T>(l == 0.f ? 0.f : sum / l);
+            a.out[((size_t)token * a.q_heads + head0 + h) * dim + d] = l == 0.f ? 0.f : sum / l;
         } else {
             const size_t slot = ((size_t)unit * a.q_heads + head0 + h) * a.n_spans + blockIdx.x;
             a.part_o[slot * dim + d] = sum;
@@ -200,20 +200,20 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_singles_kernel(const Kv4Single
             sum += __ldcg(a.part_o + (slot + s) * dim + d) * keep;
             l += __ldcg(a.part_ml + (slot + s) * 2 + 1) * keep;
         }
-        reinterpret_cast<T*>(a.out)[((size_t)token * a.q_heads + head0 + h) * dim + d] = from_f32<T>(l == 0.f ? 0.f : sum / l);
+        a.out[((size_t)token * a.q_heads + head0 + h) * dim + d] = l == 0.f ? 0.f : sum / l;
     }
 }
 
-template <typename T, int HEADS, int QUADS>
+template <int HEADS, int QUADS>
 static cudaError_t launch_singles(const Kv4Singles& a, int n, cudaStream_t stream) {
     const int share = a.q_heads / a.kv_heads, chunks = (share + HEADS - 1) / HEADS;
     const size_t smem = sizeof(float) * (HEADS * a.dim + WARPS * TILE * HEADS + WARPS * HEADS * a.dim + WARPS * HEADS * 2);
     static QilPerDevice ready;
     const cudaError_t e = ready.once(qil_device(), [] {
-        return cudaFuncSetAttribute(kv4_singles_kernel<T, HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        return cudaFuncSetAttribute(kv4_singles_kernel<HEADS, QUADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     });
     if (e != cudaSuccess) return e;
-    return qil_launch_chained(kv4_singles_kernel<T, HEADS, QUADS>, dim3(a.n_spans, a.kv_heads * chunks, n), dim3(32 * WARPS), smem, stream, a);
+    return qil_launch_chained(kv4_singles_kernel<HEADS, QUADS>, dim3(a.n_spans, a.kv_heads * chunks, n), dim3(32 * WARPS), smem, stream, a);
 }
 
 // Query heads a block takes: the power of two from `share` on, 8 at most (more makes chunks).
@@ -229,29 +229,29 @@ struct Kv4SinglesCall {
     const void* block_table;
     cudaStream_t stream;
     float scale;
-    int n, n_spans, table_height, table_width, q_heads, kv_heads, dim, page_size, num_pages, window, act;
+    int n, n_spans, table_height, table_width, q_heads, kv_heads, dim, page_size, num_pages, window;
 };
 extern "C" int qil_kv4_singles_call_bytes() { return sizeof(Kv4SinglesCall); }
 extern "C" int qil_kv4_singles(const void* packed) {
     const auto [q, pages, out, info, part_o, part_ml, tickets, block_table, stream, scale, n, n_spans, table_height, table_width, q_heads, kv_heads, dim,
-                page_size, num_pages, window, act] = kv4_call<Kv4SinglesCall>(packed);
+                page_size, num_pages, window] = kv4_call<Kv4SinglesCall>(packed);
     if (n <= 0) return 0;
     if (dim <= 0 || dim > KV4_MAX_DIM || dim % KV4_GROUP) QIL_REFUSE("head sizes 32, 64, ..., %d, not %d", KV4_MAX_DIM, dim);
     if (page_size <= 0 || page_size % 8) QIL_REFUSE("pages of a multiple of 8 positions, not %d", page_size);
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || n > 65535 || n_spans < 1) QIL_REFUSE("%d query heads, %d kv heads, %d tokens, %d spans", q_heads, kv_heads, n, n_spans);
-    const Kv4Singles a = {q, (const uint8_t*)pages, out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
+    const Kv4Singles a = {(const float*)q, (const uint8_t*)pages, (float*)out, (const int*)info, (float*)part_o, (float*)part_ml, (int*)tickets,
                           {(const int*)block_table, table_height, table_width, page_size, num_pages}, n_spans, q_heads, kv_heads, dim, window,
                           scale * 1.4426950408889634f};
     const int heads = heads_a_block(q_heads / kv_heads);
     cudaError_t e = cudaSuccess;
 #define KV4_SINGLES(HEADS)                                                                         \
-    if (heads == HEADS) QIL_DISPATCH_1(act, e = dim > 128 ? launch_singles<T, HEADS, 2>(a, n, stream) : launch_singles<T, HEADS, 1>(a, n, stream))
+    if (heads == HEADS) e = dim > 128 ? launch_singles<HEADS, 2>(a, n, stream) : launch_singles<HEADS, 1>(a, n, stream)
     KV4_SINGLES(1);
     KV4_SINGLES(2);
     KV4_SINGLES(4);
     KV4_SINGLES(8);
-    if (e != cudaSuccess) (void)cudaGetLastError();
     if (e != cudaSuccess) {
+        (void)cudaGetLastError();
         snprintf(qil_error_text, sizeof(qil_error_text), "%s", cudaGetErrorString(e));
         return (int)e;
     }

@@ -46,7 +46,7 @@ _few_libs: dict = {}
 
 
 # The C entries' arguments, packed: pointers, then 32-bit numbers (the structs beside the entries), padded to whole pointers.
-_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P11i", "9Pf11i", "9Pf13i"))
+_STORE, _READ, _SPREAD, _SINGLES, _FEW = (Struct(f"@{form}0P") for form in ("Pq10P2f17i", "5P11i", "8P11i", "9Pf10i", "9Pf13i"))
 
 
 def _entry(lib, name, struct, size):
@@ -528,7 +528,7 @@ def _singles(info, n, reach, q, pages, out, block_table, n_q_heads, n_kv_heads, 
         _check(lib, lib.qil_kv4_singles(_SINGLES.pack(
             q.data_ptr(), pages.data_ptr(), out.data_ptr(), info.data_ptr() + 16 * begin, part_o.data_ptr(), part_ml.data_ptr(), tickets.data_ptr(),
             block_table.data_ptr(), _stream(device), scale, some, n_spans, *block_table.shape, n_q_heads, n_kv_heads, head_dim, page_size,
-            pages.shape[0], window, dtype_code(q.dtype))), "kv4.attend (single tokens)")
+            pages.shape[0], window)), "kv4.attend (single tokens)")
 
 
 def _portions(plan, batch, least, beside, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, scale, window, extras):
