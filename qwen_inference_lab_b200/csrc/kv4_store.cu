@@ -348,6 +348,11 @@ __global__ void __launch_bounds__(32 * STORE_WARPS, STORE_BLOCKS) kv4_store_kern
 #pragma unroll
                 for (int i = 0; i < 8; ++i) xp[i] = mine ? to_f32<T>(src[turn.other_of(d0 + i)]) : 0.f;
             }
+            if (a.rot_dims < a.dim) {              // what is not turned has nothing to add: not an infinity times a sine of zero either
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d0 + i >= a.rot_dims) xp[i] = 0.f;
+            }
             float r = 1.f;
             if (a.norm == 1) {
                 float sq = 0.f;
