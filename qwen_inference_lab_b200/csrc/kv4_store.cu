@@ -18,6 +18,7 @@
 //
 // kv4_spread: the rows of a prompt portion's context for the kernel that attends to 16-bit operands (attention_tc.cu with float16 keys):
 // float16 keys and values with a power of two taken out of each per page of 64 and head; where a group of values is NaN, zeros and a mark.
+// An element is off by 2^-11 of itself where it is not smaller than 2^-23 of the largest of its page and head, by 2^-34 of that largest below.
 //
 // kv4_read: rows of requests as ordinary pages [page][2][kv head][slot][d] of float32 or bfloat16.
 #include "kv4.h"
@@ -475,8 +476,7 @@ static constexpr int READ_WARPS = 8;
 template <int I> __device__ __forceinline__ float code_float(unsigned word) {
     return __uint_as_float((word >> (4 * I) & 15u) | 0x4b000000u) - 8388608.f;
 }
-__device__ __forceinline__ void eight_values(unsigned word, unsigned pair, float (&v)[8]) {
-    const float s = kv4_step(pair), m = kv4_base(pair);
+__device__ __forceinline__ void eight_values(unsigned word, float s, float m, float (&v)[8]) {
     v[0] = fmaf(s, code_float<0>(word), m); v[1] = fmaf(s, code_float<1>(word), m);
     v[2] = fmaf(s, code_float<2>(word), m); v[3] = fmaf(s, code_float<3>(word), m);
     v[4] = fmaf(s, code_float<4>(word), m); v[5] = fmaf(s, code_float<5>(word), m);
@@ -511,7 +511,8 @@ kv4_read_kernel(const uint8_t* __restrict__ pages, const Kv4Table table, const i
 #pragma unroll 4
     for (int g = 0; g < groups; ++g) {
         float v[8];
-        eight_values(*reinterpret_cast<const unsigned*>(codes + g * 128), *reinterpret_cast<const unsigned*>(pairs + 4 * g), v);
+        const unsigned pair = *reinterpret_cast<const unsigned*>(pairs + 4 * g);
+        eight_values(*reinterpret_cast<const unsigned*>(codes + g * 128), kv4_step(pair), kv4_base(pair), v);
         store8(dst + g * KV4_GROUP, v);
     }
 }
@@ -549,10 +550,11 @@ struct Kv4Spread {
     int kv_heads, dim, window, least;
     int beside;                     // the kernel before this one attends to the same step's short segments
 };
-// The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.
+// The power of two that brings `largest` into [256, 512) (2^126 at most), and its inverse.  A group's largest value may lie beyond float32,
+// its step being rounded up: then 2^-119 brings it next to 512.
 __device__ __forceinline__ float bring_up(float largest, float& up) {
-    const int e = __float_as_int(largest) >> 23;            // 0 of zero and of the smallest numbers, 255 of infinities
-    const int by = e == 255 ? 0 : min(135 - e, 126);
+    const int e = min(__float_as_int(largest) >> 23, 254);            // 0 of zero and of the smallest numbers
+    const int by = min(135 - e, 126);
     up = __int_as_float((127 + by) << 23);
     return __int_as_float((127 - by) << 23);
 }
@@ -560,9 +562,8 @@ __device__ __forceinline__ unsigned two_halves(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&v);
 }
-__device__ __forceinline__ void store8_half(__half* p, const float (&v)[8], float up) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(two_halves(v[0] * up, v[1] * up), two_halves(v[2] * up, v[3] * up),
-                                              two_halves(v[4] * up, v[5] * up), two_halves(v[6] * up, v[7] * up));
+__device__ __forceinline__ void store8_half(__half* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(two_halves(v[0], v[1]), two_halves(v[2], v[3]), two_halves(v[4], v[5]), two_halves(v[6], v[7]));
 }
 
 // A block: a page of 64 positions of a head's keys or values, a run of 8 a warp (as in kv4_read).
@@ -623,8 +624,8 @@ __global__ void __launch_bounds__(32 * READ_WARPS) kv4_spread_kernel(const Kv4Sp
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
         float v[8];
-        eight_values(codes[g], pairs[g], v);
-        store8_half(dst + g * KV4_GROUP, v, up);
+        eight_values(codes[g], kv4_step(pairs[g]) * up, kv4_base(pairs[g]) * up, v);          // exact, and nothing of it is infinite
+        store8_half(dst + g * KV4_GROUP, v);
     }
     if (plane == 1) {
         if (threadIdx.x == 0) a.value_marks[at] = any;

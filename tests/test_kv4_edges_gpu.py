@@ -26,3 +26,25 @@ def test_infinite_queries_where_nothing_turns(dtype, layout, rot):
     unit = 2.0 ** -8 if dtype == BF16 else 0.0                       # the bounds of the other store tests
     size = expected.where(finite, torch.zeros_like(expected)).abs().amax()
     assert ((got - expected)[finite].abs() <= unit * expected[finite].abs() + 16 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("plane", [0, 1], ids=["keys", "values"])
+def test_groups_whose_values_pass_the_largest_float(plane):
+    """The steps of a group from -3.07e38 to the largest bfloat16 number are rounded up, and its largest value is held as 3.41e38, more than float32
+    has.  A portion's rows in front of it are finite whatever it is.  Held as a value it weighs as what it is in the rows behind it; next to it a
+    page's other values count as nothing (2^-34 of the page's largest at most)."""
+    lens = [50, 70]
+    built = attend_case(8, 2, 64, 16, [0, 0], lens, BF16, seed=31)
+    rows = [[held[i].float() for i in (0, 1)] for held in built["held"]]
+    rows[0][plane][20, 1, 5], rows[0][plane][20, 1, 9] = torch.finfo(BF16).max, -3.0705166702631557e38
+    pages, table, held = plain.build([r[0] for r in rows], [r[1] for r in rows], lens, 16, seed=3)
+    assert held[0][plane].abs().max() > torch.finfo(F32).max
+    built.update(pages=pages, table=table, held=held)
+    out = attend_run(built).cpu().double().view(-1, 8, 64)
+    assert out[:20].isfinite().all() and out[:, :4].isfinite().all() and out[50:].isfinite().all()
+    if plane == 0:
+        return
+    exact, size = plain.attention(built["q"][:50].view(50, 8, 64), *held[0], torch.arange(50), 64 ** -0.5)
+    held_off = (out[20:50] - exact[20:]).abs() <= 8 * 2.0 ** -8 * size[20:] + 2.0 ** -33 * 3.42e38
+    assert held_off[exact[20:].abs() < 3.38e38].all()
+    assert ((out[:20] - exact[:20]).abs() <= 8 * 2.0 ** -8 * size[:20] + 2.0 ** -33 * 3.42e38).all()
