@@ -18,7 +18,7 @@
 //
 // kv4_spread: the rows of a prompt portion's context for the kernel that attends to 16-bit operands (attention_tc.cu with float16 keys):
 // float16 keys and values with a power of two taken out of each per page of 64 and head; where a group of values is NaN, zeros and a mark.
-// An element is off by 2^-11 of itself where it is not smaller than 2^-23 of the largest of its page and head, by 2^-34 of that largest below.
+// An element is off by 2^-11 of itself where it is not smaller than 2^-23 of the largest of its page and head, by 2^-33 of that largest below.
 //
 // kv4_read: rows of requests as ordinary pages [page][2][kv head][slot][d] of float32 or bfloat16.
 #include "kv4.h"

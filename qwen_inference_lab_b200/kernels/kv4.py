@@ -37,6 +37,8 @@ FEW_TOKENS = 8
 #: Positions per page of rows that are read back for a portion, and the most of them at a time (of several portions; a single
 #: one may be longer): 8 heads of 128 in bfloat16 take 4 KB a position.
 READ_PAGE, MOST_READ = 64, 1 << 16
+#: The last position that the kernels count to: a tile behind it is a 32-bit number yet.
+MOST_POSITION = 2**31 - 1 - 1024
 #: Bytes that the memory for those rows grows by at most beyond what is asked for.
 MOST_GROWTH = 256 << 20
 
@@ -370,6 +372,8 @@ class StepPlan:
         rows, starts, lens = (np.asarray(list(v), dtype=np.int64) for v in (rows, starts, lens))
         if not len(rows) == len(starts) == len(lens) or (lens < 1).any() or (starts < 0).any() or (rows < 0).any():
             raise KernelError("kv4.StepPlan: a row, a start and at least one token a segment")
+        if max((starts + lens).max(initial=0), rows.max(initial=0), lens.sum()) > MOST_POSITION:
+            raise KernelError(f"kv4.StepPlan: rows, positions and tokens are 32-bit numbers of up to {MOST_POSITION}")
         arrays = describe_segments(np.cumsum(lens) - lens, starts, lens, rows)
         array = {name: torch.from_numpy(values.astype(np.int32)).to(device) for name, values in arrays.items()}
         return cls(array, {name: len(values) for name, values in arrays.items()}, np.cumsum(lens) - lens, starts, lens, rows,

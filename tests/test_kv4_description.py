@@ -104,3 +104,10 @@ def test_a_recorded_step_goes_by_what_it_is_found_by():
         found.setdefault(key, set()).add(kv4.StepPlan.of_step(ctx).singles)
     # one request fills its longest context, 48 drawn so do not
     assert {(1, 1.0), (2, 1.0), (2, 0.5), (48, 0.5)} <= set(found) and all(len(plans) == 1 for plans in found.values())
+
+
+@pytest.mark.parametrize("rows,starts,lens", [([0], [2**31 - 1], [1]), ([0], [2**32 + 5], [1]), ([2**31], [0], [1]), ([0], [2**31 - 1000], [1]),
+                                              ([0, 2**40], [0, 1], [1, 1])])
+def test_a_plan_of_numbers_beyond_32_bits_is_refused(rows, starts, lens):
+    with pytest.raises(kv4.KernelError, match="32-bit"):
+        kv4.StepPlan.of_segments(rows, starts, lens, "cpu")

@@ -32,7 +32,7 @@ def test_infinite_queries_where_nothing_turns(dtype, layout, rot):
 def test_groups_whose_values_pass_the_largest_float(plane):
     """The steps of a group from -3.07e38 to the largest bfloat16 number are rounded up, and its largest value is held as 3.41e38, more than float32
     has.  A portion's rows in front of it are finite whatever it is.  Held as a value it weighs as what it is in the rows behind it; next to it a
-    page's other values count as nothing (2^-34 of the page's largest at most)."""
+    page's other values count as nothing (2^-33 of the page's largest at most)."""
     lens = [50, 70]
     built = attend_case(8, 2, 64, 16, [0, 0], lens, BF16, seed=31)
     rows = [[held[i].float() for i in (0, 1)] for held in built["held"]]
