@@ -45,8 +45,9 @@ static constexpr int G = D / KV4_GROUP, RUN = 160 * G;
 static constexpr int WARPS = 4, TILE = 32, STAGES = 2;
 static constexpr int STAGE_BYTES = 8 * RUN;            // 4 runs of keys, 4 of values
 static constexpr int MOST_SPANS = 128, MOST_CLUSTER = 16;
-static constexpr int MOST_LIFT = 90;
-static constexpr unsigned TINY_STEP = (127 - 60) << 7; // bits of 2^-60: times 2^MOST_LIFT and a small weight it would leave the products' range
+// The power of two that p carries, p being 256 at most: p 2^118 and p s 2^118 are bfloat16 numbers for steps below 2, and the products with codes
+// counted by 2^-133 are normal float32 numbers down to p s = 2^-111.  Larger steps, of which p s 2^lift stays below 2^127 too, lower it.
+static constexpr int MOST_LIFT = 118;
 static constexpr float NOTHING = -3e38f;               // the largest score of none
 
 struct Kv4Few {
@@ -304,8 +305,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     // largest scores of rows 2 c, 2 c + 1, in their units: what is taken off a score is one of them, and the largest minus itself is zero
     // however large it is
     float most[NT][2];
-    float lift = MOST_LIFT;                       // p s stays below 2^108, so that it overflows nowhere, and far above 2^7
-    unsigned lift_limit = (100 - MOST_LIFT + 128) << 7;                       // a step of that many bits or more (NaN too) asks for another lift
+    float lift = MOST_LIFT;
+    unsigned lift_limit = 128 << 7;                 // a step of that many bits or more (NaN too) asks for another lift
     unsigned marked[NT][2];                     // groups whose values are NaN for them
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
         for (int g = 1; g < G; ++g) largest = max_pairs(largest, pairs[g]);
         const bool partly = (unsigned)(k0 - plain_low) > (unsigned)plain_more || plain_more < 0 || gone;
-        if (partly || __any_sync(0xffffffffu, (largest & 0xffffu) >= lift_limit) || (n == 0 && __all_sync(0xffffffffu, (largest & 0xffffu) < TINY_STEP))) {
+        if (partly || __any_sync(0xffffffffu, (largest & 0xffffu) >= lift_limit)) {
             const int key = k0 + lane;
             const bool inside = key >= span.first && key < span.last && !(gone >> (lane >> 3) & 1);
             unsigned nan = 0;
@@ -417,10 +418,10 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                         if (k0 + j <= pos && (a.window == 0 || k0 + j > pos - a.window)) marked[nt][i] |= groups;
                     }
             }
-            // the lift: by the exponent of the tile's largest step; higher than the usual one only where the first tile's steps are tiny
+            // the lift: by the exponent of the tile's largest step, with room for 2^8 of it
             const int exponent = (int)(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 7) - 127;
-            if (exponent + (int)lift > 100) {
-                const int lower = 92 - exponent;
+            if (exponent + (int)lift > MOST_LIFT) {
+                const int lower = MOST_LIFT - 8 - exponent;
                 const float by = scalbnf(1.f, lower - (int)lift);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -437,13 +438,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                         for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= by;
                 }
                 lift = (float)lower;
-                lift_limit = (unsigned)min(max(228 - lower, 0), 255) << 7;
+                lift_limit = (unsigned)min(MOST_LIFT + 128 - lower, 255) << 7;
                 sink = (unsigned)(127 - lower) << 7 | (unsigned)(127 - lower) << 23;
-            } else if (n == 0 && exponent > -127 && exponent < (int)(TINY_STEP >> 7) - 127) {
-                const int higher = min(92 - exponent, 118);           // p 2^lift stays below 2^127
-                lift = (float)higher;
-                lift_limit = (unsigned)max(228 - higher, 0) << 7;
-                sink = (unsigned)(127 - higher) << 7 | (unsigned)(127 - higher) << 23;
             }
             __syncwarp();
 #pragma unroll

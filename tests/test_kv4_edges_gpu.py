@@ -48,3 +48,26 @@ def test_groups_whose_values_pass_the_largest_float(plane):
     held_off = (out[20:50] - exact[20:]).abs() <= 8 * 2.0 ** -8 * size[20:] + 2.0 ** -33 * 3.42e38
     assert held_off[exact[20:].abs() < 3.38e38].all()
     assert ((out[:20] - exact[:20]).abs() <= 8 * 2.0 ** -8 * size[:20] + 2.0 ** -33 * 3.42e38).all()
+
+
+@pytest.mark.parametrize("before", ["zeros", "unseen", "ordinary"])
+@pytest.mark.parametrize("size", [1e-30, 1e-34])
+def test_tiny_values_behind_others(before, size, monkeypatch):
+    """Values of 1e-30 behind 128 positions of zeros (steps of 0), or of ordinary values that weigh 2^-300, or that weigh much: as exact as
+    others in what they add.  Single and few tokens; a warp takes every fourth tile of 32 positions, so each has other ones first where a context is
+    not cut."""
+    monkeypatch.setattr(kv4(), "_spans", lambda *rule: 1)
+    lens = [1, 4]
+    starts = [500 - n for n in lens]
+    built = attend_case(8, 2, 64, 16, starts, lens, BF16, seed=33)
+    rows = [[held[i].float() for i in (0, 1)] for held in built["held"]]
+    built["q"] = built["q"].float().abs().to(BF16)
+    for keys, values in rows:
+        values[128:] *= size
+        if before == "zeros":
+            values[:128] = 0.0
+        elif before == "unseen":
+            keys[:128] = -keys[:128].abs() - 60.0
+    pages, table, held = plain.build([r[0] for r in rows], [r[1] for r in rows], [500, 500], 16, seed=2)
+    built.update(pages=pages, table=table, held=held)
+    attend_check(built, attend_run(built))
