@@ -356,7 +356,9 @@ class StepPlan:
         """``first``, ``starts``, ``lens`` and ``rows``: the segments' on the host (numpy)."""
         self.array, self.count = array, count
         self._segments = first, starts, lens, rows
-        self.portion_lens = [lens[taken] for taken in portion_batches(starts, lens)]          # of the batches' segments
+        batches = portion_batches(starts, lens)
+        self.portion_lens = [lens[taken] for taken in batches]          # of the batches' segments
+        self.portion_ends = [(starts + lens)[taken] for taken in batches]
         self.multi_lens = lens[lens > 1]
         self.tokens = int(lens.sum())
         self.max_context, self.min_context, self.settled = int(max_context), int(min_context), int(settled)
@@ -364,6 +366,10 @@ class StepPlan:
         # the contexts of single tokens and of longer segments; of recorded steps (single tokens) the longest is a bound
         self.singles = Reach.of(ends[lens == 1], self.max_context if min_context else 0, self.min_context)
         self.multi = Reach.of(ends[lens > 1])
+        # ... and of those that share an array: ``few``, ``few_tokens``, ``portion_tokens``
+        some = lens[lens > 1]
+        self.few, self.few_tokens, self.long = (self.multi if of.all() else Reach.of(ends[lens > 1][of])
+                                                for of in (some <= FEW_ROWS, some <= FEW_TOKENS, some > FEW_TOKENS))
 
     @classmethod
     def of_segments(cls, rows, starts, lens, device):
@@ -541,21 +547,19 @@ def _portions(plan, batch, least, beside, q, pages, out, block_table, n_q_heads,
     array, count = plan.array, plan.count
     segments, n_pages = count[f"b{batch}.read"] // 4, count[f"b{batch}.table"]
     table = array[f"b{batch}.table"][:n_pages].view(segments, n_pages // segments)
+    lens = plan.portion_lens[batch]
+    most = -(-int(plan.portion_ends[batch][lens >= least].max(initial=0)) // READ_PAGE)          # pages of the longest context of those that are meant
+    if not most:
+        return
     size = n_pages * 2 * n_kv_heads * READ_PAGE * head_dim
     if q.dtype == torch.float32:
-        if not count[f"b{batch}.tiles"]:
-            return
         rows = _rows(extras, q.get_device(), 4 * size)[:4 * size].view(torch.float32).view(n_pages, 2, n_kv_heads, READ_PAGE, head_dim)
-        read(pages, block_table, array[f"b{batch}.read"], segments, n_pages // segments * READ_PAGE, rows, n_kv_heads, head_dim, page_size)
+        read(pages, block_table, array[f"b{batch}.read"], segments, most * READ_PAGE, rows, n_kv_heads, head_dim, page_size)
         attention_f32.tiles(q, rows, out, array[f"b{batch}.tiles"], count[f"b{batch}.tiles"] // 4, table, n_q_heads, n_kv_heads, head_dim, READ_PAGE,
                             window, scale)
         return
     pack = attention_tc.keys16_pack(n_q_heads, n_kv_heads)
-    lens = plan.portion_lens[batch]
     groups, n_tiles = n_q_heads // pack, int((-(-lens[lens >= least] // (attention_tc.TILE // pack))).sum())
-    if not n_tiles:
-        return
-    most = n_pages // segments
     splits = attention_tc.keys16_splits(n_tiles * groups, min(most, -(-window // READ_PAGE) + 1) if window else most)
     # rows, what goes with them and partial outputs, in one buffer: every part from a 128-byte boundary on
     heads, parts = n_pages * n_kv_heads, n_tiles * groups * splits * attention_tc.TILE if splits > 1 else 0
@@ -599,7 +603,7 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
     shape = (q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, page_size, float(scale), int(window), extras)
     count, array = plan.count, plan.array
     if q.dtype == torch.float32:
-        for name, reach in (("single_tokens", plan.singles), ("few_tokens", plan.multi)):
+        for name, reach in (("single_tokens", plan.singles), ("few_tokens", plan.few_tokens)):
             if count[name]:
                 _singles(array[name], count[name] // 4, reach, *shape)
         if (plan.multi_lens > FEW_TOKENS).any():
@@ -607,7 +611,7 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
                 for batch in range(len(plan.portion_lens)):
                     _portions(plan, batch, FEW_TOKENS + 1, False, *shape)
             else:       # heads of a size that the tile kernel does not take: token by token
-                _singles(*plan.portion_tokens(), plan.multi, *shape)
+                _singles(*plan.portion_tokens(), plan.long, *shape)
         return out
     if count["singles"]:
         _few(array["singles"], count["singles"] // 8, count["singles"] // 8, 1, plan, plan.singles, *shape)
@@ -618,7 +622,7 @@ def attend(plan, q, pages, out, block_table, n_q_heads, n_kv_heads, head_dim, pa
         most = FEW_ROWS // (n_q_heads // n_kv_heads)           # tokens
         few = plan.multi_lens[plan.multi_lens <= most]
         if len(few):
-            _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, plan.multi, *shape)
+            _few(array["few"], count["few"] // 8, int(plan.multi_lens[plan.multi_lens <= FEW_ROWS].sum()), int(few.max()), plan, plan.few, *shape)
         if len(few) < len(plan.multi_lens):
             for batch in range(len(plan.portion_lens)):
                 _portions(plan, batch, max(most, 1) + 1, batch == 0 and bool(count["singles"] or len(few)), *shape)

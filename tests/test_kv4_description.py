@@ -111,3 +111,13 @@ def test_a_recorded_step_goes_by_what_it_is_found_by():
 def test_a_plan_of_numbers_beyond_32_bits_is_refused(rows, starts, lens):
     with pytest.raises(kv4.KernelError, match="32-bit"):
         kv4.StepPlan.of_segments(rows, starts, lens, "cpu")
+
+
+def test_segments_are_planned_by_their_own_contexts():
+    """Spans of single tokens, of a few and of many go by the contexts of their own kind."""
+    plan = kv4.StepPlan.of_segments(range(5), [9000, 96, 40, 5000, 60], [1, 4, 40, 1000, 20], "cpu")
+    assert plan.singles == (9001, 0, 1.0) and plan.multi.max_context == 6000
+    assert plan.few.max_context == plan.few_tokens.max_context == 100 and plan.few_tokens.fill == 1.0 and plan.few.fill == round(16 * 260 / 3 / 100) / 16
+    assert plan.long == (6000, 0, round(16 * (80 + 6000 + 80) / 3 / 6000) / 16)
+    one = kv4.StepPlan.of_segments([0], [50], [3], "cpu")
+    assert one.few == one.few_tokens == one.multi == (53, 0, 1.0) and one.long == kv4.Reach(1, 0, 1.0)

@@ -99,3 +99,12 @@ def test_contexts_read_back_in_batches(starts, lens, dtype, monkeypatch):
     assert len(plan.portion_lens) > 2
     for window in (0, 250):
         attend_check(built, attend_run(built, window, plan=plan), window)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_portions_are_cut_by_their_own_contexts(dtype, splits):
+    """A fresh prompt beside a few tokens behind a long context: one or two tiles of keys are not cut, whatever lies beside them."""
+    built = attend_case(8, 2, 64, 16, [2400, 0, 2000], [4, 70, 1], dtype, seed=25)
+    out = attend_run(built)
+    assert splits == ([1] if dtype == BF16 else [])
+    attend_check(built, out)
