@@ -381,7 +381,13 @@ class StepPlan:
         if max((starts + lens).max(initial=0), rows.max(initial=0), lens.sum()) > MOST_POSITION:
             raise KernelError(f"kv4.StepPlan: rows, positions and tokens are 32-bit numbers of up to {MOST_POSITION}")
         arrays = describe_segments(np.cumsum(lens) - lens, starts, lens, rows)
-        array = {name: torch.from_numpy(values.astype(np.int32)).to(device) for name, values in arrays.items()}
+        # one upload, every array from a 16-byte boundary on
+        at = np.cumsum([0] + [-(-len(values) // 4) * 4 for values in arrays.values()])
+        packed = np.zeros(int(at[-1]), dtype=np.int32)
+        for begin, values in zip(at, arrays.values()):
+            packed[begin:begin + len(values)] = values
+        there = torch.from_numpy(packed).to(device)
+        array = {name: there[begin:begin + len(values)] for begin, (name, values) in zip(at.tolist(), arrays.items())}
         return cls(array, {name: len(values) for name, values in arrays.items()}, np.cumsum(lens) - lens, starts, lens, rows,
                    int((starts + lens).max(initial=0)))
 

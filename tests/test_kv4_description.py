@@ -121,3 +121,14 @@ def test_segments_are_planned_by_their_own_contexts():
     assert plan.long == (6000, 0, round(16 * (80 + 6000 + 80) / 3 / 6000) / 16)
     one = kv4.StepPlan.of_segments([0], [50], [3], "cpu")
     assert one.few == one.few_tokens == one.multi == (53, 0, 1.0) and one.long == kv4.Reach(1, 0, 1.0)
+
+
+def test_a_plan_of_the_callers_is_one_upload():
+    starts, lens = [9000, 96, 40, 5000, 60, 3], [1, 4, 40, 1001, 20, 1]
+    plan = kv4.StepPlan.of_segments(range(6), starts, lens, "cpu")
+    expected = kv4.describe_segments(np.cumsum(lens) - lens, starts, lens, range(6))
+    assert set(plan.array) == set(expected) and len({array.untyped_storage().data_ptr() for array in plan.array.values()}) == 1
+    for name, values in expected.items():
+        array = plan.array[name]
+        assert array.tolist() == values.tolist() and plan.count[name] == len(values) and array.dtype == torch.int32
+        assert (array.data_ptr() - plan.array["singles"].data_ptr()) % 16 == 0
