@@ -287,6 +287,8 @@ class GroupedQueryAttention(Mixer):
             return "its scores or projections are changed in ways that the kernels over 4-bit pages do not have"
         if self.whole_qk_norm_eps is not None or self.mixes_values:
             return "norms over whole projections and mixed values are not written to 4-bit pages"
+        if not self.scale > 0:
+            return f"the kernels over 4-bit pages scale scores by a positive number, not by {self.scale}"
         return None
 
     takes_norm = True

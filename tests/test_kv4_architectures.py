@@ -29,3 +29,11 @@ def test_every_case_says_yes_or_which_layer_cannot(folder, name):
 
 def test_the_cases_are_there():
     assert len(CASES) == 20 and ACCEPTED <= set(CASES)
+
+
+def test_scales_that_the_kernels_do_not_take():
+    from qwen_inference_lab_b200.parts import GroupedQueryAttention
+    names = {k: k for k in "qkvo"}
+    assert GroupedQueryAttention(64, 4, 2, 32, names=names, scale=0.1).kv_bits_refusal(4) is None
+    for scale in (0.0, -0.2, float("nan")):
+        assert "positive" in GroupedQueryAttention(64, 4, 2, 32, names=names, scale=scale).kv_bits_refusal(4)
