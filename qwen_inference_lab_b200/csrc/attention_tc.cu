@@ -171,7 +171,7 @@ struct AtParams {
     const int4* segments;               // (first token, its position, tokens, block-table row) each, the longest contexts first
     int n_segments, pack;
     int least;                          // segments of fewer tokens are left alone
-    float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum, largest power of their values)
+    float* part_o;                      // splits > 1: [tile][head group][split][128][AT_E], and the rows' (maximum, sum, largest power of their values, 0)
     float4* part_ml;
 #endif
 };
@@ -859,8 +859,9 @@ static int at_launch(const void* q, const void* kv, void* out, const int* tile_i
 }
 
 #if QIL_KEYS_F16
-// The keys of the pages (pages of 64) float16; see AtParams for the rest.  segments int32 [n_segments, 4]; n_tiles: of all segments of at
-// least `least` tokens, 128 / pack tokens each; splits > 1: part_o float32 [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml as many pairs of rows.
+// Keys and values of the pages (pages of 64) float16; see AtParams for the rest.  segments int32 [n_segments, 4]; n_tiles: of all segments of at
+// least `least` tokens, 128 / pack tokens each; splits > 1: float32 part_o [n_tiles * n_q_heads / pack * splits * 128 * AT_E] and part_ml
+// [n_tiles * n_q_heads / pack * splits * 128 * 4].
 extern "C" int qil_attn_tc_prefill_keys16(const void* q, const void* kv, void* out, const int* segments, int n_segments, int least, int n_tiles, int n_tokens,
                                           const int* block_table, int table_stride, int n_q_heads, int n_kv_heads, int num_pages, float scale,
                                           int window, int pack, int splits, const float* factors, const int* value_marks,

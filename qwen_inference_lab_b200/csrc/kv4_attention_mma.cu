@@ -13,15 +13,16 @@
 //            sum_g m_g sum(q_g), the sums as three bfloat16 parts each.  Nothing is rounded but the float32 sums.
 //   softmax  in the accumulators' layout; the maximum moves when it grew by more than 2^8 (p <= 256 until then, exact algebra)
 //   output   O^T = V^T p^T, 16 dimensions x 8 rows x 16 keys an MMA.  p is rounded to bfloat16 and transposed (movmatrix), a group's steps
-//            multiply it once more (p s rounded again), the codes go in as above and p carries the power of two (`lift`, by the
-//            largest step so far).  With two MMAs more
+//            multiply it once more (p s rounded again), the codes go in as above and p carries the power of two (`lift`: 2^118,
+//            less where a step was 2 or more).  With two MMAs more
 //            out = sum (c - 8) (p s) + sum p (m + 8 s):
 //            counted from the middle of a group's range the second rounding acts on |c - 8| steps, about the size of the value itself;
 //            counted from its end it cost 1.5 times the error.  The sum of p comes from the same MMA as the last sum.
 //
-// What bounds it: with few blocks the chain description -> block table -> first tile, with many the instructions a tile takes (an
-// SM issues at most 2 of AND, shift and byte permutation a cycle, 0.47 MMAs).  Other operands cost more: 128 + c or 1 + c / 16 with
-// the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits: 393
+// What bounds it: with few blocks the chain description -> block table -> first tile, with many the chain of a tile (copy, AND and shift, MMA,
+// exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: 44 % of the issue slots and 19 % of the tensor pipe
+// are used, and half of the time a scheduler has nothing to issue.  Instructions still count, since each is a link of that chain.  Other operands
+// cost more of them: 128 + c or 1 + c / 16 with the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits: 393
 // instructions for 16 keys and values of 128 dimensions.
 //
 // The lanes' keys are permuted (row r of a tile of 8: key r / 2 + 4 (r & 1)) so that the two keys that a register of the second product

@@ -42,12 +42,12 @@ def library(head_dim=MOST_DIM, v_dim=None):
     return lib
 
 
-KEYS16_PAGE = 64            # positions per page of float16 keys: a tile's
+KEYS16_PAGE = 64            # positions per page of float16 keys and values: a tile's
 _keys16_libs: dict = {}
 
 
 def keys16_library_name(head_dim):
-    """(name, defines) of the library for float16 queries and keys and bfloat16 values of ``head_dim``."""
+    """(name, defines) of the library for bfloat16 queries (made float16 in the kernel) over float16 keys and values of ``head_dim``."""
     return f"qil_attn_tc_d{head_dim}_keys16", {"QIL_HEAD_DIM": head_dim, "QIL_V_DIM": head_dim, "QIL_KEYS_F16": 1}
 
 
