@@ -12,18 +12,18 @@
 //            that keeps the products normal (and 1/16 where the codes lie higher).  S += s (q . c) in float32, and one MMA more adds
 //            sum_g m_g sum(q_g), the sums as three bfloat16 parts each.  Nothing is rounded but the float32 sums.
 //   softmax  in the accumulators' layout; the maximum moves when it grew by more than 2^8 (p <= 256 until then, exact algebra)
-//   output   O^T = V^T p^T, 16 dimensions x 8 rows x 16 keys an MMA.  p is rounded to bfloat16 and transposed (movmatrix), a group's steps
-//            multiply it once more (p s rounded again), the codes go in as above and p carries the power of two (`lift`: 2^118,
-//            less where a step was 2 or more).  With two MMAs more
-//            out = sum (c - 8) (p s) + sum p (m + 8 s):
-//            counted from the middle of a group's range the second rounding acts on |c - 8| steps, about the size of the value itself;
-//            counted from its end it cost 1.5 times the error.  The sum of p comes from the same MMA as the last sum.
+//   output   O^T = V^T p^T, 16 dimensions x 8 rows x 16 keys an MMA.  The codes go in as above and p carries the power of two (`lift`: 2^118,
+//            less where a step was 2 or more).  A weight is two bfloat16 parts, p and what its rounding left, transposed (movmatrix) one by one;
+//            times a group's steps that is p s rounded, and beside it (rest s + what that rounding left) rounded, which is off by 2^-15 of p s: two
+//            MMAs each.  With two more
+//            out = sum c (p s) + sum p m,
+//            the bases exact; the sum of p comes from the same MMAs as the last sum.  With p and p s rounded once each the result was off by
+//            2.5e-3 of 64 bits where rounding it costs 1.65e-3; now by 1.7e-3, and 8 requests of one token behind 8191 take 30.5 us instead of 28.2.
 //
 // What bounds it: with few blocks the chain description -> block table -> first tile, with many the chain of a tile (copy, AND and shift, MMA,
-// exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: 44 % of the issue slots and 19 % of the tensor pipe
-// are used, and half of the time a scheduler has nothing to issue.  Instructions still count, since each is a link of that chain.  Other operands
-// cost more of them: 128 + c or 1 + c / 16 with the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits: 393
-// instructions for 16 keys and values of 128 dimensions.
+// exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: half of the time a scheduler
+// has nothing to issue.  Instructions still count, since each is a link of that chain.  Other operands
+// cost more of them: 128 + c or 1 + c / 16 with the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits.
 //
 // The lanes' keys are permuted (row r of a tile of 8: key r / 2 + 4 (r & 1)) so that the two keys that a register of the second product
 // pairs are c and c + 4.  Every read of shared memory is free of bank conflicts.
@@ -95,12 +95,12 @@ __device__ __forceinline__ unsigned times_bf16(unsigned a, unsigned b) {
     const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const unsigned*>(&v);
 }
-// m + 8 s of two pairs, rounded once.
-__device__ __forceinline__ unsigned middles(unsigned a, unsigned b) {
-    const unsigned steps = __byte_perm(a, b, 0x5410), bases = __byte_perm(a, b, 0x7632);
-    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&steps), __float2bfloat162_rn(8.f), *reinterpret_cast<const __nv_bfloat162*>(&bases));
+// a b + c of two pairs each, rounded once.
+__device__ __forceinline__ unsigned fma_bf16(unsigned a, unsigned b, unsigned c) {
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&c));
     return *reinterpret_cast<const unsigned*>(&v);
 }
+__device__ __forceinline__ unsigned minus_bf16(unsigned a) { return a ^ 0x80008000u; }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -299,10 +299,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         unit[nt][1] = q_unit[nt * 8 + 2 * c + 1];
     }
 
-    float acc[NT][G][2][4], side[NT][4], less[NT][(G + 1) / 2][4];
-    // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p (m + 8 s)), row 8 sum(p).
-    // less: -8 sum(p s) times 2^(lift - 133) with p s as the first operand: query row r, of two groups the even one in columns 0 .. 3 and
-    // the odd one in 4 .. 7, keys 0 .. 7 in row r and 8 .. 15 in row 8 + r
+    float acc[NT][G][2][4], side[NT][4];
+    // acc times 2^(lift - 133), rows 8 .. 15 2^(lift - 129); side: row g sum(p m), row 8 sum(p)
     // largest scores of rows 2 c, 2 c + 1, in their units: what is taken off a score is one of them, and the largest minus itself is zero
     // however large it is
     float most[NT][2];
@@ -316,11 +314,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[nt][g][0][i] = acc[nt][g][1][i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            side[nt][i] = 0.f;
-#pragma unroll
-            for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] = 0.f;
-        }
+        for (int i = 0; i < 4; ++i) side[nt][i] = 0.f;
         most[nt][0] = most[nt][1] = NOTHING;
         marked[nt][0] = marked[nt][1] = 0u;
     }
@@ -330,7 +324,6 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 
     unsigned sink = (127 - MOST_LIFT) << 7 | (127 - MOST_LIFT) << 23;         // 2^-lift, twice
     const unsigned one = r == 0 ? 0x3f803f80u : 0u;
-    const unsigned eight0 = r < 4 ? 0x80088008u : 0u, eight1 = r < 4 ? 0u : 0x80088008u;      // codes of -8
     // tiles of keys that every row sees begin in [plain_low, plain_low + plain_more]
     const int plain_low = max(span.first, a.window > 0 ? pos_high - a.window + 1 : 0);
     const int plain_more = min(pos_low - TILE + 1, span.last - TILE) - plain_low;
@@ -425,7 +418,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 const int lower = MOST_LIFT - 8 - exponent;
                 const float by = scalbnf(1.f, lower - (int)lift);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -433,11 +426,6 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                             acc[nt][g][0][i] *= by;
                             acc[nt][g][1][i] *= by;
                         }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= by;
-                }
                 lift = (float)lower;
                 lift_limit = (unsigned)min(MOST_LIFT + 128 - lower, 255) << 7;
                 sink = (unsigned)(127 - lower) << 7 | (unsigned)(127 - lower) << 23;
@@ -455,8 +443,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                         if (!seen) sc[u][nt][i] = -INFINITY;
                     }
         }
-        unsigned p0[2][NT], p1[2][NT];
-        // ---- softmax, and p 2^lift as the second product's operand: p0[u][nt], p1: keys c, c + 4 of runs 2 u and 2 u + 1, row 8 nt + r
+        unsigned p[2][NT][2], rest[2][NT][2];
+        // ---- softmax, and p 2^lift as the second product's operand, as two bfloat16 parts: p[u][nt][i]: keys c, c + 4 of run 2 u + i, row 8 nt + r
         float peak[NT][2];
         bool grew = false;
 #pragma unroll
@@ -472,15 +460,15 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 float keep[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float p = peak[nt][i];
-                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 4));
-                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 8));
-                    p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 16));
-                    const bool grow = (p - most[nt][i]) * unit[nt][i] > 8.f;
-                    keep[i] = grow ? fast_exp2((most[nt][i] - p) * unit[nt][i]) : 1.f;
+                    float high = peak[nt][i];
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+                    const bool grow = (high - most[nt][i]) * unit[nt][i] > 8.f;
+                    keep[i] = grow ? fast_exp2((most[nt][i] - high) * unit[nt][i]) : 1.f;
                     if (grow) {
-                        most[nt][i] = p;
-                        far = far || fabsf(p * unit[nt][i]) > 0x1p20f;
+                        most[nt][i] = high;
+                        far = far || fabsf(high * unit[nt][i]) > 0x1p20f;
                     }
                 }
 #pragma unroll
@@ -492,11 +480,6 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                     }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) side[nt][i] *= keep[i & 1];
-                const float even = __shfl_sync(0xffffffffu, keep[0], r >> 1), odd = __shfl_sync(0xffffffffu, keep[1], r >> 1);     // of row r
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int g = 0; g < (G + 1) / 2; ++g) less[nt][g][i] *= r & 1 ? odd : even;
             }
             far = __any_sync(0xffffffffu, far);
         }
@@ -509,8 +492,12 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     e[i] = fast_exp2(far ? fmaf(sc[u][nt][i] - most[nt][i & 1], unit[nt][i & 1], lift) : fmaf(sc[u][nt][i], unit[nt][i & 1], minus[i & 1]));
-                p0[u][nt] = transposed(pack_bf16(e[0], e[1]));
-                p1[u][nt] = transposed(pack_bf16(e[2], e[3]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const unsigned first = pack_bf16(e[2 * i], e[2 * i + 1]);
+                    p[u][nt][i] = transposed(first);
+                    rest[u][nt][i] = transposed(pack_bf16(e[2 * i] - kv4_step(first), e[2 * i + 1] - kv4_base(first)));
+                }
             }
         }
         // ---- output
@@ -527,13 +514,15 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
             load_pairs(run1 + 128 * G + (c + 4) * 4 * G, pb);
 #pragma unroll
             for (int g = 0; g < G; ++g) steps1[g] = __byte_perm(pa[g], pb[g], 0x5410);
-            // row g of the side sums: m + 8 s of group r (rows beyond the groups repeat them and are not looked at)
+            // row g of the side sums: m of group r (rows beyond the groups repeat them and are not looked at)
             const unsigned* at0 = reinterpret_cast<const unsigned*>(run0 + 128 * G + 4 * (r % G));
             const unsigned* at1 = reinterpret_cast<const unsigned*>(run1 + 128 * G + 4 * (r % G));
-            const unsigned middle0 = middles(at0[c * G], at0[(c + 4) * G]), middle1 = middles(at1[c * G], at1[(c + 4) * G]);
+            const unsigned base0 = __byte_perm(at0[c * G], at0[(c + 4) * G], 0x7632), base1 = __byte_perm(at1[c * G], at1[(c + 4) * G], 0x7632);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(side[nt], middle0, one, middle1, one, times_bf16(p0[u][nt], sink), times_bf16(p1[u][nt], sink));
-            unsigned ps[NT][G][2];                                 // p s of the groups
+            for (int nt = 0; nt < NT; ++nt) {
+                mma(side[nt], base0, one, base1, one, times_bf16(p[u][nt][0], sink), times_bf16(p[u][nt][1], sink));
+                mma(side[nt], base0, one, base1, one, times_bf16(rest[u][nt][0], sink), times_bf16(rest[u][nt][1], sink));
+            }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const unsigned char* from0 = run0 + g * 128 + (r >> 1) * 4;
@@ -543,12 +532,14 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 const unsigned xs = x >> 8, ys = y >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    ps[nt][g][0] = times_bf16(p0[u][nt], steps0[g]);
-                    ps[nt][g][1] = times_bf16(p1[u][nt], steps1[g]);
-                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, ps[nt][g][0], ps[nt][g][1]);
-                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, ps[nt][g][0], ps[nt][g][1]);
-                    if (g & 1) mma(less[nt][g / 2], ps[nt][g - 1][0], ps[nt][g - 1][1], ps[nt][g][0], ps[nt][g][1], eight0, eight1);
-                    else if (g == G - 1) mma(less[nt][g / 2], ps[nt][g][0], ps[nt][g][1], 0u, 0u, eight0, eight1);
+                    // p s, what that rounds off (a number of 8 bits) and the rest's product
+                    const unsigned ps0 = times_bf16(p[u][nt][0], steps0[g]), ps1 = times_bf16(p[u][nt][1], steps1[g]);
+                    const unsigned off0 = fma_bf16(rest[u][nt][0], steps0[g], fma_bf16(p[u][nt][0], steps0[g], minus_bf16(ps0)));
+                    const unsigned off1 = fma_bf16(rest[u][nt][1], steps1[g], fma_bf16(p[u][nt][1], steps1[g], minus_bf16(ps1)));
+                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, ps0, ps1);
+                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, ps0, ps1);
+                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, off0, off1);
+                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, off0, off1);
                 }
             }
         }
@@ -575,8 +566,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float middle = __shfl_sync(0xffffffffu, side[nt][i], 4 * g + c), eights = __shfl_sync(0xffffffffu, less[nt][g / 2][0] + less[nt][g / 2][2], 4 * (2 * c + i) + 2 * (g & 1));
-                const float add = (marked[nt][i] >> g & 1) ? __int_as_float(0x7fc00000) : fmaf(eights * 0x1p100f, down, middle);
+                const float bases = __shfl_sync(0xffffffffu, side[nt][i], 4 * g + c);
+                const float add = (marked[nt][i] >> g & 1) ? __int_as_float(0x7fc00000) : bases;
                 float4 o;                                  // 2^133 2^-lift is beyond float32 for a lift below 6: in two steps
                 o.x = fmaf(acc[nt][g][0][i] * 0x1p100f, down, add);
                 o.y = fmaf(acc[nt][g][0][2 + i] * 0x1p96f, down, add);
