@@ -15,10 +15,11 @@
 //   output   O^T = V^T p^T, 16 dimensions x 8 rows x 16 keys an MMA.  The codes go in as above and p carries the power of two (`lift`: 2^118,
 //            less where a step was 2 or more).  A weight is two bfloat16 parts, p and what its rounding left, transposed (movmatrix) one by one;
 //            times a group's steps that is p s rounded, and beside it (rest s + what that rounding left) rounded, which is off by 2^-15 of p s: two
-//            MMAs each.  With two more
+//            MMAs each, or one where a block has 4 rows at most, since the second parts then take the columns that would be empty.  With two (one) more
 //            out = sum c (p s) + sum p m,
 //            the bases exact; the sum of p comes from the same MMAs as the last sum.  With p and p s rounded once each the result was off by
-//            2.5e-3 of 64 bits where rounding it costs 1.65e-3; now by 1.7e-3, and 8 requests of one token behind 8191 take 30.5 us instead of 28.2.
+//            2.5e-3 of 64 bits where rounding it costs 1.65e-3; now by 1.7e-3.  8 requests of one token behind 8191 (4 rows a block) took 28.2 us with
+//            one part, 30.6 with MMAs of their own for the second, 29.5 in the empty columns; 8 of 5 tokens behind 4000 34.3 and 36.4.
 //
 // What bounds it: with few blocks the chain description -> block table -> first tile, with many the chain of a tile (copy, AND and shift, MMA,
 // exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: half of the time a scheduler
@@ -140,8 +141,11 @@ __device__ __forceinline__ void load_pairs(const uint8_t* at, unsigned (&w)[G]) 
 // registers a thread and next to no spills; 2 with all the registers they want stream 4.2 TB/s where 4 stream 4.6, 5 spill (2.7).
 constexpr int blocks_a_sm(int nt) { return nt == 1 ? (D <= 128 ? 4 : 2) : (D <= 64 ? 4 : D <= 128 ? 3 : 1); }
 
-template <int NT>
+// TWICE: up to 4 rows, each in two columns of the MMAs, c and c + 4 alike: the second parts of the products with steps go through the
+// second columns, which are added at the end, and take no MMAs of their own.
+template <int NT, bool TWICE>
 __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(const Kv4Few a) {
+    constexpr int ROWS = TWICE ? 4 : 8 * NT;               // of a block
     extern __shared__ __align__(16) unsigned char shared[];
     __shared__ uint4 q_frag[G * NT][32];                   // the second operand of the scores' MMAs, as the lanes hold it
     __shared__ unsigned q_sums[8 * NT][2 * G];             // of a row's groups: the sums' first two parts, the third
@@ -155,9 +159,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     const int4 info = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z];
     const int4 more = reinterpret_cast<const int4*>(a.info)[2 * blockIdx.z + 1];
     const int first_token = info.x, pos0 = info.y, all_rows = info.z * share, longest = more.y;
-    const int kv = blockIdx.y, my_span = blockIdx.x % a.n_spans, row0 = blockIdx.x / a.n_spans * 8 * NT;
+    const int kv = blockIdx.y, my_span = blockIdx.x % a.n_spans, row0 = blockIdx.x / a.n_spans * ROWS;
     if (row0 >= all_rows || info.z > a.most_tokens) return;            // a segment of more tokens is somebody else's
-    const int rows = min(8 * NT, all_rows - row0);
+    const int rows = min(ROWS, all_rows - row0);
     const int pos_low = pos0 + row0 / share, pos_high = pos0 + (row0 + rows - 1) / share;        // of the block's rows
     const int low = a.window > 0 ? max(0, pos_low + 1 - a.window) : 0;
     const int reach = a.window > 0 ? min(longest, a.window + info.z + TILE - 1) : longest;
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     // ---- queries: a warp a row, a lane 4 neighbouring dimensions (twice beyond 128); times 2^up the row's largest lies in [2^115, 2^116).
     // All of a warp's rows are on their way before the first is looked at: a row takes 0.9 us by itself.
     {
-        constexpr int QUADS = (D + 127) / 128, MINE = 2 * NT;
+        constexpr int QUADS = (D + 127) / 128, MINE = ROWS / WARPS, COPIES = TWICE ? 2 : 1;
         uint2 word[MINE][QUADS];
 #pragma unroll
         for (int j = 0; j < MINE; ++j) {
@@ -262,20 +266,23 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 if (d < D) {
                     // dimension 8 c + i of the group: of register i % 4 of lane (row, c) the lower half, for i >= 4 the upper one; odd ones meet
                     // codes that lie four bits higher
-                    bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + of / 8][(of & 7) * 4 + (lane >> 1 & 3)]) + (lane & 1);
-                    to[0] = __float2bfloat16_rn(q[n][0]);
-                    to[2] = __float2bfloat16_rn(q[n][1] * 0.0625f);
-                    to[4] = __float2bfloat16_rn(q[n][2]);
-                    to[6] = __float2bfloat16_rn(q[n][3] * 0.0625f);
-                    if ((lane & 7) == 0) {
-                        const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
-                        q_sums[of][2 * g] = pack_bf16(first, second);
-                        q_sums[of][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+#pragma unroll
+                    for (int copy = of; copy < of + 4 * COPIES; copy += 4) {
+                        bf16* to = reinterpret_cast<bf16*>(&q_frag[g * NT + copy / 8][(copy & 7) * 4 + (lane >> 1 & 3)]) + (lane & 1);
+                        to[0] = __float2bfloat16_rn(q[n][0]);
+                        to[2] = __float2bfloat16_rn(q[n][1] * 0.0625f);
+                        to[4] = __float2bfloat16_rn(q[n][2]);
+                        to[6] = __float2bfloat16_rn(q[n][3] * 0.0625f);
+                        if ((lane & 7) == 0) {
+                            const float first = __bfloat162float(__float2bfloat16_rn(sum)), second = __bfloat162float(__float2bfloat16_rn(sum - first));
+                            q_sums[copy][2 * g] = pack_bf16(first, second);
+                            q_sums[copy][2 * g + 1] = pack_bf16(sum - first - second, 0.f);
+                        }
                     }
                 }
             }
             // of queries beyond 2^108 a score's unit would be infinite, and infinity times a score of zero
-            if (lane == 0) q_unit[of] = fminf(scalbnf(a.scale_log2, 133 - up), 3e38f);
+            if (lane < COPIES) q_unit[of + 4 * lane] = fminf(scalbnf(a.scale_log2, 133 - up), 3e38f);
         }
     }
     __syncthreads();
@@ -320,7 +327,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     }
     const int order = (r >> 1) + (r & 1) * 4;                     // the key of 8 that row r stands for
     const unsigned half = r & 1 ? 0x7632u : 0x5410u;              // my half of a word of values, of two keys
-    auto row_pos = [&](int nt, int i) { return pos0 + min(row0 + nt * 8 + 2 * c + i, all_rows - 1) / share; };
+    auto row_pos = [&](int nt, int i) { return pos0 + min(row0 + (nt * 8 + 2 * c + i) % ROWS, all_rows - 1) / share; };
+    const unsigned second = r >= 4 ? ~0u : 0u;                   // TWICE: my column is a second one
 
     unsigned sink = (127 - MOST_LIFT) << 7 | (127 - MOST_LIFT) << 23;         // 2^-lift, twice
     const unsigned one = r == 0 ? 0x3f803f80u : 0u;
@@ -520,8 +528,14 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
             const unsigned base0 = __byte_perm(at0[c * G], at0[(c + 4) * G], 0x7632), base1 = __byte_perm(at1[c * G], at1[(c + 4) * G], 0x7632);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                mma(side[nt], base0, one, base1, one, times_bf16(p[u][nt][0], sink), times_bf16(p[u][nt][1], sink));
-                mma(side[nt], base0, one, base1, one, times_bf16(rest[u][nt][0], sink), times_bf16(rest[u][nt][1], sink));
+                if constexpr (TWICE) {
+                    mma(side[nt], base0, one, base1, one, times_bf16(second ? rest[u][nt][0] : p[u][nt][0], sink), times_bf16(second ? rest[u][nt][1] : p[u][nt][1], sink));
+                    rest[u][nt][0] &= second;
+                    rest[u][nt][1] &= second;
+                } else {
+                    mma(side[nt], base0, one, base1, one, times_bf16(p[u][nt][0], sink), times_bf16(p[u][nt][1], sink));
+                    mma(side[nt], base0, one, base1, one, times_bf16(rest[u][nt][0], sink), times_bf16(rest[u][nt][1], sink));
+                }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -532,12 +546,15 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 const unsigned xs = x >> 8, ys = y >> 8;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    // p s, what that rounds off (a number of 8 bits) and the rest's product
+                    // p s, what that rounds off (a number of 8 bits) and the rest's product; TWICE: 0 and 0 in the first columns, which gives p s again
                     const unsigned ps0 = times_bf16(p[u][nt][0], steps0[g]), ps1 = times_bf16(p[u][nt][1], steps1[g]);
-                    const unsigned off0 = fma_bf16(rest[u][nt][0], steps0[g], fma_bf16(p[u][nt][0], steps0[g], minus_bf16(ps0)));
-                    const unsigned off1 = fma_bf16(rest[u][nt][1], steps1[g], fma_bf16(p[u][nt][1], steps1[g], minus_bf16(ps1)));
-                    mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, ps0, ps1);
-                    mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, ps0, ps1);
+                    const unsigned less0 = TWICE ? minus_bf16(ps0) & second : minus_bf16(ps0), less1 = TWICE ? minus_bf16(ps1) & second : minus_bf16(ps1);
+                    const unsigned off0 = fma_bf16(rest[u][nt][0], steps0[g], fma_bf16(p[u][nt][0], steps0[g], less0));
+                    const unsigned off1 = fma_bf16(rest[u][nt][1], steps1[g], fma_bf16(p[u][nt][1], steps1[g], less1));
+                    if constexpr (!TWICE) {
+                        mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, ps0, ps1);
+                        mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, ps0, ps1);
+                    }
                     mma(acc[nt][g][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, off0, off1);
                     mma(acc[nt][g][1], xs & 0x000f000fu, xs & 0x00f000f0u, ys & 0x000f000fu, ys & 0x00f000f0u, off0, off1);
                 }
@@ -552,6 +569,17 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     const bool alone = span.count == 1;
     float* rows_o = reinterpret_cast<float*>(shared);
     const float down = scalbnf(1.f, 33 - (int)lift);
+    if constexpr (TWICE) {                       // the second columns
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            side[0][i] += __shfl_xor_sync(0xffffffffu, side[0][i], 2);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                acc[0][g][0][i] += __shfl_xor_sync(0xffffffffu, acc[0][g][0][i], 2);
+                acc[0][g][1][i] += __shfl_xor_sync(0xffffffffu, acc[0][g][1][i], 2);
+            }
+        }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         if (r == 0) {
@@ -576,7 +604,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
                 *reinterpret_cast<float4*>(rows_o + (warp * 8 + 2 * c + i) * D + g * KV4_GROUP + 4 * r) = o;
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 8 * (D / 4); i += 32 * WARPS) {
+        for (int i = threadIdx.x; i < (TWICE ? 4 : 8) * (D / 4); i += 32 * WARPS) {
             const int of = i / (D / 4), d = i % (D / 4) * 4, row = row0 + nt * 8 + of;
             if (row >= all_rows) break;
             float peak = -INFINITY;
@@ -639,7 +667,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        int* ticket = a.tickets + (size_t)more.x * a.q_heads + kv * all_rows + row0 / (8 * NT);
+        int* ticket = a.tickets + (size_t)more.x * a.q_heads + kv * all_rows + row0 / ROWS;
         last_block = atomicAdd(ticket, 1) == span.count - 1;
         if (last_block) *ticket = 0;
     }
@@ -681,20 +709,21 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_a_sm(NT)) kv4_few_kernel(co
     }
 }
 
-template <int NT>
+template <int NT, bool TWICE>
 static int launch(const Kv4Few& a, int n, int most_rows, cudaStream_t stream) {
     const int ring = WARPS * STAGES * STAGE_BYTES, rows = WARPS * 8 * D * 4, weights = 8 * NT * a.n_spans * 4;
     const int smem = ring > rows ? (ring > weights ? ring : weights) : (rows > weights ? rows : weights);
     static QilPerDevice configured;
     const cudaError_t reserved = configured.once(qil_device(), [] {
-        const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        return e != cudaSuccess ? e : cudaFuncSetAttribute(kv4_few_kernel<NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<NT, TWICE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(kv4_few_kernel<NT, TWICE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (reserved != cudaSuccess) QIL_REFUSE("kv4: cannot reserve shared memory or clusters of %d blocks: %s", MOST_CLUSTER, cudaGetErrorString(reserved));
-    const dim3 grid(a.n_spans * ((most_rows + 8 * NT - 1) / (8 * NT)), a.kv_heads, n);
+    constexpr int ROWS = TWICE ? 4 : 8 * NT;
+    const dim3 grid(a.n_spans * ((most_rows + ROWS - 1) / ROWS), a.kv_heads, n);
     if (grid.y > 65535 || grid.z > 65535) QIL_REFUSE("kv4: %d segments of %d kv heads", n, a.kv_heads);
-    const cudaError_t e = a.clustered ? qil_launch_clusters(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, a.n_spans, stream, a)
-                                      : qil_launch_chained(kv4_few_kernel<NT>, grid, dim3(32 * WARPS), smem, stream, a);
+    const cudaError_t e = a.clustered ? qil_launch_clusters(kv4_few_kernel<NT, TWICE>, grid, dim3(32 * WARPS), smem, a.n_spans, stream, a)
+                                      : qil_launch_chained(kv4_few_kernel<NT, TWICE>, grid, dim3(32 * WARPS), smem, stream, a);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         snprintf(qil_error_text, sizeof(qil_error_text), "%s", cudaGetErrorString(e));
@@ -732,7 +761,7 @@ extern "C" int qil_kv4_few(const void* packed) {
                       settled,
                       scale * 1.4426950408889634f};
     const int rows = most_tokens * (q_heads / kv_heads);
-    if (nt == 1) return launch<1>(a, n, rows, stream);
-    if (nt == 2) return launch<2>(a, n, rows, stream);
+    if (nt == 1) return rows <= 4 ? launch<1, true>(a, n, rows, stream) : launch<1, false>(a, n, rows, stream);
+    if (nt == 2) return launch<2, false>(a, n, rows, stream);
     QIL_REFUSE("kv4: %d tiles of rows a block", nt);
 }

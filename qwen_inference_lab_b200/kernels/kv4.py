@@ -411,7 +411,8 @@ class StepPlan:
 #: Keys that a block of the span kernels takes at a time: a tile of 32 for each of its four warps.
 STEP = 128
 #: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 by its tiles of rows (one B200, a
-#: recorded chain of the kernel; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
+#: recorded chain of the kernel; up to 4 rows 1.11, 1.46, 2.37, 2.46, of 8 1.25, 1.63, 2.51, 2.59, of 16 1.57, 2.02, 3.05, 4.3, with which no number of
+#: spans was better; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
 STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 2.9, 4.0, 4.6)}
 SINGLES_STEP_US = (2.0, 2.4, 3.0)
 #: ... a launch and a block's start, and what a join of spans costs at all and for every span: by tiles of rows through memory, the last
