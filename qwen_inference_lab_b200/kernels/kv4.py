@@ -29,8 +29,8 @@ MOST_DIM = 256
 PLAN_KEY = "kv4_attention"        # the step planner whose arrays ``attend`` reads (``describe_segments`` makes them)
 #: Rows (tokens of a segment times query heads of a kv head) up to which the kernel that walks the codes takes more than one token; of
 #: more the rows are read back once and attended to as 16-bit pages.  Measured (us, this kernel / the other one; 4 heads of 128 a kv head; of
-#: 2, 4, 8, 12, 16 tokens): 8 segments behind 4000 18 / 75, 33 / 77, 55 / 77, 56 / 78, 96 / 79; one 11 / 26, 14 / 26, 18 / 26, 29 / 26, 23 / 26; 8
-#: behind 500 9 / 21, 14 / 21, 18 / 21, 18 / 21, 23 / 24; 4 behind 16000 31 / 138, 58 / 138, 91 / 138, 111 / 138, 149 / 139.
+#: 2, 4, 8, 12, 16 tokens): 8 segments behind 4000 20 / 74, 35 / 74, 59 / 75, 61 / 76, 102 / 77; one 11 / 26, 14 / 26, 18 / 26, 19 / 27, 23 / 27; 8
+#: behind 500 8 / 21, 13 / 21, 17 / 21, 18 / 21, 23 / 23; 4 behind 16000 32 / 134, 61 / 134, 87 / 135, 117 / 135, 151 / 135.
 FEW_ROWS = 48
 #: Tokens of a segment up to which the 32-bit path takes them one by one.
 FEW_TOKENS = 8
@@ -411,8 +411,8 @@ class StepPlan:
 #: Keys that a block of the span kernels takes at a time: a tile of 32 for each of its four warps.
 STEP = 128
 #: What a step takes, in us, with that many blocks on an SM: of the tensor-core kernel for heads of 128 by its tiles of rows (one B200, a
-#: recorded chain of the kernel; up to 4 rows 1.11, 1.46, 2.37, 2.46, of 8 1.25, 1.63, 2.51, 2.59, of 16 1.57, 2.02, 3.05, 4.3, with which no number of
-#: spans was better; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
+#: recorded chain of the kernel; up to 4 rows 1.11, 1.46, 2.37, 2.46, of 8 1.25, 1.63, 2.51, 2.59, of 16 1.57, 2.02, 3.05, 4.3, which choose
+#: other spans for few calls, better and worse ones; a step of another head size takes (0.4 + 0.15 G) of it by G = head_dim / 32), and of the other kernel.
 STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 2.9, 4.0, 4.6)}
 SINGLES_STEP_US = (2.0, 2.4, 3.0)
 #: ... a launch and a block's start, and what a join of spans costs at all and for every span: by tiles of rows through memory, the last
@@ -424,13 +424,14 @@ JOINS_US = {1: (JOIN_US, SPAN_US), 2: (5.0, 0.2)}
 CLUSTER_SPAN_US = 0.14
 #: Spans that are a cluster where all of them run at the same time, by tiles of rows.  Clusters of other sizes are placed badly (8 requests behind 8191,
 #: 9 spans: 27.4 through memory, 37.6 as clusters; one request and 16 spans 11.3 / 12.6), and so are clusters of a second wave (16
-#: requests behind 8191 and 8 spans 51.6 / 52.8).
+#: requests behind 8191 and 8 spans 51.6 / 52.8).  16 blocks have to fit into one group of SMs, which leaves places empty: of one request of 12 tokens behind 4000
+#: (24 clusters of 16, 3 blocks an SM) some come second, 27.6 as 16 spans and 18.8 as 8; of 5 tokens (16 clusters) 17.2 and 17.7.
 CLUSTERS = {1: (2, 4, 8), 2: (2, 4, 8, 16)}
-SMS = 148
+SMS, SMS_FOR_16 = 148, 100
 
 
 def _clustered(n, blocks_per_span, step_us, clusters) -> bool:
-    return n in clusters and blocks_per_span * n <= SMS * len(step_us)
+    return n in clusters and blocks_per_span * n <= (SMS_FOR_16 if n == 16 else SMS) * len(step_us)
 
 
 @functools.lru_cache(maxsize=4096)

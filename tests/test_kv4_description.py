@@ -132,3 +132,11 @@ def test_a_plan_of_the_callers_is_one_upload():
         array = plan.array[name]
         assert array.tolist() == values.tolist() and plan.count[name] == len(values) and array.dtype == torch.int32
         assert (array.data_ptr() - plan.array["singles"].data_ptr()) % 16 == 0
+
+
+def test_three_tiles_of_rows_are_not_cut_into_clusters_of_sixteen():
+    """One request of 12 tokens with 4 heads on a key: 24 clusters of 16 blocks do not run at the same time."""
+    reach = kv4.Reach(4012, 0, 1.0)
+    spans = lambda blocks: kv4._spans(blocks, kv4.STEP_US[2][:3], 1.0, reach, 0, 128, kv4.JOINS_US[2], kv4.CLUSTERS[2])
+    assert spans(24) == 8 and kv4._clustered(8, 24, kv4.STEP_US[2][:3], kv4.CLUSTERS[2])
+    assert not kv4._clustered(16, 24, kv4.STEP_US[2][:3], kv4.CLUSTERS[2]) and kv4._clustered(16, 16, kv4.STEP_US[2][:3], kv4.CLUSTERS[2])
