@@ -22,8 +22,8 @@
 //            one part, 30.6 with MMAs of their own for the second, 29.5 in the empty columns; 8 of 5 tokens behind 4000 34.3 and 36.4.
 //
 // What bounds it: with few blocks the chain description -> block table -> first tile, with many the chain of a tile (copy, AND and shift, MMA,
-// exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: half of the time a scheduler
-// has nothing to issue.  Instructions still count, since each is a link of that chain.  Other operands
+// exponential, transposition, MMA), of which an SM has 16 warps with one tile each under way: 44 % of the issue slots
+// and 16 % of the tensor pipe are used.  Instructions still count, since each is a link of that chain.  Other operands
 // cost more of them: 128 + c or 1 + c / 16 with the offset taken off afterwards, and e4m3 (a code's byte is code 2^-9), whose MMAs are taken apart into two of 16 bits.
 //
 // The lanes' keys are permuted (row r of a tile of 8: key r / 2 + 4 (r & 1)) so that the two keys that a register of the second product
@@ -138,7 +138,8 @@ __device__ __forceinline__ void load_pairs(const uint8_t* at, unsigned (&w)[G]) 
 }
 
 // How many blocks of this kernel share an SM: what the launch bounds ask for.  Of heads of 128 and one tile of rows 4 blocks have 128
-// registers a thread and next to no spills; 2 with all the registers they want stream 4.2 TB/s where 4 stream 4.6, 5 spill (2.7).
+// registers a thread and next to no spills; 2 with all the registers they want stream 4.2 TB/s where 4 stream 4.6, 5 spill (2.7; with
+// weights of one part each).
 constexpr int blocks_a_sm(int nt) { return nt == 1 ? (D <= 128 ? 4 : 2) : (D <= 64 ? 4 : D <= 128 ? 3 : 1); }
 
 // TWICE: up to 4 rows, each in two columns of the MMAs, c and c + 4 alike: the second parts of the products with steps go through the

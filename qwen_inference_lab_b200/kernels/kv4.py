@@ -326,8 +326,8 @@ def recorded_fill(ends) -> float:
     """How full a recorded step of single tokens takes its contexts ``ends`` to be, as a part of the longest: all of it, or half.  Two
     values, so that a number of requests has two recordings a bucket of the longest context, and a step's is one that was made for steps
     like it.  Measured (us, spans for full ones / for half of it; 32 heads of 128 over 8; contexts all of the longest, spread evenly up to it, all but one a
-    sixteenth of it): 48 requests, 16384 206 / 217, 140 / 131, 71 / 50; 64, 8192 152 / 164, 133 / 103, 92 / 26; 16, 8192 46 / 52, 45 / 36, 28 / 20; 128, 2048
-    75 / 110, 60 / 71, 26 / 20."""
+    sixteenth of it): 48 requests, 16384 221 / 221, 151 / 139, 73 / 53; 64, 8192 166 / 170, 142 / 106, 87 / 27; 16, 8192 49 / 54, 48 / 38, 29 / 21; 128, 2048
+    79 / 111, 62 / 72, 28 / 20."""
     return 1.0 if 4 * float(ends.mean()) >= 3 * float(ends.max()) else 0.5
 
 
@@ -416,15 +416,15 @@ STEP = 128
 STEP_US = {1: (1.18, 1.58, 2.5, 2.6), 2: (1.65, 2.9, 4.0, 4.6)}
 SINGLES_STEP_US = (2.0, 2.4, 3.0)
 #: ... a launch and a block's start, and what a join of spans costs at all and for every span: by tiles of rows through memory, the last
-#: block to arrive, and as a cluster of blocks.  Measured (us, memory / cluster): one request of 2 tokens behind 2043 and 2, 4, 8, 16 spans 17.5 /
-#: 14.6, 14.4 / 10.5, 10.9 / 8.6, 10.6 / 8.9, of 4 tokens 26.8 / 21.2, 21.9 / 14.8, 17.2 / 12.1, 16.8 / 12.3; 8 requests of one token behind 8191
-#: and 8 spans 28.2 / 26.8.
+#: block to arrive, and as a cluster of blocks.  Measured (us, memory / cluster): one request of 2 tokens behind 2043 and 2, 4, 8, 16 spans 18.3 /
+#: 15.4, 14.7 / 10.6, 11.0 / 8.6, 10.2 / 8.8, of 4 tokens 26.8 / 21.3, 21.8 / 14.7, 17.2 / 11.9, 16.8 / 11.9; 8 requests of one token behind 8191
+#: and 8 spans 29.2 / 28.4.
 START_US, JOIN_US, SPAN_US = tuning.KV4_START_US, tuning.KV4_JOIN_US, tuning.KV4_SPAN_US
 JOINS_US = {1: (JOIN_US, SPAN_US), 2: (5.0, 0.2)}
 CLUSTER_SPAN_US = 0.14
 #: Spans that are a cluster where all of them run at the same time, by tiles of rows.  Clusters of other sizes are placed badly (8 requests behind 8191,
-#: 9 spans: 27.4 through memory, 37.6 as clusters; one request and 16 spans 11.3 / 12.6), and so are clusters of a second wave (16
-#: requests behind 8191 and 8 spans 51.6 / 52.8).  16 blocks have to fit into one group of SMs, which leaves places empty: of one request of 12 tokens behind 4000
+#: 9 spans: 28.1 through memory, 37.0 as clusters; one request and 16 spans 10.9 / 12.7), and so are clusters of a second wave (24
+#: requests behind 4095 and 3 spans 37.2 / 45.9).  16 blocks have to fit into one group of SMs, which leaves places empty: of one request of 12 tokens behind 4000
 #: (24 clusters of 16, 3 blocks an SM) some come second, 27.6 as 16 spans and 18.8 as 8; of 5 tokens (16 clusters) 17.2 and 17.7.
 CLUSTERS = {1: (2, 4, 8), 2: (2, 4, 8, 16)}
 SMS, SMS_FOR_16 = 148, 100
@@ -437,7 +437,7 @@ def _clustered(n, blocks_per_span, step_us, clusters) -> bool:
 @functools.lru_cache(maxsize=4096)
 def _plan(blocks_per_span, step_us, size, lo, hi, most, join, clusters, fill) -> int:
     """The number of spans that costs least per step of keys at both ends of [lo, hi] steps of longest context, of which the contexts have
-    ``fill`` on the average: half a span more than that share of the spans holds something (48 requests of up to 16384: 3 spans 169 us, 9 145)."""
+    ``fill`` on the average: half a span more than that share of the spans holds something (48 requests spread evenly up to 16384: 3 spans 151 us, 10 137)."""
     full = SMS * len(step_us)
 
     def cost(steps, n):
